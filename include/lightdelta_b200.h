@@ -48,7 +48,9 @@ extern "C" {
 #define LD_FAULT_WAIT_TIMEOUT 0x20u       /* a bounded in-kernel wait expired: the CTA stored nothing more and returned */
 #define LD_FAULT_VERIFY_DRAFTS 0x40u      /* greedy_verify: a request has more drafts than steps */
 #define LD_FAULT_VERIFY_RANGE 0x80u       /* greedy_verify: metadata points outside the logits or token ids */
-#define LD_FAULT_CONV_SLOT_RANGE 0x100u   /* conv update: a conv-state slot index >= n_conv_slots */
+#define LD_FAULT_CONV_SLOT_RANGE 0x100u   /* conv update, conv prefill: a conv-state slot index >= n_conv_slots */
+#define LD_FAULT_TABLE_BLOCKS 0x200u      /* prompt path: a request's blocks do not fit its table row or the free list */
+#define LD_FAULT_TABLE_LENGTHS 0x400u     /* request_tables: a negative length, or more tokens than the outputs hold */
 
 /* Head dimension handled by every kernel (K = V). */
 #define LD_HEAD_DIM 128
@@ -58,6 +60,9 @@ extern "C" {
 /* Largest number of draft tokens per request in ld_greedy_verify (its sampled rows hold
  * num_speculative_steps + 1 tokens). */
 #define LD_MAX_VERIFY_STEPS 7
+
+/* Tokens per chunk of ld_prefill; block sizes of the prompt path's tables are multiples of it there. */
+#define LD_PREFILL_CHUNK 64
 
 /* Message of the last LD_ERR_* returned on the calling thread ("" if none). */
 const char* ld_last_error(void);
@@ -333,6 +338,101 @@ int ld_decode_packed_noalloc(const void* qkv, int64_t qkv_row_stride, const void
                              int64_t slot_stride, const void* gate, int64_t gate_row_stride, const void* weight,
                              int weight_dtype, void* out, int64_t n_tokens, int64_t num_k_heads,
                              int64_t num_v_heads, float eps, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------------------------
+ * The prompt path: block tables, causal convolution and gated delta rule attention over whole
+ * prompts (or pieces of prompts).  No counterpart in the reference, which leaves prompts to its
+ * host engine's kernels (python/lightdelta/integration/vllm_layer.py:93-135).
+ *
+ * A request r brings the tokens [cu[r], cu[r+1]) and has context[r] tokens behind it.  Row r of
+ * `table` (int32, `table_width` blocks, rows table_row_stride apart) names one slot per block of
+ * `block_size` token positions.  Slot table[r, b] holds the state (and the convolution window)
+ * after the last token of block b, or after the request's last token so far if that lies in b:
+ *   - a request with context[r] > 0 starts from slot table[r, (context[r] - 1) / block_size];
+ *   - one with context[r] == 0 starts from nothing (its slots are not read);
+ *   - wherever a block or the request ends, slot table[r, block] is written if it is > 0.
+ * Source and first destination are the same slot when context[r] is inside a block: it is read
+ * before it is written.  A slot that a call writes must be named by no other block that the call
+ * reads or writes, of the same request or another.  A caller that keeps one slot per request
+ * passes rows of one block with a block_size above its longest prompt, or 0 for the blocks whose
+ * states it does not want.
+ * ---------------------------------------------------------------------------------------------
+ */
+
+/*
+ * Gated delta rule attention over prompts, with ld_decode's mathematics: outputs and states are
+ * those of ld_decode called once per token, up to rounding (the recurrence's outputs stay fp32
+ * until the gated norm, and sums run over chunks of LD_PREFILL_CHUNK tokens).
+ *
+ * Activations, a_log, dt_bias, gate, weight, out: as in ld_decode.  state: fp32 or bf16
+ * (state_dtype) [n_slots, HV, 128, 128] pool, slot stride in elements (a multiple of 4 or 8); the
+ * recurrence runs in fp32 and each stored state is rounded to the pool's type.
+ * block_size is a positive multiple of LD_PREFILL_CHUNK.
+ *
+ * A request with no tokens writes nothing, and rows of `out` that belong to no request are left
+ * as they are.  A request with context[r] > 0 whose source slot is <= 0 or >= n_slots, with
+ * context[r] < 0, or whose blocks go past table_width gets zero outputs and no state writes
+ * (LD_FAULT_DECODE_SLOT_RANGE / LD_FAULT_TABLE_BLOCKS; a null source sets no bit); tokens outside
+ * [0, n_tokens) skip the request (LD_FAULT_DECODE_TOKENS).  A destination slot >= n_slots is not
+ * written (LD_FAULT_DECODE_SLOT_RANGE).  A token whose inputs are not finite spoils its request
+ * from the start of its chunk (positions are cut into chunks at multiples of LD_PREFILL_CHUNK).
+ */
+int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a_row_stride, const void* b,
+               int64_t b_row_stride, const float* a_log, const void* dt_bias, int dt_bias_dtype, const int32_t* table,
+               int64_t table_row_stride, int64_t table_width, int64_t block_size, const int32_t* context,
+               const int32_t* cu, int64_t n_requests, void* state, int state_dtype, int64_t n_slots,
+               int64_t slot_stride, const void* gate, int64_t gate_row_stride, const void* weight, int weight_dtype,
+               void* out, int64_t n_tokens, int64_t num_k_heads, int64_t num_v_heads, float eps, void* stream);
+
+/*
+ * The causal conv1d of the q, k, v channels over prompts, in front of ld_prefill:
+ *   y_t = silu(bias + sum_j W[:, j] * x[t - conv_width + 1 + j]), fp32 products and sums, rounded to
+ *   bf16 once, with the inputs before a request's first token taken from positions
+ *   [0, conv_width - 1) of its source slot (zeros when context[r] == 0).  Wherever a block or the
+ *   request ends, the last conv_width - 1 inputs become positions [0, conv_width - 1) of the
+ *   block's slot (its other positions stay), where ld_conv_update with accepted = 1 continues.
+ *
+ * x: [n_tokens, dim] bf16, rows x_row_stride apart.  out: [n_tokens, dim] bf16 contiguous, which
+ *   must not overlap x (nor the rows between x's: the two extents are compared).
+ * conv_state, conv_weight, conv_bias, conv_width: as in ld_conv_update, conv_state_len >=
+ *   conv_width - 1.  block_size >= 1 (ld_prefill needs a multiple of LD_PREFILL_CHUNK).
+ * Rows of no request are left as they are.  Requests that ld_prefill would not run are not run
+ * here either: zero outputs and no windows written (LD_FAULT_CONV_SLOT_RANGE /
+ * LD_FAULT_TABLE_BLOCKS), or skipped where their tokens are out of range (LD_FAULT_DECODE_TOKENS).
+ */
+int ld_conv_prefill(const void* x, int64_t x_row_stride, int64_t n_tokens, int64_t dim, void* conv_state,
+                    int64_t n_conv_slots, int64_t conv_slot_stride, int64_t conv_dim_stride, int64_t conv_pos_stride,
+                    int64_t conv_state_len, const void* conv_weight, const void* conv_bias, int64_t conv_width,
+                    const int32_t* table, int64_t table_row_stride, int64_t table_width, int64_t block_size,
+                    const int32_t* context, const int32_t* cu, int64_t n_requests, void* out, void* stream);
+
+/*
+ * Token offsets, block table, positions and cache slots of a batch from its request lengths, on
+ * the device.  query_lens[r] new tokens follow context[r] held ones (int32, n_requests each):
+ *   cu[0..n_requests]   prefix sums of query_lens (int32);
+ *   table[r, b]         for the blocks b that the new tokens begin, ceil(context/block_size) <= b <
+ *                       ceil((context + query)/block_size): the next entry of free_blocks, requests
+ *                       in order, blocks in order; every other entry stays;
+ *   positions[i]        context[r] + i - cu[r] for token i of request r (int64);
+ *   slot_map[i]         table[r, position / block_size] * block_size + position % block_size (int64);
+ *   state_slots[r]      (slot of the block of r's last new token, slot of the block of its last held
+ *                       token), 0 where there is no such token.  With them as `indices` and
+ *                       accepted = 2, ld_decode takes a one-token request from its held state to its
+ *                       new block's slot, across a block's end too;
+ *   used[0]             free blocks taken, over all requests.
+ * positions and slot_map hold n_tokens entries; those behind the last token are -1.  A token whose
+ * block is null (<= 0) has slot -1.
+ * Where free_blocks runs out the entries are 0, and blocks past table_width are not written
+ * (LD_FAULT_TABLE_BLOCKS; used[0] still counts them).  Negative lengths count as 0 and tokens
+ * behind n_tokens are left out (LD_FAULT_TABLE_LENGTHS).
+ * block_size is 1 through 2^30; any block size is accepted, ld_prefill needs multiples of
+ * LD_PREFILL_CHUNK.
+ */
+int ld_request_tables(const int32_t* query_lens, const int32_t* context, int64_t n_requests,
+                      const int32_t* free_blocks, int64_t n_free, int32_t* table, int64_t table_row_stride,
+                      int64_t table_width, int64_t block_size, int32_t* cu, int64_t* positions, int64_t* slot_map,
+                      int64_t n_tokens, int32_t* state_slots, int32_t* used, void* stream);
 
 #ifdef __cplusplus
 }

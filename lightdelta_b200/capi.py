@@ -30,6 +30,9 @@ LD_FAULT_WAIT_TIMEOUT = 0x20
 LD_FAULT_VERIFY_DRAFTS = 0x40
 LD_FAULT_VERIFY_RANGE = 0x80
 LD_FAULT_CONV_SLOT_RANGE = 0x100
+LD_FAULT_TABLE_BLOCKS = 0x200
+LD_FAULT_TABLE_LENGTHS = 0x400
+PREFILL_CHUNK = 64
 HEAD_DIM = 128
 MAX_WIDTH = 4
 MAX_VERIFY_STEPS = 7
@@ -86,6 +89,16 @@ def lib() -> ctypes.CDLL:
     handle.ld_conv_decode.restype = i32
     handle.ld_conv_update.argtypes = [p, i64, i64, i64, p, i64, i64, i64, i64, i64, p, p, i64, p, i64, p, p, i64, i64, p]
     handle.ld_conv_update.restype = i32
+    handle.ld_request_tables.argtypes = [p, p, i64, p, i64, p, i64, i64, i64, p, p, p, i64, p, p, p]
+    handle.ld_request_tables.restype = i32
+    handle.ld_conv_prefill.argtypes = [p, i64, i64, i64, p, i64, i64, i64, i64, i64, p, p, i64, p, i64, i64, i64, p, p,
+                                       i64, p, p]
+    handle.ld_conv_prefill.restype = i32
+    handle.ld_prefill.argtypes = [
+        p, i64, p, i64, p, i64, p, p, i32, p, i64, i64, i64, p, p, i64, p, i32, i64, i64, p, i64, p, i32, p, i64, i64,
+        i64, f32, p,
+    ]
+    handle.ld_prefill.restype = i32
     handle.ld_programmatic_launch.argtypes = [i32]
     handle.ld_programmatic_launch.restype = i32
     handle.ld_decode_wait_test.argtypes = [i64, i32]
@@ -252,6 +265,41 @@ def conv_update(x, conv_state, conv_weight, conv_bias, slots, accepted, cu, max_
         None if conv_bias is None else conv_bias.data_ptr(), w.shape[1], slots.data_ptr(), slots.stride(0),
         None if accepted is None else accepted.data_ptr(), cu.data_ptr(), slots.numel(), int(max_tokens),
         _stream(x, stream),
+    ))
+
+
+def request_tables(query_lens, context, free_blocks, table, cu, positions, slot_map, state_slots, used, block_size,
+                   stream=None):
+    """ld_request_tables on torch tensors laid out as torch.ops.lightdelta.request_tables expects."""
+    check(lib().ld_request_tables(
+        query_lens.data_ptr(), context.data_ptr(), query_lens.numel(), free_blocks.data_ptr(), free_blocks.numel(),
+        table.data_ptr(), table.stride(0), table.shape[1], int(block_size), cu.data_ptr(), positions.data_ptr(),
+        slot_map.data_ptr(), positions.numel(), state_slots.data_ptr(), used.data_ptr(), _stream(query_lens, stream),
+    ))
+
+
+def conv_prefill(x, conv_state, conv_weight, conv_bias, table, context, cu, out, block_size, stream=None):
+    """ld_conv_prefill on torch tensors laid out as torch.ops.lightdelta.conv_prefill expects."""
+    w = conv_weight.reshape(conv_weight.shape[0], -1)
+    check(lib().ld_conv_prefill(
+        x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], conv_state.data_ptr(), conv_state.shape[0],
+        conv_state.stride(0), conv_state.stride(1), conv_state.stride(2), conv_state.shape[2], w.data_ptr(),
+        None if conv_bias is None else conv_bias.data_ptr(), w.shape[1], table.data_ptr(), table.stride(0),
+        table.shape[1], int(block_size), context.data_ptr(), cu.data_ptr(), context.numel(), out.data_ptr(),
+        _stream(x, stream),
+    ))
+
+
+def prefill(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, out, block_size, eps=1e-6, stream=None):
+    """ld_prefill on torch tensors laid out as torch.ops.lightdelta.prefill expects."""
+    hv = state.shape[1]
+    h = (qkv.shape[1] // HEAD_DIM - hv) // 2
+    check(lib().ld_prefill(
+        qkv.data_ptr(), qkv.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_log.data_ptr(),
+        dt_bias.data_ptr(), _dtype_code(dt_bias), table.data_ptr(), table.stride(0), table.shape[1], int(block_size),
+        context.data_ptr(), cu.data_ptr(), context.numel(), state.data_ptr(), _dtype_code(state), state.shape[0],
+        state.stride(0), gate.data_ptr(), gate.stride(0), weight.data_ptr(), _dtype_code(weight), out.data_ptr(),
+        qkv.shape[0], h, hv, float(eps), _stream(qkv, stream),
     ))
 
 

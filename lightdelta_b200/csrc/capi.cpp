@@ -45,7 +45,7 @@ extern "C" int ld_programmatic_launch(int enable) {
 
 extern "C" int ld_fault_flags(uint32_t* flags, int clear) {
   if (flags == nullptr) return ldb::set_error(LD_ERR_INVALID, "ld_fault_flags: flags is NULL");
-  uint32_t decode = 0, state_io = 0, verify = 0, conv = 0;
+  uint32_t decode = 0, state_io = 0, verify = 0, conv = 0, prefill = 0, conv_prefill = 0, tables = 0;
   int rc = ldb::decode_faults(&decode, clear);
   if (rc != LD_OK) return rc;
   rc = ldb::state_io_faults(&state_io, clear);
@@ -54,6 +54,12 @@ extern "C" int ld_fault_flags(uint32_t* flags, int clear) {
   if (rc != LD_OK) return rc;
   rc = ldb::conv_faults(&conv, clear);
   if (rc != LD_OK) return rc;
-  *flags = decode | state_io | verify | conv;
+  rc = ldb::prefill_faults(&prefill, clear);
+  if (rc != LD_OK) return rc;
+  rc = ldb::conv_prefill_faults(&conv_prefill, clear);
+  if (rc != LD_OK) return rc;
+  rc = ldb::tables_faults(&tables, clear);
+  if (rc != LD_OK) return rc;
+  *flags = decode | state_io | verify | conv | prefill | conv_prefill | tables;
   return ldb::ok();
 }

@@ -1,0 +1,374 @@
+// Causal depthwise conv1d and silu over whole prompts: the step between the projection and ld_prefill.
+//
+//   y_t = silu(bias + sum_{j<w} W[:, j] x_{t-w+1+j}),  x before the request's first token taken from the
+//   convolution window in its source slot (zeros without context); wherever a block or the request ends,
+//   the last w - 1 inputs become the window in the block's slot, positions 0 .. w - 2, which is where
+//   ld_conv_update with accepted = 1 (and the next piece of the prompt) finds them.
+//
+// Products and sums are fp32, rounded once at the end.  (ld_conv_update rounds each product to bf16, as
+// the host engine's kernel that it replaces does.)
+//
+// One pass bound by HBM: 2 bytes read and 2 written per (token, channel).  A thread owns 8 channels of a
+// tile of consecutive tokens, whatever requests they belong to, and slides the window along, so a tile
+// reads w - 1 rows beyond its own; rows come in batches of 8 loads before the first is used.  silu costs
+// two special-function operations per value, 0.7 of the time HBM needs, which the batches overlap.
+// A request's first w - 1 tokens all go to the thread that has its first one: only that thread reads the
+// history, so it can also write the slot when a request goes on inside a block and its source slot is
+// its first destination.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "internal.h"
+#include "launch.cuh"
+#include "lightdelta_b200.h"
+
+namespace ldb {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kBatch = 8;  // rows loaded together
+
+__device__ unsigned int g_conv_prefill_faults;
+
+struct ConvPrefillArgs {
+  const __nv_bfloat16* x;
+  int64_t x_row;
+  int64_t n_tokens;
+  int64_t dim;
+  __nv_bfloat16* state;  // element (slot, channel, position) at slot*s_slot + channel*s_dim + position*s_pos
+  int64_t n_slots, s_slot, s_dim, s_pos;
+  const __nv_bfloat16* weight;
+  const __nv_bfloat16* bias;
+  const int32_t* table;
+  int64_t table_row, table_width, block_size;
+  const int32_t* context;
+  const int32_t* cu;
+  int n_requests;
+  int tile;  // tokens per thread
+  __nv_bfloat16* out;
+};
+
+template <int kVec>
+struct Row {  // kVec consecutive bf16 channels of one token
+  __nv_bfloat16 v[kVec];
+};
+
+template <int kVec>
+__device__ __forceinline__ Row<kVec> load_row(const __nv_bfloat16* at) {
+  Row<kVec> r;
+  if constexpr (kVec == 8) {
+    *reinterpret_cast<uint4*>(r.v) = *reinterpret_cast<const uint4*>(at);
+  } else {
+    r.v[0] = *at;
+  }
+  return r;
+}
+
+template <int kVec>
+__device__ __forceinline__ void store_row(__nv_bfloat16* at, const Row<kVec>& r) {
+  if constexpr (kVec == 8) {
+    *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(r.v);
+  } else {
+    *at = r.v[0];
+  }
+}
+
+template <int kVec>
+__device__ __forceinline__ Row<kVec> zero_row() {
+  Row<kVec> r;
+#pragma unroll
+  for (int c = 0; c < kVec; ++c) r.v[c] = __float2bfloat16_rn(0.0f);
+  return r;
+}
+
+// One position of a slot's window for this thread's channels.
+template <int kVec>
+__device__ __forceinline__ Row<kVec> load_window(const ConvPrefillArgs& p, int32_t slot, int64_t channel, int position) {
+  const __nv_bfloat16* at = p.state + slot * p.s_slot + channel * p.s_dim + position * p.s_pos;
+  Row<kVec> r;
+#pragma unroll
+  for (int c = 0; c < kVec; ++c) r.v[c] = at[c * p.s_dim];
+  return r;
+}
+
+template <int kVec>
+__device__ __forceinline__ void store_window(const ConvPrefillArgs& p, int32_t slot, int64_t channel, int position,
+                                             const Row<kVec>& r) {
+  __nv_bfloat16* at = p.state + slot * p.s_slot + channel * p.s_dim + position * p.s_pos;
+#pragma unroll
+  for (int c = 0; c < kVec; ++c) at[c * p.s_dim] = r.v[c];
+}
+
+// The request that a thread is in.
+struct Place {
+  int64_t begin, end;   // its tokens
+  int64_t context;
+  int64_t next_end;     // the next token after which a block or the request ends
+  const int32_t* row;
+  int32_t source;       // slot of the history (0: none)
+  int32_t kept;         // block that the request's first thread writes because it is also read (-1: none)
+  bool ok;              // false: zero outputs, nothing else
+};
+
+__device__ __forceinline__ void enter(const ConvPrefillArgs& p, int r, int64_t token, bool report, Place& at) {
+  at.begin = p.cu[r];
+  at.end = p.cu[r + 1];
+  at.context = p.context[r];
+  at.row = p.table + r * p.table_row;
+  at.source = 0;
+  at.kept = -1;
+  at.next_end = at.end;
+  unsigned int fault = 0;
+  at.ok = at.context >= 0 && (at.context + (at.end - at.begin) - 1) / p.block_size < p.table_width;
+  if (!at.ok) {
+    fault = LD_FAULT_TABLE_BLOCKS;
+  } else {
+    if (at.context > 0) {
+      at.source = at.row[(at.context - 1) / p.block_size];
+      if (at.source >= p.n_slots) fault = LD_FAULT_CONV_SLOT_RANGE;
+      at.ok = at.source > 0 && at.source < p.n_slots;
+      if (at.context % p.block_size != 0) at.kept = static_cast<int32_t>(at.context / p.block_size);
+    }
+    const int64_t position = at.context + (token - at.begin);
+    at.next_end = min(at.end, at.begin + (position / p.block_size + 1) * p.block_size - at.context);
+  }
+  if (fault != 0 && report) atomicOr(&g_conv_prefill_faults, fault);
+}
+
+// The input `back` >= 1 tokens before token t of the request: an earlier row, or its history.
+template <int kVec, int kWidth>
+__device__ __forceinline__ Row<kVec> earlier(const ConvPrefillArgs& p, const Place& at, int64_t t, int back,
+                                             int64_t channel) {
+  const int64_t i = t - back;
+  if (i >= at.begin) return load_row<kVec>(p.x + i * p.x_row + channel);
+  if (at.source == 0) return zero_row<kVec>();
+  return load_window<kVec>(p, at.source, channel, static_cast<int>(kWidth - 1 + (i - at.begin)));
+}
+
+template <int kVec, int kWidth>
+__global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefillArgs p) {
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const int64_t channel = (static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x) * kVec;
+  int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+  const int64_t t1 = min(t0 + p.tile, p.n_tokens);
+
+  // The request of the first token: the last r with cu[r] <= t0, by 32-way bisection (the warp's lanes
+  // probe together).  Offsets that are out of order or range are caught by the checks below.
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.n_requests;  // cu[lo] <= t0 (or lo is 0), cu[hi] > t0 (or hi is the end)
+  while (hi - lo > 1) {
+    const int width = (hi - lo + 31) / 32;
+    const int probe = lo + (lane + 1) * width;
+    const bool below = probe < hi && p.cu[probe] <= t0;
+    const unsigned int votes = __ballot_sync(0xffffffffu, below);
+    const int passed = __popc(votes);  // probes are in order, so the votes are a prefix
+    const int next = lo + passed * width;
+    hi = min(hi, next + width);
+    lo = next;
+  }
+  int r = lo;
+  if (channel >= p.dim) return;
+  // The tile before takes what is left of a request's first w - 1 tokens (a first token at t0 - 1 or so).
+  const int64_t begun = p.cu[r];
+  if (begun >= 0 && begun < t0 && t0 < begun + kWidth - 1) {
+    t0 = max(t0, min(static_cast<int64_t>(p.cu[r + 1]), begun + kWidth - 1));
+  }
+  int64_t limit = t1;
+  const int64_t limit_most = min(t1 + kWidth - 2, p.n_tokens);
+  const bool report = channel == 0;
+
+  float wt[kWidth][kVec], bias[kVec];
+#pragma unroll
+  for (int c = 0; c < kVec; ++c) {
+#pragma unroll
+    for (int j = 0; j < kWidth; ++j) wt[j][c] = __bfloat162float(p.weight[(channel + c) * kWidth + j]);
+    bias[c] = p.bias != nullptr ? __bfloat162float(p.bias[channel + c]) : 0.0f;
+  }
+
+  Place at;
+  at.end = -1;  // no request yet
+  Row<kVec> window[kWidth - 1];  // inputs t - w + 1 .. t - 1
+#pragma unroll
+  for (int j = 0; j < kWidth - 1; ++j) window[j] = zero_row<kVec>();
+  for (int64_t b0 = t0; b0 < limit; b0 += kBatch) {
+    Row<kVec> rows[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (b0 + i < limit_most) rows[i] = load_row<kVec>(p.x + (b0 + i) * p.x_row + channel);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t t = b0 + i;
+      if (t >= limit) break;
+      if (t >= at.end) {  // first token of the tile, or of another request
+        while (r < p.n_requests && p.cu[r + 1] <= t) ++r;
+        if (r >= p.n_requests) return;  // rows behind the last request stay as they are
+        if (p.cu[r] > t || p.cu[r] < 0 || p.cu[r + 1] > p.n_tokens) {
+          if (report && p.cu[r] <= t) atomicOr(&g_conv_prefill_faults, LD_FAULT_DECODE_TOKENS);
+          continue;  // rows of no request
+        }
+        enter(p, r, t, report, at);
+        if (t == at.begin) limit = max(limit, min(at.end, t + kWidth - 1));
+        if (at.ok) {
+#pragma unroll
+          for (int j = 0; j < kWidth - 1; ++j) window[j] = earlier<kVec, kWidth>(p, at, t, kWidth - 1 - j, channel);
+          if (t == at.begin && at.kept >= 0) {
+            // This thread has read the source slot, which is the request's first destination too:
+            // it writes it now, whichever tile its block's last token lies in.
+            const int64_t stop = min(at.end, at.begin + static_cast<int64_t>(at.kept + 1) * p.block_size - at.context);
+            Row<kVec> last[kWidth - 1];
+#pragma unroll
+            for (int j = 0; j < kWidth - 1; ++j) last[j] = earlier<kVec, kWidth>(p, at, stop, kWidth - 1 - j, channel);
+#pragma unroll
+            for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, at.source, channel, j, last[j]);
+          }
+        }
+      }
+      __nv_bfloat16* out = p.out + t * p.dim + channel;
+      if (!at.ok) {
+        store_row<kVec>(out, zero_row<kVec>());
+        continue;
+      }
+      Row<kVec> y;
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) {
+        float acc = bias[c];
+#pragma unroll
+        for (int j = 0; j < kWidth - 1; ++j) acc = fmaf(__bfloat162float(window[j].v[c]), wt[j][c], acc);
+        acc = fmaf(__bfloat162float(rows[i].v[c]), wt[kWidth - 1][c], acc);
+        // The fast exponential and division are within a few fp32 ulps, far below bf16's rounding.
+        y.v[c] = __float2bfloat16_rn(__fdividef(acc, 1.0f + __expf(-acc)));
+      }
+      store_row<kVec>(out, y);
+#pragma unroll
+      for (int j = 0; j + 1 < kWidth - 1; ++j) window[j] = window[j + 1];
+      window[kWidth - 2] = rows[i];
+      if (t + 1 == at.next_end) {
+        const int64_t position = at.context + (t - at.begin);
+        const int64_t block = position / p.block_size;
+        if (block != at.kept) {
+          const int32_t slot = at.row[block];
+          if (slot > 0 && slot < p.n_slots) {
+#pragma unroll
+            for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, slot, channel, j, window[j]);
+          } else if (slot >= p.n_slots && report) {
+            atomicOr(&g_conv_prefill_faults, LD_FAULT_CONV_SLOT_RANGE);
+          }
+        }
+        at.next_end = min(at.end, at.next_end + p.block_size);
+      }
+    }
+  }
+}
+
+bool aligned(const void* ptr, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; }
+
+template <int kWidth>
+cudaError_t launch_width(ConvPrefillArgs& args, bool vec, cudaStream_t stream) {
+  const int64_t groups = (args.dim + (vec ? 8 : 1) * kThreads - 1) / ((vec ? 8 : 1) * kThreads);
+  // 32 tokens per thread read 3 rows of 35 twice; 8 tokens per thread spread short batches over the SMs.
+  args.tile = args.n_tokens * groups >= 32 * 4 * 148 ? 32 : 8;
+  const dim3 grid(static_cast<unsigned int>((args.n_tokens + args.tile - 1) / args.tile),
+                  static_cast<unsigned int>(groups));
+  if (vec) return launch(conv_prefill_kernel<8, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
+  return launch(conv_prefill_kernel<1, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
+}
+
+}  // namespace
+
+int conv_prefill_faults(uint32_t* flags, int clear) {
+  uint32_t value = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(&value, g_conv_prefill_faults, sizeof(value));
+  if (err == cudaSuccess && clear) {
+    const uint32_t zero = 0;
+    err = cudaMemcpyToSymbol(g_conv_prefill_faults, &zero, sizeof(zero));
+  }
+  if (err != cudaSuccess) return set_error(LD_ERR_CUDA, "ld_fault_flags: %s", cudaGetErrorString(err));
+  *flags = value;
+  return LD_OK;
+}
+
+}  // namespace ldb
+
+extern "C" int ld_conv_prefill(const void* x, int64_t x_row_stride, int64_t n_tokens, int64_t dim, void* conv_state,
+                               int64_t n_conv_slots, int64_t conv_slot_stride, int64_t conv_dim_stride,
+                               int64_t conv_pos_stride, int64_t conv_state_len, const void* conv_weight,
+                               const void* conv_bias, int64_t conv_width, const int32_t* table,
+                               int64_t table_row_stride, int64_t table_width, int64_t block_size,
+                               const int32_t* context, const int32_t* cu, int64_t n_requests, void* out,
+                               void* stream) {
+  using namespace ldb;
+  if (conv_width < 2 || conv_width > 4) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: kernel width must be 2 through 4");
+  }
+  if (conv_state_len < conv_width - 1) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: the conv state holds fewer than width - 1 positions");
+  }
+  if (block_size < 1) return set_error(LD_ERR_INVALID, "conv_prefill: block_size must be positive");
+  if (n_requests < 0 || n_requests > INT32_MAX / 2 || n_tokens < 0 || n_tokens > INT32_MAX || dim < 1 ||
+      dim > INT32_MAX / 2) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: request, token or channel count out of range");
+  }
+  if (table_width < 1 || table_row_stride < table_width) {
+    return set_error(LD_ERR_INVALID,
+                     "conv_prefill: the table needs at least one block per row and rows that do not overlap");
+  }
+  if (x_row_stride < dim || n_conv_slots < 1 || conv_slot_stride < 0 || conv_dim_stride < 1 || conv_pos_stride < 1) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: invalid strides or slot count");
+  }
+  const bool dims_disjoint =
+      conv_dim_stride >= conv_state_len * conv_pos_stride || conv_pos_stride >= dim * conv_dim_stride;
+  const int64_t slot_extent = (dim - 1) * conv_dim_stride + (conv_state_len - 1) * conv_pos_stride + 1;
+  if (!dims_disjoint || (n_conv_slots > 1 && conv_slot_stride < slot_extent)) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: the conv state's strides make slots, channels or positions overlap");
+  }
+  if (n_requests == 0 || n_tokens == 0) return ok();
+  if (x == nullptr || conv_state == nullptr || conv_weight == nullptr || table == nullptr || context == nullptr ||
+      cu == nullptr || out == nullptr) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: a required pointer is NULL");
+  }
+  if (!aligned(x, 2) || !aligned(conv_state, 2) || !aligned(conv_weight, 2) || !aligned(conv_bias, 2) ||
+      !aligned(out, 2)) {
+    return set_error(LD_ERR_INVALID, "conv_prefill: bf16 tensors must be 2-byte aligned");
+  }
+  // Neighbouring tiles read the same inputs, so the outputs cannot take their place.
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), o0 = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t x1 = x0 + 2 * static_cast<uintptr_t>((n_tokens - 1) * x_row_stride + dim);
+  const uintptr_t o1 = o0 + 2 * static_cast<uintptr_t>(n_tokens * dim);
+  if (x0 < o1 && o0 < x1) return set_error(LD_ERR_INVALID, "conv_prefill: out must not overlap x");
+  ConvPrefillArgs args;
+  args.x = static_cast<const __nv_bfloat16*>(x);
+  args.x_row = x_row_stride;
+  args.n_tokens = n_tokens;
+  args.dim = dim;
+  args.state = static_cast<__nv_bfloat16*>(conv_state);
+  args.n_slots = n_conv_slots;
+  args.s_slot = conv_slot_stride;
+  args.s_dim = conv_dim_stride;
+  args.s_pos = conv_pos_stride;
+  args.weight = static_cast<const __nv_bfloat16*>(conv_weight);
+  args.bias = static_cast<const __nv_bfloat16*>(conv_bias);
+  args.table = table;
+  args.table_row = table_row_stride;
+  args.table_width = table_width;
+  args.block_size = block_size;
+  args.context = context;
+  args.cu = cu;
+  args.n_requests = static_cast<int>(n_requests);
+  args.tile = 0;
+  args.out = static_cast<__nv_bfloat16*>(out);
+  const bool vec = dim % 8 == 0 && aligned(x, 16) && x_row_stride % 8 == 0 && aligned(out, 16);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err;
+  switch (conv_width) {
+    case 2: err = launch_width<2>(args, vec, s); break;
+    case 3: err = launch_width<3>(args, vec, s); break;
+    default: err = launch_width<4>(args, vec, s); break;
+  }
+  if (err != cudaSuccess) return set_error(LD_ERR_CUDA, "conv prefill launch failed: %s", cudaGetErrorString(err));
+  return ok();
+}

@@ -26,5 +26,8 @@ int decode_faults(uint32_t* flags, int clear);
 int state_io_faults(uint32_t* flags, int clear);
 int verify_faults(uint32_t* flags, int clear);
 int conv_faults(uint32_t* flags, int clear);
+int prefill_faults(uint32_t* flags, int clear);
+int conv_prefill_faults(uint32_t* flags, int clear);
+int tables_faults(uint32_t* flags, int clear);
 
 }  // namespace ldb

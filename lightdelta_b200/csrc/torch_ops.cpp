@@ -32,12 +32,13 @@ struct DecodeGeometry {
   int64_t h, hv, n;
 };
 
-// The reference launcher's tensor checks (csrc/gdn_decode.cu:367-403), head counts from the tensors.
-DecodeGeometry check_decode(const at::Tensor& qkv, const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_log,
-                            const at::Tensor& dt_bias, const at::Tensor& indices, const at::Tensor& cu,
-                            const at::Tensor& accepted, const at::Tensor& state, const at::Tensor& gate,
-                            const at::Tensor& weight, const at::Tensor& out, double eps,
-                            at::ScalarType state_type = at::kFloat) {
+// The reference launcher's checks of the layer's tensors (csrc/gdn_decode.cu:367-403), head counts from the
+// tensors; `indices`, `cu` and `accepted` are checked where a caller passes them (check_decode).
+DecodeGeometry check_layer(const at::Tensor& qkv, const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_log,
+                           const at::Tensor& dt_bias, const at::Tensor& state, const at::Tensor& gate,
+                           const at::Tensor& weight, const at::Tensor& out, double eps, at::ScalarType state_type,
+                           const at::Tensor* indices = nullptr, const at::Tensor* cu = nullptr,
+                           const at::Tensor* accepted = nullptr) {
   TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, "qkv must be CUDA BF16");
   for (const auto& t : {a, b, gate, out}) {
     TORCH_CHECK(t.device() == qkv.device() && t.scalar_type() == at::kBFloat16 && t.stride(-1) == 1,
@@ -48,9 +49,11 @@ DecodeGeometry check_decode(const at::Tensor& qkv, const at::Tensor& a, const at
   TORCH_CHECK(state.device() == qkv.device() && state.scalar_type() == state_type && state.stride(-1) == 1,
               state_type == at::kFloat ? "state and A_log must be CUDA FP32 with dense rows"
                                        : "state must be CUDA BF16 with dense rows");
-  for (const auto& t : {indices, cu, accepted}) {
-    TORCH_CHECK(t.device() == qkv.device() && t.scalar_type() == at::kInt && t.is_contiguous(),
-                "metadata must be contiguous CUDA int32");
+  if (indices != nullptr) {
+    for (const auto& t : {*indices, *cu, *accepted}) {
+      TORCH_CHECK(t.device() == qkv.device() && t.scalar_type() == at::kInt && t.is_contiguous(),
+                  "metadata must be contiguous CUDA int32");
+    }
   }
   for (const auto& t : {dt_bias, weight}) {
     TORCH_CHECK(t.device() == qkv.device() && t.is_contiguous() &&
@@ -66,7 +69,8 @@ DecodeGeometry check_decode(const at::Tensor& qkv, const at::Tensor& a, const at
               "qkv must be [tokens,(2*H+HV)*128] with HV=state.size(1)");
   const int64_t h = (qkv.size(1) / LD_HEAD_DIM - hv) / 2;
   TORCH_CHECK(hv % h == 0, "value heads must be a multiple of key heads");
-  TORCH_CHECK(indices.dim() == 2 && indices.size(1) >= 1 && indices.size(1) <= LD_MAX_WIDTH,
+  TORCH_CHECK(indices == nullptr ||
+                  (indices->dim() == 2 && indices->size(1) >= 1 && indices->size(1) <= LD_MAX_WIDTH),
               "decode/MTP supports 1 through 4 tokens per request");
   const auto n = qkv.size(0);
   TORCH_CHECK(a.sizes() == at::IntArrayRef({n, hv}) && b.sizes() == a.sizes() &&
@@ -75,11 +79,19 @@ DecodeGeometry check_decode(const at::Tensor& qkv, const at::Tensor& a, const at
               "invalid activation shape or output layout");
   TORCH_CHECK(a_log.numel() == hv && dt_bias.numel() == hv && weight.numel() == LD_HEAD_DIM,
               "invalid weight shapes");
-  TORCH_CHECK(cu.dim() == 1 && cu.numel() == indices.size(0) + 1 && accepted.dim() == 1 &&
-                  accepted.numel() == indices.size(0),
+  TORCH_CHECK(indices == nullptr || (cu->dim() == 1 && cu->numel() == indices->size(0) + 1 && accepted->dim() == 1 &&
+                                     accepted->numel() == indices->size(0)),
               "invalid request metadata shapes");
   TORCH_CHECK(eps > 0, "norm epsilon must be positive");
   return DecodeGeometry{h, hv, n};
+}
+
+DecodeGeometry check_decode(const at::Tensor& qkv, const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_log,
+                            const at::Tensor& dt_bias, const at::Tensor& indices, const at::Tensor& cu,
+                            const at::Tensor& accepted, const at::Tensor& state, const at::Tensor& gate,
+                            const at::Tensor& weight, const at::Tensor& out, double eps,
+                            at::ScalarType state_type = at::kFloat) {
+  return check_layer(qkv, a, b, a_log, dt_bias, state, gate, weight, out, eps, state_type, &indices, &cu, &accepted);
 }
 
 }  // namespace
@@ -302,6 +314,101 @@ void greedy_verify(const at::Tensor& logits, const at::Tensor& cu_num_logits, co
                             num_sampled.data_ptr<int32_t>(), num_rejected.data_ptr<int32_t>(), stream_of(logits)));
 }
 
+namespace {
+
+// table, context and cu of the prompt path.
+void check_table(const at::Tensor& on, const at::Tensor& table, const at::Tensor& context, const at::Tensor& cu) {
+  TORCH_CHECK(table.device() == on.device() && table.scalar_type() == at::kInt && table.dim() == 2 &&
+                  table.size(1) >= 1 && table.stride(1) == 1 &&
+                  (table.size(0) <= 1 || table.stride(0) >= table.size(1)),
+              "table must be a CUDA int32 [requests, blocks] matrix with dense rows");
+  for (const auto& t : {context, cu}) {
+    TORCH_CHECK(t.device() == on.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(),
+                "request metadata must be contiguous CUDA int32 vectors");
+  }
+  TORCH_CHECK(context.numel() == table.size(0) && cu.numel() == table.size(0) + 1, "invalid request metadata shapes");
+}
+
+// Row stride of a matrix whose only row may carry any stride.
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+}  // namespace
+
+// Extension (no reference schema): token offsets, block table, positions, slot map and state slots
+// of a batch from its request lengths.
+void request_tables(const at::Tensor& query_lens, const at::Tensor& context, const at::Tensor& free_blocks,
+                    at::Tensor table, at::Tensor cu, at::Tensor positions, at::Tensor slot_map, at::Tensor state_slots,
+                    at::Tensor used, int64_t block_size) {
+  TORCH_CHECK(query_lens.is_cuda() && query_lens.scalar_type() == at::kInt && query_lens.dim() == 1 &&
+                  query_lens.is_contiguous(),
+              "query_lens must be a contiguous CUDA int32 vector");
+  const c10::cuda::CUDAGuard guard(query_lens.device());
+  const int64_t n = query_lens.numel();
+  check_table(query_lens, table, context, cu);
+  TORCH_CHECK(context.numel() == n, "query_lens and context differ in length");
+  TORCH_CHECK(free_blocks.device() == query_lens.device() && free_blocks.scalar_type() == at::kInt &&
+                  free_blocks.dim() == 1 && free_blocks.is_contiguous(),
+              "free_blocks must be a contiguous CUDA int32 vector");
+  for (const auto& t : {positions, slot_map}) {
+    TORCH_CHECK(t.device() == query_lens.device() && t.scalar_type() == at::kLong && t.dim() == 1 && t.is_contiguous(),
+                "positions and slot_map must be contiguous CUDA int64 vectors");
+  }
+  TORCH_CHECK(positions.numel() == slot_map.numel(), "positions and slot_map differ in length");
+  TORCH_CHECK(state_slots.device() == query_lens.device() && state_slots.scalar_type() == at::kInt &&
+                  state_slots.sizes() == at::IntArrayRef({n, 2}) && state_slots.is_contiguous(),
+              "state_slots must be a contiguous CUDA int32 [requests, 2] matrix");
+  TORCH_CHECK(used.device() == query_lens.device() && used.scalar_type() == at::kInt && used.numel() == 1,
+              "used must be one CUDA int32");
+  check_rc(ld_request_tables(query_lens.data_ptr<int32_t>(), context.data_ptr<int32_t>(), n,
+                             free_blocks.data_ptr<int32_t>(), free_blocks.numel(), table.data_ptr<int32_t>(),
+                             row_stride(table), table.size(1), block_size, cu.data_ptr<int32_t>(),
+                             positions.data_ptr<int64_t>(), slot_map.data_ptr<int64_t>(), positions.numel(),
+                             state_slots.data_ptr<int32_t>(), used.data_ptr<int32_t>(), stream_of(query_lens)));
+}
+
+// Extension (no reference schema): the causal conv1d and silu over prompts, whose windows go to the
+// blocks' slots.
+void conv_prefill(const at::Tensor& x, at::Tensor conv_state, const at::Tensor& conv_weight,
+                  const c10::optional<at::Tensor>& conv_bias, const at::Tensor& table, const at::Tensor& context,
+                  const at::Tensor& cu, at::Tensor out, int64_t block_size) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.stride(1) == 1,
+              "x must be a CUDA BF16 [tokens, dim] matrix with dense rows");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const ConvTensors conv = check_conv(x, conv_state, conv_weight, conv_bias);
+  check_table(x, table, context, cu);
+  TORCH_CHECK(out.device() == x.device() && out.scalar_type() == at::kBFloat16 && out.sizes() == x.sizes() &&
+                  out.is_contiguous(),
+              "out must be a contiguous CUDA BF16 tensor of x's shape");
+  if (x.size(0) == 0) return;
+  check_rc(ld_conv_prefill(x.data_ptr(), row_stride(x), x.size(0), x.size(1), conv_state.data_ptr(),
+                           conv_state.size(0), conv_state.stride(0), conv_state.stride(1), conv_state.stride(2),
+                           conv_state.size(2), conv.weight.data_ptr(), conv.bias, conv.weight.size(1),
+                           table.data_ptr<int32_t>(), row_stride(table), table.size(1), block_size,
+                           context.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), context.numel(), out.data_ptr(),
+                           stream_of(x)));
+}
+
+// Extension (no reference schema): the chunked form of decode's recurrence over prompts, on an fp32 or
+// bf16 state pool.
+void prefill(const at::Tensor& qkv, const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_log,
+             const at::Tensor& dt_bias, const at::Tensor& table, const at::Tensor& context, const at::Tensor& cu,
+             at::Tensor state, const at::Tensor& gate, const at::Tensor& weight, at::Tensor out, int64_t block_size,
+             double eps) {
+  TORCH_CHECK(qkv.is_cuda(), "qkv must be CUDA BF16");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  check_table(qkv, table, context, cu);
+  const DecodeGeometry geo = check_layer(qkv, a, b, a_log, dt_bias, state, gate, weight, out, eps,
+                                         state.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat);
+  if (geo.n == 0) return;
+  check_rc(ld_prefill(qkv.data_ptr(), row_stride(qkv), a.data_ptr(), row_stride(a), b.data_ptr(), row_stride(b),
+                      a_log.data_ptr<float>(), dt_bias.data_ptr(), dtype_code(dt_bias), table.data_ptr<int32_t>(),
+                      row_stride(table), table.size(1), block_size, context.data_ptr<int32_t>(),
+                      cu.data_ptr<int32_t>(), context.numel(), state.data_ptr(), dtype_code(state), state.size(0),
+                      state.size(0) > 1 ? state.stride(0) : geo.hv * LD_HEAD_DIM * LD_HEAD_DIM, gate.data_ptr(),
+                      geo.n > 1 ? gate.stride(0) : geo.hv * LD_HEAD_DIM, weight.data_ptr(), dtype_code(weight),
+                      out.data_ptr(), geo.n, geo.h, geo.hv, static_cast<float>(eps), stream_of(qkv)));
+}
+
 }  // namespace lightdelta_b200
 
 TORCH_LIBRARY(lightdelta, m) {
@@ -327,6 +434,15 @@ TORCH_LIBRARY(lightdelta, m) {
       "greedy_verify(Tensor logits, Tensor cu_num_logits, Tensor query_start_loc, Tensor input_ids, "
       "Tensor num_draft_tokens, Tensor seq_lens, Tensor prefill_len, Tensor(a!) sampled, "
       "Tensor(b!) num_sampled, Tensor(c!) num_rejected) -> ()");
+  m.def(
+      "request_tables(Tensor query_lens, Tensor context, Tensor free_blocks, Tensor(t!) table, Tensor(c!) cu, "
+      "Tensor(p!) positions, Tensor(m!) slot_map, Tensor(s!) state_slots, Tensor(u!) used, int block_size) -> ()");
+  m.def(
+      "conv_prefill(Tensor x, Tensor(c!) conv_state, Tensor conv_weight, Tensor? conv_bias, Tensor table, "
+      "Tensor context, Tensor cu, Tensor(o!) out, int block_size) -> ()");
+  m.def(
+      "prefill(Tensor qkv, Tensor a, Tensor b, Tensor a_log, Tensor dt_bias, Tensor table, Tensor context, "
+      "Tensor cu, Tensor(s!) state, Tensor gate, Tensor weight, Tensor(o!) out, int block_size, float eps) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(lightdelta, CUDA, m) {
@@ -338,4 +454,7 @@ TORCH_LIBRARY_IMPL(lightdelta, CUDA, m) {
   m.impl("greedy_verify", lightdelta_b200::greedy_verify);
   m.impl("conv_decode", lightdelta_b200::conv_decode);
   m.impl("conv_update", lightdelta_b200::conv_update);
+  m.impl("request_tables", lightdelta_b200::request_tables);
+  m.impl("conv_prefill", lightdelta_b200::conv_prefill);
+  m.impl("prefill", lightdelta_b200::prefill);
 }

@@ -4,7 +4,8 @@ Mirror of the reference's python/lightdelta/ops/__init__.py:1-21: importing this
 the native registration library (here lightdelta_b200/_C.so, built for sm_100a) and registers
 no-op fake kernels so the ops can be traced.  After import, ``torch.ops.lightdelta.decode``,
 ``gather_state`` and ``scatter_state`` have the reference's exact schemas; ``copy_state`` is an
-extension.  A missing library raises: there is no CPU fallback.
+extension, and so are the prompt path's ``request_tables``, ``conv_prefill`` and ``prefill``.  A missing
+library raises: there is no CPU fallback.
 """
 
 from __future__ import annotations
@@ -62,4 +63,20 @@ def _conv_decode_fake(qkv, conv_state, conv_weight, conv_bias, a, b, a_log, dt_b
 
 @torch.library.register_fake("lightdelta::conv_update")
 def _conv_update_fake(x, conv_state, conv_weight, conv_bias, slots, accepted, cu, max_tokens):
+    return None
+
+
+@torch.library.register_fake("lightdelta::request_tables")
+def _request_tables_fake(query_lens, context, free_blocks, table, cu, positions, slot_map, state_slots, used,
+                         block_size):
+    return None
+
+
+@torch.library.register_fake("lightdelta::conv_prefill")
+def _conv_prefill_fake(x, conv_state, conv_weight, conv_bias, table, context, cu, out, block_size):
+    return None
+
+
+@torch.library.register_fake("lightdelta::prefill")
+def _prefill_fake(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, out, block_size, eps):
     return None
