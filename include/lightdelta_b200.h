@@ -383,7 +383,16 @@ int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a
                int64_t table_row_stride, int64_t table_width, int64_t block_size, const int32_t* context,
                const int32_t* cu, int64_t n_requests, void* state, int state_dtype, int64_t n_slots,
                int64_t slot_stride, const void* gate, int64_t gate_row_stride, const void* weight, int weight_dtype,
-               void* out, int64_t n_tokens, int64_t num_k_heads, int64_t num_v_heads, float eps, void* stream);
+               void* out, int64_t n_tokens, int64_t num_k_heads, int64_t num_v_heads, float eps, void* workspace,
+               int64_t workspace_size, void* stream);
+
+/*
+ * Bytes of device memory that ld_prefill needs as `workspace` (128-byte aligned) for a call of these sizes:
+ * about 16 KiB per token at 16 key and 32 value heads.  It is written and read by the call alone, needs no
+ * clearing, and may be used again by work behind the call on the same stream; calls that may overlap (other
+ * streams, graphs that run side by side) need one each.  Negative: -LD_ERR_INVALID.
+ */
+int64_t ld_prefill_workspace(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads);
 
 /*
  * The causal conv1d of the q, k, v channels over prompts, in front of ld_prefill:

@@ -96,9 +96,11 @@ def lib() -> ctypes.CDLL:
     handle.ld_conv_prefill.restype = i32
     handle.ld_prefill.argtypes = [
         p, i64, p, i64, p, i64, p, p, i32, p, i64, i64, i64, p, p, i64, p, i32, i64, i64, p, i64, p, i32, p, i64, i64,
-        i64, f32, p,
+        i64, f32, p, i64, p,
     ]
     handle.ld_prefill.restype = i32
+    handle.ld_prefill_workspace.argtypes = [i64, i64, i64, i64]
+    handle.ld_prefill_workspace.restype = i64
     handle.ld_programmatic_launch.argtypes = [i32]
     handle.ld_programmatic_launch.restype = i32
     handle.ld_decode_wait_test.argtypes = [i64, i32]
@@ -290,16 +292,31 @@ def conv_prefill(x, conv_state, conv_weight, conv_bias, table, context, cu, out,
     ))
 
 
-def prefill(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, out, block_size, eps=1e-6, stream=None):
-    """ld_prefill on torch tensors laid out as torch.ops.lightdelta.prefill expects."""
+def prefill_workspace(tokens: int, requests: int, num_k_heads: int, num_v_heads: int) -> int:
+    """Bytes of workspace that ld_prefill needs for a call of these sizes."""
+    size = lib().ld_prefill_workspace(tokens, requests, num_k_heads, num_v_heads)
+    if size < 0:
+        raise LightDeltaError(-size, last_error())
+    return size
+
+
+def prefill(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, out, block_size, eps=1e-6,
+            workspace=None, stream=None):
+    """ld_prefill on torch tensors laid out as torch.ops.lightdelta.prefill expects; `workspace` is a CUDA
+    byte tensor of prefill_workspace(...) bytes at least."""
+    import torch
+
     hv = state.shape[1]
     h = (qkv.shape[1] // HEAD_DIM - hv) // 2
+    if workspace is None:
+        workspace = torch.empty(prefill_workspace(qkv.shape[0], context.numel(), h, hv), dtype=torch.uint8,
+                                device=qkv.device)
     check(lib().ld_prefill(
         qkv.data_ptr(), qkv.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_log.data_ptr(),
         dt_bias.data_ptr(), _dtype_code(dt_bias), table.data_ptr(), table.stride(0), table.shape[1], int(block_size),
         context.data_ptr(), cu.data_ptr(), context.numel(), state.data_ptr(), _dtype_code(state), state.shape[0],
         state.stride(0), gate.data_ptr(), gate.stride(0), weight.data_ptr(), _dtype_code(weight), out.data_ptr(),
-        qkv.shape[0], h, hv, float(eps), _stream(qkv, stream),
+        qkv.shape[0], h, hv, float(eps), workspace.data_ptr(), workspace.numel(), _stream(qkv, stream),
     ))
 
 

@@ -400,13 +400,19 @@ void prefill(const at::Tensor& qkv, const at::Tensor& a, const at::Tensor& b, co
   const DecodeGeometry geo = check_layer(qkv, a, b, a_log, dt_bias, state, gate, weight, out, eps,
                                          state.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat);
   if (geo.n == 0) return;
+  // The workspace comes from torch's caching allocator, on the current stream (in a capture, from the
+  // graph's own pool), and goes back to it when the launches are queued.
+  const int64_t bytes = ld_prefill_workspace(geo.n, context.numel(), geo.h, geo.hv);
+  TORCH_CHECK(bytes >= 0, ld_last_error());
+  const at::Tensor workspace = at::empty({bytes}, qkv.options().dtype(at::kByte));
   check_rc(ld_prefill(qkv.data_ptr(), row_stride(qkv), a.data_ptr(), row_stride(a), b.data_ptr(), row_stride(b),
                       a_log.data_ptr<float>(), dt_bias.data_ptr(), dtype_code(dt_bias), table.data_ptr<int32_t>(),
                       row_stride(table), table.size(1), block_size, context.data_ptr<int32_t>(),
                       cu.data_ptr<int32_t>(), context.numel(), state.data_ptr(), dtype_code(state), state.size(0),
                       state.size(0) > 1 ? state.stride(0) : geo.hv * LD_HEAD_DIM * LD_HEAD_DIM, gate.data_ptr(),
                       geo.n > 1 ? gate.stride(0) : geo.hv * LD_HEAD_DIM, weight.data_ptr(), dtype_code(weight),
-                      out.data_ptr(), geo.n, geo.h, geo.hv, static_cast<float>(eps), stream_of(qkv)));
+                      out.data_ptr(), geo.n, geo.h, geo.hv, static_cast<float>(eps), workspace.data_ptr(), bytes,
+                      stream_of(qkv)));
 }
 
 }  // namespace lightdelta_b200
