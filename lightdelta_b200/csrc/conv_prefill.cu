@@ -8,7 +8,7 @@
 // Products and sums are fp32, rounded once at the end.  (ld_conv_update rounds each product to bf16, as
 // the host engine's kernel that it replaces does.)
 //
-// One pass bound by HBM: 2 bytes read and 2 written per (token, channel).  A thread owns 8 channels of a
+// One pass bound by HBM: 2 bytes read and 2 written per (token, channel).  A thread owns 4 channels of a
 // tile of consecutive tokens, whatever requests they belong to, and slides the window along, so a tile
 // reads w - 1 rows beyond its own; rows come in batches of 8 loads before the first is used.  silu costs
 // two special-function operations per value, 0.7 of the time HBM needs, which the batches overlap.
@@ -29,7 +29,8 @@ namespace ldb {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kBatch = 8;  // rows loaded together
+constexpr int kBatch = 8;   // rows loaded together
+constexpr int kVector = 4;  // channels per thread where rows allow 8-byte accesses
 
 __device__ unsigned int g_conv_prefill_faults;
 
@@ -52,15 +53,15 @@ struct ConvPrefillArgs {
 };
 
 template <int kVec>
-struct Row {  // kVec consecutive bf16 channels of one token
+struct __align__(2 * kVec) Row {  // kVec consecutive bf16 channels of one token
   __nv_bfloat16 v[kVec];
 };
 
 template <int kVec>
 __device__ __forceinline__ Row<kVec> load_row(const __nv_bfloat16* at) {
   Row<kVec> r;
-  if constexpr (kVec == 8) {
-    *reinterpret_cast<uint4*>(r.v) = *reinterpret_cast<const uint4*>(at);
+  if constexpr (kVec == 4) {
+    *reinterpret_cast<uint2*>(r.v) = *reinterpret_cast<const uint2*>(at);
   } else {
     r.v[0] = *at;
   }
@@ -69,8 +70,8 @@ __device__ __forceinline__ Row<kVec> load_row(const __nv_bfloat16* at) {
 
 template <int kVec>
 __device__ __forceinline__ void store_row(__nv_bfloat16* at, const Row<kVec>& r) {
-  if constexpr (kVec == 8) {
-    *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(r.v);
+  if constexpr (kVec == 4) {
+    *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(r.v);
   } else {
     *at = r.v[0];
   }
@@ -178,7 +179,6 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
     t0 = max(t0, min(static_cast<int64_t>(p.cu[r + 1]), begun + kWidth - 1));
   }
   int64_t limit = t1;
-  const int64_t limit_most = min(t1 + kWidth - 2, p.n_tokens);
   const bool report = channel == 0;
 
   float wt[kWidth][kVec], bias[kVec];
@@ -194,73 +194,80 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
   Row<kVec> window[kWidth - 1];  // inputs t - w + 1 .. t - 1
 #pragma unroll
   for (int j = 0; j < kWidth - 1; ++j) window[j] = zero_row<kVec>();
-  for (int64_t b0 = t0; b0 < limit; b0 += kBatch) {
+  for (int64_t t = t0; t < limit;) {
+    if (t >= at.end) {  // first token of the tile, or of another request
+      while (r < p.n_requests && p.cu[r + 1] <= t) ++r;
+      if (r >= p.n_requests) return;  // rows behind the last request stay as they are
+      const int64_t begin = p.cu[r], end = p.cu[r + 1];
+      if (begin > t || begin < 0 || end > p.n_tokens) {
+        if (report && begin <= t) atomicOr(&g_conv_prefill_faults, LD_FAULT_DECODE_TOKENS);
+        t = max(t + 1, begin > t ? begin : end);  // rows of no request
+        continue;
+      }
+      enter(p, r, t, report, at);
+      if (t == at.begin) limit = max(limit, min(at.end, t + kWidth - 1));
+      if (at.ok) {
+#pragma unroll
+        for (int j = 0; j < kWidth - 1; ++j) window[j] = earlier<kVec, kWidth>(p, at, t, kWidth - 1 - j, channel);
+        if (t == at.begin && at.kept >= 0) {
+          // This thread has read the source slot, which is the request's first destination too: it
+          // writes it now, whichever tile its block's last token lies in.
+          const int64_t stop = min(at.end, at.begin + static_cast<int64_t>(at.kept + 1) * p.block_size - at.context);
+          Row<kVec> last[kWidth - 1];
+#pragma unroll
+          for (int j = 0; j < kWidth - 1; ++j) last[j] = earlier<kVec, kWidth>(p, at, stop, kWidth - 1 - j, channel);
+#pragma unroll
+          for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, at.source, channel, j, last[j]);
+        }
+      }
+    }
+    // Up to kBatch tokens that end with their block, request or tile.
+    const int64_t stop = min(limit, at.ok ? at.next_end : at.end);
+    const int count = static_cast<int>(min(stop - t, static_cast<int64_t>(kBatch)));
+    const __nv_bfloat16* x = p.x + t * p.x_row + channel;
+    __nv_bfloat16* out = p.out + t * p.dim + channel;
+    if (!at.ok) {
+      for (int i = 0; i < count; ++i) store_row<kVec>(out + i * p.dim, zero_row<kVec>());
+      t += count;
+      continue;
+    }
     Row<kVec> rows[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (b0 + i < limit_most) rows[i] = load_row<kVec>(p.x + (b0 + i) * p.x_row + channel);
+      if (i < count) rows[i] = load_row<kVec>(x + i * p.x_row);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int64_t t = b0 + i;
-      if (t >= limit) break;
-      if (t >= at.end) {  // first token of the tile, or of another request
-        while (r < p.n_requests && p.cu[r + 1] <= t) ++r;
-        if (r >= p.n_requests) return;  // rows behind the last request stay as they are
-        if (p.cu[r] > t || p.cu[r] < 0 || p.cu[r + 1] > p.n_tokens) {
-          if (report && p.cu[r] <= t) atomicOr(&g_conv_prefill_faults, LD_FAULT_DECODE_TOKENS);
-          continue;  // rows of no request
+      if (i < count) {
+        Row<kVec> y;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+          float acc = bias[c];
+#pragma unroll
+          for (int j = 0; j < kWidth - 1; ++j) acc = fmaf(__bfloat162float(window[j].v[c]), wt[j][c], acc);
+          acc = fmaf(__bfloat162float(rows[i].v[c]), wt[kWidth - 1][c], acc);
+          // The fast exponential and division are within a few fp32 ulps, far below bf16's rounding.
+          y.v[c] = __float2bfloat16_rn(__fdividef(acc, 1.0f + __expf(-acc)));
         }
-        enter(p, r, t, report, at);
-        if (t == at.begin) limit = max(limit, min(at.end, t + kWidth - 1));
-        if (at.ok) {
+        store_row<kVec>(out + i * p.dim, y);
 #pragma unroll
-          for (int j = 0; j < kWidth - 1; ++j) window[j] = earlier<kVec, kWidth>(p, at, t, kWidth - 1 - j, channel);
-          if (t == at.begin && at.kept >= 0) {
-            // This thread has read the source slot, which is the request's first destination too:
-            // it writes it now, whichever tile its block's last token lies in.
-            const int64_t stop = min(at.end, at.begin + static_cast<int64_t>(at.kept + 1) * p.block_size - at.context);
-            Row<kVec> last[kWidth - 1];
+        for (int j = 0; j + 1 < kWidth - 1; ++j) window[j] = window[j + 1];
+        window[kWidth - 2] = rows[i];
+      }
+    }
+    t += count;
+    if (t == at.next_end) {
+      const int64_t block = (at.context + (t - 1 - at.begin)) / p.block_size;
+      if (block != at.kept) {
+        const int32_t slot = at.row[block];
+        if (slot > 0 && slot < p.n_slots) {
 #pragma unroll
-            for (int j = 0; j < kWidth - 1; ++j) last[j] = earlier<kVec, kWidth>(p, at, stop, kWidth - 1 - j, channel);
-#pragma unroll
-            for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, at.source, channel, j, last[j]);
-          }
+          for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, slot, channel, j, window[j]);
+        } else if (slot >= p.n_slots && report) {
+          atomicOr(&g_conv_prefill_faults, LD_FAULT_CONV_SLOT_RANGE);
         }
       }
-      __nv_bfloat16* out = p.out + t * p.dim + channel;
-      if (!at.ok) {
-        store_row<kVec>(out, zero_row<kVec>());
-        continue;
-      }
-      Row<kVec> y;
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) {
-        float acc = bias[c];
-#pragma unroll
-        for (int j = 0; j < kWidth - 1; ++j) acc = fmaf(__bfloat162float(window[j].v[c]), wt[j][c], acc);
-        acc = fmaf(__bfloat162float(rows[i].v[c]), wt[kWidth - 1][c], acc);
-        // The fast exponential and division are within a few fp32 ulps, far below bf16's rounding.
-        y.v[c] = __float2bfloat16_rn(__fdividef(acc, 1.0f + __expf(-acc)));
-      }
-      store_row<kVec>(out, y);
-#pragma unroll
-      for (int j = 0; j + 1 < kWidth - 1; ++j) window[j] = window[j + 1];
-      window[kWidth - 2] = rows[i];
-      if (t + 1 == at.next_end) {
-        const int64_t position = at.context + (t - at.begin);
-        const int64_t block = position / p.block_size;
-        if (block != at.kept) {
-          const int32_t slot = at.row[block];
-          if (slot > 0 && slot < p.n_slots) {
-#pragma unroll
-            for (int j = 0; j < kWidth - 1; ++j) store_window<kVec>(p, slot, channel, j, window[j]);
-          } else if (slot >= p.n_slots && report) {
-            atomicOr(&g_conv_prefill_faults, LD_FAULT_CONV_SLOT_RANGE);
-          }
-        }
-        at.next_end = min(at.end, at.next_end + p.block_size);
-      }
+      at.next_end = min(at.end, at.next_end + p.block_size);
     }
   }
 }
@@ -269,12 +276,13 @@ bool aligned(const void* ptr, uintptr_t bytes) { return (reinterpret_cast<uintpt
 
 template <int kWidth>
 cudaError_t launch_width(ConvPrefillArgs& args, bool vec, cudaStream_t stream) {
-  const int64_t groups = (args.dim + (vec ? 8 : 1) * kThreads - 1) / ((vec ? 8 : 1) * kThreads);
+  const int channels = (vec ? kVector : 1) * kThreads;
+  const int64_t groups = (args.dim + channels - 1) / channels;
   // 32 tokens per thread read 3 rows of 35 twice; 8 tokens per thread spread short batches over the SMs.
   args.tile = args.n_tokens * groups >= 32 * 4 * 148 ? 32 : 8;
   const dim3 grid(static_cast<unsigned int>((args.n_tokens + args.tile - 1) / args.tile),
                   static_cast<unsigned int>(groups));
-  if (vec) return launch(conv_prefill_kernel<8, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
+  if (vec) return launch(conv_prefill_kernel<kVector, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
   return launch(conv_prefill_kernel<1, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
 }
 
@@ -361,7 +369,7 @@ extern "C" int ld_conv_prefill(const void* x, int64_t x_row_stride, int64_t n_to
   args.n_requests = static_cast<int>(n_requests);
   args.tile = 0;
   args.out = static_cast<__nv_bfloat16*>(out);
-  const bool vec = dim % 8 == 0 && aligned(x, 16) && x_row_stride % 8 == 0 && aligned(out, 16);
+  const bool vec = dim % kVector == 0 && aligned(x, 8) && x_row_stride % kVector == 0 && aligned(out, 8);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t err;
   switch (conv_width) {

@@ -302,40 +302,32 @@ __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row
   }
 }
 
-// Scales one piece of a row from bf16 to fp16 in place (exact: a power of two per row brings the largest
-// magnitude to [1, 2)) and leaves the row's factor, its L2 norm's reciprocal times that power.
-__device__ __forceinline__ void scale_row(uint16_t* tile, float* factor, int i, int part) {
-  uint16_t* piece = tile + swz<kDim>(i, part * 8);
-  const uint4 raw = *reinterpret_cast<const uint4*>(piece);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
-  float sum = 0.0f, top = 0.0f;
+// Scales one row from bf16 to fp16 in place, by one thread: exact, since a power of two brings the row's
+// largest magnitude to [1, 2).  Returns that power's inverse.
+__device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
+  uint16_t* row = tile + i * kDim;
+  uint32_t top2 = 0;  // the largest magnitudes so far of even and odd columns; bf16 magnitudes order as integers
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = __uint_as_float(w[e] << 16);
-    x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+  for (int piece = 0; piece < kDim / 8; ++piece) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(row + ((piece ^ (i & 7)) << 3));
+    top2 = __vmaxu2(__vmaxu2(top2, raw.x & 0x7fff7fffu), raw.y & 0x7fff7fffu);
+    top2 = __vmaxu2(__vmaxu2(top2, raw.z & 0x7fff7fffu), raw.w & 0x7fff7fffu);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    sum = fmaf(x[e], x[e], sum);
-    top = fmaxf(top, fabsf(x[e]));
-  }
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  }
-  int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xff);
-  e = min(max(e, 1), 253);
+  const int e = min(max(static_cast<int>(max(top2 >> 16, top2 & 0xffffu) >> 7), 1), 253);
   const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
-  const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
-  uint4 y;
-  y.x = pack_half(x[0] * down, x[1] * down);
-  y.y = pack_half(x[2] * down, x[3] * down);
-  y.z = pack_half(x[4] * down, x[5] * down);
-  y.w = pack_half(x[6] * down, x[7] * down);
-  *reinterpret_cast<uint4*>(piece) = y;
-  if (part == 0) factor[i] = up * rsqrtf(sum + 1e-6f);
+#pragma unroll
+  for (int piece = 0; piece < kDim / 8; ++piece) {
+    uint4* at = reinterpret_cast<uint4*>(row + ((piece ^ (i & 7)) << 3));
+    const uint4 raw = *at;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t y[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      y[n] = pack_half(__uint_as_float(w[n] << 16) * down, __uint_as_float(w[n] & 0xffff0000u) * down);
+    }
+    *at = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
 }
 
 // g and beta of the chunk's tokens for one value head and G's running sums (in powers of two), by one
@@ -384,8 +376,10 @@ __device__ __forceinline__ void chunk_gates(const PrefillArgs& p, PairSmem& s, i
   }
 }
 
-// Products of this warp's 16 rows of k~ and q~ with the rows of k~ up to its own.
-__device__ __forceinline__ void row_products(const PairSmem& s, int w, int lane, float (&kk)[4][2][4],
+// Products of this warp's 16 rows of k~ and q~ with the rows of k~ up to its own, and the rows' factors
+// (the L2 norm's reciprocal times the power of two that the scaling took) from the diagonals of k~ k~^T
+// and q~ q~^T.
+__device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float (&kk)[4][2][4],
                                              float (&qk)[4][2][4]) {
   const uint32_t k_a = lane_addr<kDim, true>(s.k, lane) + w * 16 * kDim * 2;
   const uint32_t q_a = lane_addr<kDim, true>(s.q, lane) + w * 16 * kDim * 2;
@@ -398,11 +392,15 @@ __device__ __forceinline__ void row_products(const PairSmem& s, int w, int lane,
       for (int e = 0; e < 4; ++e) kk[nb][m][e] = qk[nb][m][e] = 0.0f;
     }
   }
+  float qq[2][4] = {};
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) {
     uint32_t ak[4], aq[4];
     ldsm4(block<kDim>(k_a, 0, ks), ak);
     ldsm4(block<kDim>(q_a, 0, ks), aq);
+    // A fragments are (rows 0-7, cols 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15): as B, rows 0-7 are 0, 2.
+    mma(qq[0], aq, aq[0], aq[2]);
+    mma(qq[1], aq, aq[1], aq[3]);
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) {
       if (nb <= w) {
@@ -414,6 +412,23 @@ __device__ __forceinline__ void row_products(const PairSmem& s, int w, int lane,
           mma(qk[nb][m], aq, b[2 * m], b[2 * m + 1]);
         }
       }
+    }
+  }
+  // Element (g, g) of the diagonal block is with t = g / 2 (of 8 columns), and (g + 8, g + 8) likewise.
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float k2 = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) {
+      if (nb == w) k2 = (g & 1) ? kk[nb][half][2 * half + 1] : kk[nb][half][2 * half];
+    }
+    const float q2 = (g & 1) ? qq[half][2 * half + 1] : qq[half][2 * half];
+    if (t == g / 2) {
+      const int i = 16 * w + g + 8 * half;
+      const float up_k = s.fk[i], up_q = s.fq[i];
+      s.fk[i] = up_k * rsqrtf(k2 * up_k * up_k + 1e-6f);
+      s.fq[i] = up_q * rsqrtf(q2 * up_q * up_q + 1e-6f);
     }
   }
 }
@@ -630,10 +645,11 @@ __global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(cons
   const int head0 = kh * p.heads_ratio;
   if (w < p.heads_ratio) chunk_gates(p, s, w, token0, row_lo, row_hi, head0 + w, lane);
   if constexpr (kVec) cp_async_wait();
-#pragma unroll 2
-  for (int pass = 0; pass < kChunk / 8; ++pass) {  // each thread scales the pieces that it loaded
-    scale_row(reinterpret_cast<uint16_t*>(s.k), s.fk, pass * 8 + (tid >> 4), tid & 15);
-    scale_row(reinterpret_cast<uint16_t*>(s.q), s.fq, pass * 8 + (tid >> 4), tid & 15);
+  __syncthreads();
+  if (tid < kChunk) {
+    s.fk[tid] = scale_row(reinterpret_cast<uint16_t*>(s.k), tid);
+  } else {
+    s.fq[tid - kChunk] = scale_row(reinterpret_cast<uint16_t*>(s.q), tid - kChunk);
   }
   __syncthreads();
   {
@@ -649,6 +665,7 @@ __global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(cons
   }
   float kk[4][2][4], qk[4][2][4];
   row_products(s, w, lane, kk, qk);
+  __syncthreads();
 #pragma unroll 1
   for (int n = 0; n < p.heads_ratio; ++n) {
     const int at = n % kGroup;
@@ -694,18 +711,22 @@ struct ChainSmem {
   __align__(16) float o[kChunk * kORow];
 };
 
+template <typename Image>
+__device__ __forceinline__ void copy_image(Image& to, const Image* from, int tid) {
+  constexpr int kPieces = sizeof(Image) / 16, kWhole = kPieces / kCopyThreads;
+  const uint32_t dst = smem_u32(&to) + 16 * tid;
+  const unsigned char* src = reinterpret_cast<const unsigned char*>(from) + 16 * tid;
+#pragma unroll
+  for (int i = 0; i < kWhole; ++i) cp_async16(dst + 16 * kCopyThreads * i, src + 16 * kCopyThreads * i);
+  if (tid < kPieces % kCopyThreads) cp_async16(dst + 16 * kCopyThreads * kWhole, src + 16 * kCopyThreads * kWhole);
+}
+
 template <bool kVec>
 __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Request& rq, int64_t chunk,
                                            int64_t place, int head, int tid) {
   const int kh = head / p.heads_ratio;
-  const uint4* key = reinterpret_cast<const uint4*>(p.keys + place * p.num_k_heads + kh);
-  const uint32_t key_to = smem_u32(&st.key);
-#pragma unroll 4
-  for (int i = tid; i < static_cast<int>(sizeof(KeyImage) / 16); i += kCopyThreads) cp_async16(key_to + 16 * i, key + i);
-  const uint4* pair = reinterpret_cast<const uint4*>(p.pairs + place * p.num_v_heads + head);
-  const uint32_t pair_to = smem_u32(&st.pair);
-#pragma unroll 4
-  for (int i = tid; i < static_cast<int>(sizeof(PairImage) / 16); i += kCopyThreads) cp_async16(pair_to + 16 * i, pair + i);
+  copy_image(st.key, p.keys + place * p.num_k_heads + kh, tid);
+  copy_image(st.pair, p.pairs + place * p.num_v_heads + head, tid);
   const int64_t local0 = chunk * kChunk - rq.lead;
   const int row_lo = chunk == 0 ? rq.lead : 0;
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
@@ -761,7 +782,7 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     const float rstd = rsqrtf(sq * (1.0f / kDim) + p.eps);
-    if (i < row_lo || i >= row_hi) continue;
+    const bool live = i >= row_lo && i < row_hi;
     __nv_bfloat16* row = out + static_cast<int64_t>(i) * p.num_v_heads * kDim;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -773,9 +794,11 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
       __nv_bfloat16* at = row + 64 * half;
       if constexpr (kVec) {
         const __nv_bfloat162 lo = __floats2bfloat162_rn(y0, y1), hi = __floats2bfloat162_rn(y2, y3);
-        *reinterpret_cast<uint2*>(at) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-      } else {
+        if (live) {
+          *reinterpret_cast<uint2*>(at) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+      } else if (live) {
         at[0] = __float2bfloat16_rn(y0);
         at[1] = __float2bfloat16_rn(y1);
         at[2] = __float2bfloat16_rn(y2);

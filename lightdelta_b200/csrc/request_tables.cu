@@ -25,7 +25,7 @@
 namespace ldb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 
 __device__ unsigned int g_tables_faults;
 
@@ -46,6 +46,7 @@ struct TablesArgs {
   int n_requests;
   int stretch;  // requests per thread of the scan
   uint32_t block_size;
+  int shift;    // log2(block_size) when it is a power of two, else -1
 };
 
 // Lengths of one request: new and held tokens (negative ones count as 0), held and wanted blocks.
@@ -53,16 +54,22 @@ struct Lengths {
   uint32_t query, context, have, want;
 };
 
-__device__ __forceinline__ uint32_t blocks_of(uint32_t tokens, uint32_t size) {
-  return tokens / size + (tokens % size != 0);
+// Whole blocks in front of a position (a uniform choice: the division is about twenty instructions).
+__device__ __forceinline__ uint32_t block_index(const TablesArgs& p, uint32_t position) {
+  return p.shift >= 0 ? position >> p.shift : position / p.block_size;
+}
+
+__device__ __forceinline__ uint32_t blocks_of(const TablesArgs& p, uint32_t tokens) {
+  const uint32_t whole = block_index(p, tokens);
+  return whole + (whole * p.block_size != tokens);
 }
 
 __device__ __forceinline__ Lengths lengths_of(const TablesArgs& p, int r) {
   Lengths l;
   l.query = static_cast<uint32_t>(max(p.query[r], 0));
   l.context = static_cast<uint32_t>(max(p.context[r], 0));
-  l.have = blocks_of(l.context, p.block_size);
-  l.want = blocks_of(l.context + l.query, p.block_size);  // two int32: no wrap
+  l.have = blocks_of(p, l.context);
+  l.want = blocks_of(p, l.context + l.query);  // two int32: no wrap
   return l;
 }
 
@@ -106,6 +113,7 @@ __global__ void __launch_bounds__(kThreads) request_tables_kernel(const TablesAr
   // This thread's stretch, then the sums in front of it.
   unsigned int fault = 0;
   int64_t tokens = 0, blocks = 0;
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) {
     const Lengths l = lengths_of(p, r);
     tokens += l.query;
@@ -141,16 +149,6 @@ __global__ void __launch_bounds__(kThreads) request_tables_kernel(const TablesAr
   const int64_t all_tokens = s.tokens[kThreads], all_blocks = s.blocks[kThreads];
 
   if (blockIdx.x == 0) {
-    // Offsets and state slots, by the thread that scanned the request.
-    int64_t at = s.tokens[tid], first = s.blocks[tid];
-    for (int r = r0; r < r1; ++r) {
-      const Lengths l = lengths_of(p, r);
-      p.cu[r] = static_cast<int32_t>(min(at, static_cast<int64_t>(INT32_MAX)));
-      p.state_slots[2 * r] = l.query > 0 ? block_of(p, r, l.want - 1, l, first) : 0;
-      p.state_slots[2 * r + 1] = l.context > 0 ? block_of(p, r, l.have - 1, l, first) : 0;
-      at += l.query;
-      first += l.want - l.have;
-    }
     if (tid == 0) {
       p.cu[p.n_requests] = static_cast<int32_t>(min(all_tokens, static_cast<int64_t>(INT32_MAX)));
       p.used[0] = static_cast<int32_t>(min(all_blocks, static_cast<int64_t>(INT32_MAX)));
@@ -162,6 +160,19 @@ __global__ void __launch_bounds__(kThreads) request_tables_kernel(const TablesAr
 
   const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = start; i < p.n_requests; i += step) {  // offsets and state slots
+    const int r = static_cast<int>(i), f = r / p.stretch;
+    int64_t at = s.tokens[f], first = s.blocks[f];
+    for (int k = f * p.stretch; k < r; ++k) {
+      const Lengths l = lengths_of(p, k);
+      at += l.query;
+      first += l.want - l.have;
+    }
+    const Lengths l = lengths_of(p, r);
+    p.cu[r] = static_cast<int32_t>(min(at, static_cast<int64_t>(INT32_MAX)));
+    p.state_slots[2 * r] = l.query > 0 ? block_of(p, r, l.want - 1, l, first) : 0;
+    p.state_slots[2 * r + 1] = l.context > 0 ? block_of(p, r, l.have - 1, l, first) : 0;
+  }
   for (int64_t i = start; i < all_blocks; i += step) {
     const int f = find_stretch(s.blocks, i);
     int r = f * p.stretch;
@@ -187,9 +198,10 @@ __global__ void __launch_bounds__(kThreads) request_tables_kernel(const TablesAr
         l = lengths_of(p, ++r);
       }
       const uint32_t pos = l.context + static_cast<uint32_t>(i - at);
-      const int32_t block = block_of(p, r, pos / p.block_size, l, first);
+      const uint32_t index = block_index(p, pos);
+      const int32_t block = block_of(p, r, index, l, first);
       position = pos;
-      if (block > 0) slot = static_cast<int64_t>(block) * p.block_size + pos % p.block_size;
+      if (block > 0) slot = static_cast<int64_t>(block) * p.block_size + (pos - index * p.block_size);
     }
     p.positions[i] = position;
     p.slot_map[i] = slot;
@@ -261,8 +273,13 @@ extern "C" int ld_request_tables(const int32_t* query_lens, const int32_t* conte
   args.n_requests = static_cast<int>(n_requests);
   args.stretch = static_cast<int>(std::max<int64_t>((n_requests + kThreads - 1) / kThreads, 1));
   args.block_size = static_cast<uint32_t>(block_size);
-  // Two tokens per thread, at most one wave of two CTAs per SM.
-  const int64_t ctas = std::min<int64_t>(std::max<int64_t>((n_tokens + 2 * kThreads - 1) / (2 * kThreads), 1), 296);
+  args.shift = -1;
+  for (int bit = 0; bit <= 30; ++bit) {
+    if (block_size == 1LL << bit) args.shift = bit;
+  }
+  // One item per thread, at most one wave of two CTAs per SM.
+  const int64_t items = std::max<int64_t>(std::max(n_tokens, n_requests), 1);
+  const int64_t ctas = std::min<int64_t>((items + kThreads - 1) / kThreads, 296);
   const cudaError_t err = launch(request_tables_kernel, dim3(static_cast<unsigned int>(ctas)), dim3(kThreads), 0,
                                  static_cast<cudaStream_t>(stream), 1, args);
   if (err != cudaSuccess) return set_error(LD_ERR_CUDA, "request tables launch failed: %s", cudaGetErrorString(err));
