@@ -34,7 +34,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompil
 
 CAPI_SOURCES = ["gdn_decode.cu", "state_io.cu", "greedy_verify.cu", "conv_update.cu", "decode_noalloc.cu",
                 "request_tables.cu", "conv_prefill.cu", "prefill.cu", "capi.cpp"]
-CAPI_HEADERS = ["internal.h", "launch.cuh", "exports.map"]
+CAPI_HEADERS = ["internal.h", "launch.cuh", "math.cuh", "exports.map"]
 
 
 def cuda_home() -> Path:

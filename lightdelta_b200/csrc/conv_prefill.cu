@@ -24,6 +24,7 @@
 #include "internal.h"
 #include "launch.cuh"
 #include "lightdelta_b200.h"
+#include "math.cuh"
 
 namespace ldb {
 namespace {
@@ -52,18 +53,22 @@ struct ConvPrefillArgs {
   __nv_bfloat16* out;
 };
 
+// kVec consecutive channels of one token: bf16 pairs in memory order (one channel alone: the low half).
 template <int kVec>
-struct __align__(2 * kVec) Row {  // kVec consecutive bf16 channels of one token
-  __nv_bfloat16 v[kVec];
+struct Row {
+  static constexpr int kWords = (kVec + 1) / 2;
+  uint32_t w[kWords];
 };
 
 template <int kVec>
 __device__ __forceinline__ Row<kVec> load_row(const __nv_bfloat16* at) {
   Row<kVec> r;
   if constexpr (kVec == 4) {
-    *reinterpret_cast<uint2*>(r.v) = *reinterpret_cast<const uint2*>(at);
+    const uint2 raw = *reinterpret_cast<const uint2*>(at);
+    r.w[0] = raw.x;
+    r.w[1] = raw.y;
   } else {
-    r.v[0] = *at;
+    r.w[0] = __bfloat16_as_ushort(*at);
   }
   return r;
 }
@@ -71,9 +76,9 @@ __device__ __forceinline__ Row<kVec> load_row(const __nv_bfloat16* at) {
 template <int kVec>
 __device__ __forceinline__ void store_row(__nv_bfloat16* at, const Row<kVec>& r) {
   if constexpr (kVec == 4) {
-    *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(r.v);
+    *reinterpret_cast<uint2*>(at) = make_uint2(r.w[0], r.w[1]);
   } else {
-    *at = r.v[0];
+    *at = __ushort_as_bfloat16(static_cast<unsigned short>(r.w[0]));
   }
 }
 
@@ -81,7 +86,7 @@ template <int kVec>
 __device__ __forceinline__ Row<kVec> zero_row() {
   Row<kVec> r;
 #pragma unroll
-  for (int c = 0; c < kVec; ++c) r.v[c] = __float2bfloat16_rn(0.0f);
+  for (int i = 0; i < Row<kVec>::kWords; ++i) r.w[i] = 0;
   return r;
 }
 
@@ -89,9 +94,11 @@ __device__ __forceinline__ Row<kVec> zero_row() {
 template <int kVec>
 __device__ __forceinline__ Row<kVec> load_window(const ConvPrefillArgs& p, int32_t slot, int64_t channel, int position) {
   const __nv_bfloat16* at = p.state + slot * p.s_slot + channel * p.s_dim + position * p.s_pos;
-  Row<kVec> r;
+  Row<kVec> r = zero_row<kVec>();
 #pragma unroll
-  for (int c = 0; c < kVec; ++c) r.v[c] = at[c * p.s_dim];
+  for (int c = 0; c < kVec; ++c) {
+    r.w[c / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(at[c * p.s_dim])) << (16 * (c & 1));
+  }
   return r;
 }
 
@@ -100,7 +107,9 @@ __device__ __forceinline__ void store_window(const ConvPrefillArgs& p, int32_t s
                                              const Row<kVec>& r) {
   __nv_bfloat16* at = p.state + slot * p.s_slot + channel * p.s_dim + position * p.s_pos;
 #pragma unroll
-  for (int c = 0; c < kVec; ++c) at[c * p.s_dim] = r.v[c];
+  for (int c = 0; c < kVec; ++c) {
+    at[c * p.s_dim] = __ushort_as_bfloat16(static_cast<unsigned short>(r.w[c / 2] >> (16 * (c & 1))));
+  }
 }
 
 // The request that a thread is in.
@@ -181,12 +190,17 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
   int64_t limit = t1;
   const bool report = channel == 0;
 
-  float wt[kWidth][kVec], bias[kVec];
+  constexpr int kWords = Row<kVec>::kWords;
+  float2 wt[kWidth][kWords], bias[kWords];
 #pragma unroll
-  for (int c = 0; c < kVec; ++c) {
+  for (int i = 0; i < kWords; ++i) {
+    const int64_t c0 = channel + 2 * i, c1 = kVec > 1 ? c0 + 1 : c0;
 #pragma unroll
-    for (int j = 0; j < kWidth; ++j) wt[j][c] = __bfloat162float(p.weight[(channel + c) * kWidth + j]);
-    bias[c] = p.bias != nullptr ? __bfloat162float(p.bias[channel + c]) : 0.0f;
+    for (int j = 0; j < kWidth; ++j) {
+      wt[j][i] = make_float2(__bfloat162float(p.weight[c0 * kWidth + j]), __bfloat162float(p.weight[c1 * kWidth + j]));
+    }
+    bias[i] = p.bias != nullptr ? make_float2(__bfloat162float(p.bias[c0]), __bfloat162float(p.bias[c1]))
+                                : make_float2(0.0f, 0.0f);
   }
 
   Place at;
@@ -241,13 +255,14 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
       if (i < count) {
         Row<kVec> y;
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-          float acc = bias[c];
+        for (int c = 0; c < kWords; ++c) {
+          float2 acc = bias[c];
 #pragma unroll
-          for (int j = 0; j < kWidth - 1; ++j) acc = fmaf(__bfloat162float(window[j].v[c]), wt[j][c], acc);
-          acc = fmaf(__bfloat162float(rows[i].v[c]), wt[kWidth - 1][c], acc);
-          // The fast exponential and division are within a few fp32 ulps, far below bf16's rounding.
-          y.v[c] = __float2bfloat16_rn(__fdividef(acc, 1.0f + __expf(-acc)));
+          for (int j = 0; j < kWidth - 1; ++j) {
+            acc = fma2(make_float2(bf16_low(window[j].w[c]), bf16_high(window[j].w[c])), wt[j][c], acc);
+          }
+          acc = fma2(make_float2(bf16_low(rows[i].w[c]), bf16_high(rows[i].w[c])), wt[kWidth - 1][c], acc);
+          y.w[c] = pack_bf16(silu_fast(acc.x), silu_fast(acc.y));
         }
         store_row<kVec>(out + i * p.dim, y);
 #pragma unroll

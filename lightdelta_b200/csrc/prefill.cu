@@ -23,13 +23,20 @@
 // gdn_prefill_pairs_kernel, one CTA per (chunk, key head), scales q and k, forms their products once for
 // all value heads of the key head, and leaves q, k, T, P and the rows' factors in a workspace, as the
 // images that the second kernel copies to shared memory.  gdn_prefill_chain_kernel, one CTA per
-// (request, value head), then carries the state from chunk to chunk: eight chain warps hold the 128 x
-// 128 state as accumulator fragments, 16 value rows each.  S k, T R and the update all have the state's
-// value rows as M, so every warp carries its rows through all chunks without exchanging anything with
-// the others (an accumulator fragment is the next product's A fragment).  Four more warps copy the next
-// chunk in and normalise and store the chunk before's outputs.  A first form that prepared each chunk
-// inside the chain's CTA took 1,242 us on 24 prompts of 16,000 tokens in all (16 key, 32 value heads):
-// its preparation, 33,000 cycles a chunk of short dependent steps, held the chain's 10,500 up.
+// (request, value head), then carries the state from chunk to chunk on the tensor cores' tcgen05
+// instructions, value rows as the M = 128 of every product:
+//   Y = S k~, O = S q~   A = S hi, lo in TMEM      B = k~, q~ (K-major)
+//   U = T R              A = R hi, lo in TMEM      B = T hi, lo
+//   P u                  A = u hi in TMEM          B = P
+//   dS = u k~            A = k_out u hi, lo        B = the same k~ tile, read MN-major
+// Eight chain warps keep the fp32 state in registers, 16 value rows each, in the layout that 16-lane TMEM
+// loads and stores use; between products they scale, split and store the next A operand.  Four warps copy
+// the next chunk in, four normalise and store the chunk before's outputs.
+//
+// History of the split, 24 prompts of 16,000 tokens in all, 16 key and 32 value heads (and one prompt of
+// 16,384): one kernel that prepared each chunk inside the chain's CTA, 1,242 us (4,878); pairs apart and the
+// chain on mma.sync with the state as its fragments, 555 us (1,646): 11,200 cycles a chunk, of which the
+// 3,200 mma.sync of a chunk are 6,400.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -40,6 +47,7 @@
 #include "internal.h"
 #include "launch.cuh"
 #include "lightdelta_b200.h"
+#include "math.cuh"
 
 namespace ldb {
 namespace {
@@ -47,19 +55,22 @@ namespace {
 constexpr int kDim = LD_HEAD_DIM;
 constexpr int kChunk = LD_PREFILL_CHUNK;
 constexpr int kPairThreads = 128;
-constexpr int kCopyThreads = 128;
-constexpr int kChainWarps = 8;
-constexpr int kChainThreads = kCopyThreads + 32 * kChainWarps;
+constexpr int kMoveThreads = 256;   // chain kernel: warps 0-7 copy chunks in and store outputs,
+constexpr int kStateThreads = 256;  // warps 8-15 carry the state
+constexpr int kChainThreads = kMoveThreads + kStateThreads;
+constexpr uint64_t kWaitNs = 1000000000;  // bound of every in-kernel wait
 constexpr int kORow = kDim + 4;  // floats per row of the output tile: the +4 spreads its rows over the banks
 static_assert(kChunk == 64, "fragment loops below are written for chunks of 64 tokens");
 
+constexpr int kHalf = kChunk * 64;    // elements of half a 128-column tile
+constexpr int kKeyHalf = 2 * kHalf;   // from a half of k (or q) to its other half
+
 __device__ unsigned int g_prefill_faults;
 
-// Workspace images.  Tiles of 128 columns are swizzled (swz), triangular matrices are packed 16 x 16
-// blocks (tri), exactly as the chain reads them from shared memory.
+// Workspace images.  Tiles of 128 columns are swizzled (swz) as the chain's products read them; triangular
+// matrices are packed 16 x 16 blocks (tri), which the chain's copies spread to swizzled tiles.
 struct __align__(128) KeyImage {  // per (chunk, key head)
-  __half k[kChunk * kDim];        // k rows x 2^-e
-  __half q[kChunk * kDim];        // q rows x 2^-e
+  __half kq[2 * kChunk * kDim];   // columns 0-63 of k x 2^-e, then of q x 2^-e, then columns 64-127 likewise
 };
 
 constexpr int kTriBlocks = 10;  // 16 x 16 blocks on and below the diagonal of a 64 x 64 matrix
@@ -156,12 +167,86 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Named barriers of the chain kernel: the first three hand buffers between the threads that move data and
+// those that carry the state, kBarState joins the latter.
+constexpr int kBarFull = 1, kBarOReady = 3, kBarOFree = 4, kBarState = 5;
 __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory");
 }
-// Named barriers of the chain kernel, which hand its buffers over (two each of full and empty).
-constexpr int kBarFull = 1, kBarEmpty = 3, kBarOReady = 5, kBarOFree = 6;
+__device__ __forceinline__ void bar_state() {
+  asm volatile("bar.sync %0, %1;" ::"n"(kBarState), "n"(kStateThreads) : "memory");
+}
+
+// ---- tcgen05: products with A and D in TMEM and B in shared memory.  One warp calls, with the same values in
+// every lane, and its elected lane issues.
+// Instruction descriptor of kind::f16: fp16 A and B, fp32 D, M = 128; bit 16 reads B MN-major.
+__host__ __device__ constexpr uint32_t mma_shape(int n, bool b_mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24) | (b_mn_major ? 1u << 16 : 0u);
+}
+
+// Shared-memory descriptor of a 128-byte swizzled tile: atoms of 8 rows x 128 bytes, 1024 bytes apart along
+// the rows; 64-column halves (MN-major only) kKeyHalf apart.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(2 * kKeyHalf >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+  return elected;
+}
+
+// D[128 x n] (+)= A[128 x 16] B[16 x n].
+__device__ __forceinline__ void umma(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t shape,
+                                     bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(accumulate)), "r"(elected)
+      : "memory");
+}
+
+// The barrier's phase completes when every product issued so far has.
+__device__ __forceinline__ void umma_commit(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(elected)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 64 fp32 columns of this warp's 16 lanes, as eight accumulator fragments (row g: columns 8n + 2t, + 1 in
+// elements 0, 1; row g + 8 in 2, 3).  Loads and their wait are one statement, so nothing reads too early.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&r)[8][4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0][0]), "=f"(r[0][1]), "=f"(r[0][2]), "=f"(r[0][3]), "=f"(r[1][0]), "=f"(r[1][1]), "=f"(r[1][2]),
+        "=f"(r[1][3]), "=f"(r[2][0]), "=f"(r[2][1]), "=f"(r[2][2]), "=f"(r[2][3]), "=f"(r[3][0]), "=f"(r[3][1]),
+        "=f"(r[3][2]), "=f"(r[3][3]), "=f"(r[4][0]), "=f"(r[4][1]), "=f"(r[4][2]), "=f"(r[4][3]), "=f"(r[5][0]),
+        "=f"(r[5][1]), "=f"(r[5][2]), "=f"(r[5][3]), "=f"(r[6][0]), "=f"(r[6][1]), "=f"(r[6][2]), "=f"(r[6][3]),
+        "=f"(r[7][0]), "=f"(r[7][1]), "=f"(r[7][2]), "=f"(r[7][3])
+      : "r"(addr)
+      : "memory");
+}
+
+// Four k-steps of packed A fragments to 32 columns of this warp's 16 lanes.
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&a)[4][4]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(a[0][0]), "r"(a[0][1]), "r"(a[0][2]), "r"(a[0][3]), "r"(a[1][0]), "r"(a[1][1]), "r"(a[1][2]), "r"(a[1][3]),
+      "r"(a[2][0]), "r"(a[2][1]), "r"(a[2][2]), "r"(a[2][3]), "r"(a[3][0]), "r"(a[3][1]), "r"(a[3][2]), "r"(a[3][3])
+      : "memory");
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   const int bytes = live ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
@@ -173,31 +258,30 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------
-// swizzled tiles: 16-byte pieces of a row are stored at piece ^ (row mod 8), so that the eight rows
-// of an 8 x 8 matrix lie in different banks
+// swizzled tiles: 64 rows of 64 16-bit columns, 128 bytes a row, whose 16-byte pieces are stored at
+// piece ^ (row mod 8): the 128-byte swizzle of matrix descriptors, free of bank conflicts for ldmatrix too.
+// A 128-column tile is two such halves, kStride elements apart (kKeyHalf for k and q, which alternate).
 // ------------------------------------------------------------------------------------------
-template <int kCols>
+template <int kStride>
 __device__ __forceinline__ int swz(int row, int col) {
-  constexpr int kPieces = kCols / 8;
-  static_assert(kPieces >= 8, "rows of eight pieces at least");
-  return row * kCols + ((((col >> 3) ^ (row & 7)) << 3) | (col & 7));
+  return (col >> 6) * kStride + row * 64 + (((((col >> 3) & 7) ^ (row & 7)) << 3) | (col & 7));
 }
 
 // Address that this lane gives to ldmatrix.x4 for the 16 x 16 block at (0, 0) of a tile: matrices in the
 // order (rows 0-7, cols 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15), or with kRowsFirst
 // (0-7, 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15).  Row blocks start at multiples of 8, so the swizzle
-// depends on the lane alone and the block at (16 rb, 16 cb) is at block<kCols>(address, rb, cb).
-template <int kCols, bool kRowsFirst>
+// depends on the lane alone and the block at (16 rb, 16 cb) is at block<kStride>(address, rb, cb).
+template <bool kRowsFirst>
 __device__ __forceinline__ uint32_t lane_addr(const void* tile, int lane) {
   const int m = lane >> 3;
   const int row = (lane & 7) + 8 * (kRowsFirst ? (m & 1) : (m >> 1));
   const int piece = (kRowsFirst ? (m >> 1) : (m & 1)) ^ (lane & 7);
-  return smem_u32(tile) + row * kCols * 2 + (piece << 4);
+  return smem_u32(tile) + row * 128 + (piece << 4);
 }
 
-template <int kCols>
+template <int kStride>
 __device__ __forceinline__ uint32_t block(uint32_t addr, int rb, int cb) {
-  return (addr ^ (cb << 5)) + rb * (16 * kCols * 2);
+  return (addr ^ ((cb & 3) << 5)) + (cb >> 2) * (2 * kStride) + rb * (16 * 128);
 }
 
 // Packed triangular matrices: block (ib, jb), jb <= ib, of 16 rows of 32 bytes; the two 16-byte pieces of
@@ -219,11 +303,12 @@ __device__ __forceinline__ uint32_t pack_half(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// x, y as two fp16 terms: hi the nearest, lo the nearest to what hi leaves.
-__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
+// x.x, x.y as two fp16 terms: hi the nearest, lo the nearest to what hi leaves.
+__device__ __forceinline__ void split(float2 x, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  const float2 r = add2(x, make_float2(-f.x, -f.y));
+  const __half2 l = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -250,31 +335,27 @@ __device__ __forceinline__ float load_param(const void* p, int index, int is_bf1
 
 __device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 
-// 2^x of non-positive x, within 2 ulp of the fp32 value (0 below 2^-126).
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// z sigmoid(z) with the fast exponential and division: a few fp32 ulps, far below bf16's rounding.
-__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
-
 // ------------------------------------------------------------------------------------------
 // pairs: what a chunk's tokens mean to one another
 // ------------------------------------------------------------------------------------------
 constexpr int kGroup = 4;  // value heads whose gates are computed together, one per warp
 
-struct PairSmem {
-  __align__(256) __half k[kChunk * kDim];
-  __align__(256) __half q[kChunk * kDim];
+struct PairWork {
   PairImage image;
-  __align__(128) __half l_hi[6 * 256];  // L's blocks below the diagonal ones, packed row by row
+  __align__(128) __half l_hi[6 * 256];   // L's blocks below the diagonal ones, packed row by row
   __align__(128) __half l_lo[6 * 256];
   __align__(16) float diag[4][16 * 16];  // L's diagonal blocks
+};
+
+struct PairSmem {
+  __align__(1024) unsigned char tiles[sizeof(KeyImage)];  // the key image, then, its products in registers, PairWork
   float g_hi[kGroup][kChunk], g_lo[kGroup][kChunk], beta[kGroup][kChunk];
   float fk[kChunk], fq[kChunk];
+
+  __device__ __forceinline__ __half* kq() { return reinterpret_cast<__half*>(tiles); }
+  __device__ __forceinline__ PairWork& work() { return *reinterpret_cast<PairWork*>(tiles); }
 };
+static_assert(sizeof(PairWork) <= sizeof(KeyImage), "the work area takes the tiles' place");
 
 // Element (row, col) of a block strictly below the diagonal of the packed L, and the byte offset of a block.
 __host__ __device__ constexpr int low_block(int ib, int jb) { return (ib * (ib - 1) / 2 + jb) * 512; }
@@ -283,15 +364,15 @@ __device__ __forceinline__ int low(int row, int col) {
   return low_block(row >> 4, col >> 4) / 2 + r * 16 + ((((c >> 3) ^ ((r >> 2) & 1)) << 3) | (c & 7));
 }
 
-template <bool kVec>
+template <bool kVec, int kThreads, int kStride>
 __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row_stride, int row_lo, int row_hi,
                                           uint16_t* tile, int tid) {
 #pragma unroll
-  for (int pass = 0; pass < kChunk / 8; ++pass) {
-    const int i = pass * 8 + (tid >> 4);
+  for (int pass = 0; pass < kChunk / (kThreads / 16); ++pass) {
+    const int i = pass * (kThreads / 16) + (tid >> 4);
     const int col = (tid & 15) * 8;
     const bool live = i >= row_lo && i < row_hi;
-    uint16_t* dst = tile + swz<kDim>(i, col);
+    uint16_t* dst = tile + swz<kStride>(i, col);
     const __nv_bfloat16* src = base + static_cast<int64_t>(live ? i : row_lo) * row_stride + col;
     if constexpr (kVec) {
       cp_async16(smem_u32(dst), src, live);
@@ -305,11 +386,11 @@ __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row
 // Scales one row from bf16 to fp16 in place, by one thread: exact, since a power of two brings the row's
 // largest magnitude to [1, 2).  Returns that power's inverse.
 __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
-  uint16_t* row = tile + i * kDim;
+  uint16_t* row = tile + i * 64;
   uint32_t top2 = 0;  // the largest magnitudes so far of even and odd columns; bf16 magnitudes order as integers
 #pragma unroll
   for (int piece = 0; piece < kDim / 8; ++piece) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(row + ((piece ^ (i & 7)) << 3));
+    const uint4 raw = *reinterpret_cast<const uint4*>(row + (piece >> 3) * kKeyHalf + (((piece & 7) ^ (i & 7)) << 3));
     top2 = __vmaxu2(__vmaxu2(top2, raw.x & 0x7fff7fffu), raw.y & 0x7fff7fffu);
     top2 = __vmaxu2(__vmaxu2(top2, raw.z & 0x7fff7fffu), raw.w & 0x7fff7fffu);
   }
@@ -317,7 +398,7 @@ __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
   const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
 #pragma unroll
   for (int piece = 0; piece < kDim / 8; ++piece) {
-    uint4* at = reinterpret_cast<uint4*>(row + ((piece ^ (i & 7)) << 3));
+    uint4* at = reinterpret_cast<uint4*>(row + (piece >> 3) * kKeyHalf + (((piece & 7) ^ (i & 7)) << 3));
     const uint4 raw = *at;
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t y[4];
@@ -381,9 +462,9 @@ __device__ __forceinline__ void chunk_gates(const PrefillArgs& p, PairSmem& s, i
 // and q~ q~^T.
 __device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float (&kk)[4][2][4],
                                              float (&qk)[4][2][4]) {
-  const uint32_t k_a = lane_addr<kDim, true>(s.k, lane) + w * 16 * kDim * 2;
-  const uint32_t q_a = lane_addr<kDim, true>(s.q, lane) + w * 16 * kDim * 2;
-  const uint32_t k_b = lane_addr<kDim, false>(s.k, lane);
+  const uint32_t k_a = lane_addr<true>(s.kq(), lane) + w * 16 * 128;
+  const uint32_t q_a = lane_addr<true>(s.kq() + kHalf, lane) + w * 16 * 128;
+  const uint32_t k_b = lane_addr<false>(s.kq(), lane);
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
 #pragma unroll
@@ -396,8 +477,8 @@ __device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) {
     uint32_t ak[4], aq[4];
-    ldsm4(block<kDim>(k_a, 0, ks), ak);
-    ldsm4(block<kDim>(q_a, 0, ks), aq);
+    ldsm4(block<kKeyHalf>(k_a, 0, ks), ak);
+    ldsm4(block<kKeyHalf>(q_a, 0, ks), aq);
     // A fragments are (rows 0-7, cols 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15): as B, rows 0-7 are 0, 2.
     mma(qq[0], aq, aq[0], aq[2]);
     mma(qq[1], aq, aq[1], aq[3]);
@@ -405,7 +486,7 @@ __device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float
     for (int nb = 0; nb < 4; ++nb) {
       if (nb <= w) {
         uint32_t b[4];
-        ldsm4(block<kDim>(k_b, nb, ks), b);
+        ldsm4(block<kKeyHalf>(k_b, nb, ks), b);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           mma(kk[nb][m], ak, b[2 * m], b[2 * m + 1]);
@@ -464,14 +545,14 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
         const float l1 = j + 1 < i ? row_k[half] * d1 * kk[nb][m][2 * half + 1] : 0.0f;
         const float p0 = j <= i ? row_q[half] * d0 * qk[nb][m][2 * half] : 0.0f;
         const float p1 = j + 1 <= i ? row_q[half] * d1 * qk[nb][m][2 * half + 1] : 0.0f;
-        *reinterpret_cast<uint32_t*>(&s.image.p[tri(i, j)]) = pack_half(p0, p1);
+        *reinterpret_cast<uint32_t*>(&s.work().image.p[tri(i, j)]) = pack_half(p0, p1);
         if (nb == w) {
-          *reinterpret_cast<float2*>(&s.diag[w][(g + 8 * half) * 16 + (j & 15)]) = make_float2(l0, l1);
+          *reinterpret_cast<float2*>(&s.work().diag[w][(g + 8 * half) * 16 + (j & 15)]) = make_float2(l0, l1);
         } else {
           uint32_t hi, lo;
-          split(l0, l1, hi, lo);
-          *reinterpret_cast<uint32_t*>(&s.l_hi[low(i, j)]) = hi;
-          *reinterpret_cast<uint32_t*>(&s.l_lo[low(i, j)]) = lo;
+          split(make_float2(l0, l1), hi, lo);
+          *reinterpret_cast<uint32_t*>(&s.work().l_hi[low(i, j)]) = hi;
+          *reinterpret_cast<uint32_t*>(&s.work().l_lo[low(i, j)]) = lo;
         }
       }
     }
@@ -487,7 +568,7 @@ __device__ __forceinline__ void invert_diagonal(PairSmem& s, int w, int lane) {
     float sum0 = i == c ? 1.0f : 0.0f, sum1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < i; ++j) {
-      const float l = s.diag[w][i * 16 + j];
+      const float l = s.work().diag[w][i * 16 + j];
       if (j & 1) {
         sum1 = fmaf(-l, x[j], sum1);
       } else {
@@ -500,8 +581,8 @@ __device__ __forceinline__ void invert_diagonal(PairSmem& s, int w, int lane) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const __half hi = __float2half_rn(x[i]);
-      s.image.t_hi[tri(16 * w + i, 16 * w + c)] = hi;
-      s.image.t_lo[tri(16 * w + i, 16 * w + c)] = __float2half_rn(x[i] - __half2float(hi));
+      s.work().image.t_hi[tri(16 * w + i, 16 * w + c)] = hi;
+      s.work().image.t_lo[tri(16 * w + i, 16 * w + c)] = __float2half_rn(x[i] - __half2float(hi));
     }
   }
 }
@@ -509,8 +590,8 @@ __device__ __forceinline__ void invert_diagonal(PairSmem& s, int w, int lane) {
 // The 16 x 16 blocks of T below diagonal block w, top to bottom:
 //   T_iw = -T_ii sum_{k=w}^{i-1} L_ik T_kw,  held transposed so that each result is the next A operand.
 __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
-  const uint32_t t_hi = tri_addr(s.image.t_hi, lane), t_lo = tri_addr(s.image.t_lo, lane);
-  const uint32_t l_hi = tri_addr(s.l_hi, lane), l_lo = tri_addr(s.l_lo, lane);
+  const uint32_t t_hi = tri_addr(s.work().image.t_hi, lane), t_lo = tri_addr(s.work().image.t_lo, lane);
+  const uint32_t l_hi = tri_addr(s.work().l_hi, lane), l_lo = tri_addr(s.work().l_lo, lane);
   uint32_t x_hi[3][4], x_lo[3][4];  // T_kw^T as A fragments, k = w, w + 1, w + 2
   // ldmatrix.trans of T_ww: matrices (cols 0-7, rows 0-7), (cols 8-15, rows 0-7), (0-7, 8-15), (8-15, 8-15).
   ldsm4_t(t_hi + tri_block(w, w), x_hi[0]);
@@ -536,8 +617,8 @@ __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
       uint32_t a_hi[4], a_lo[4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        split(m[n][0], m[n][1], a_hi[2 * n], a_lo[2 * n]);
-        split(m[n][2], m[n][3], a_hi[2 * n + 1], a_lo[2 * n + 1]);
+        split(make_float2(m[n][0], m[n][1]), a_hi[2 * n], a_lo[2 * n]);
+        split(make_float2(m[n][2], m[n][3]), a_hi[2 * n + 1], a_lo[2 * n + 1]);
       }
       float y[2][4] = {};
       uint32_t b_hi[4], b_lo[4];
@@ -555,14 +636,14 @@ __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          split(-y[n][2 * half], -y[n][2 * half + 1], hi[half], lo[half]);
+          split(make_float2(-y[n][2 * half], -y[n][2 * half + 1]), hi[half], lo[half]);
           const int col = 16 * w + g + 8 * half, row = 16 * i + 8 * n + 2 * t;
           const __half2 h = *reinterpret_cast<const __half2*>(&hi[half]);
           const __half2 l = *reinterpret_cast<const __half2*>(&lo[half]);
-          s.image.t_hi[tri(row, col)] = __low2half(h);
-          s.image.t_hi[tri(row + 1, col)] = __high2half(h);
-          s.image.t_lo[tri(row, col)] = __low2half(l);
-          s.image.t_lo[tri(row + 1, col)] = __high2half(l);
+          s.work().image.t_hi[tri(row, col)] = __low2half(h);
+          s.work().image.t_hi[tri(row + 1, col)] = __high2half(h);
+          s.work().image.t_lo[tri(row, col)] = __low2half(l);
+          s.work().image.t_lo[tri(row + 1, col)] = __high2half(l);
         }
         if (d < 3) {
           x_hi[d < 3 ? d : 0][2 * n] = hi[0];
@@ -608,7 +689,7 @@ __device__ __forceinline__ bool find_request(const PrefillArgs& p, int64_t r, Re
 }
 
 template <bool kVec>
-__global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(const PrefillArgs p) {
+__global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(const PrefillArgs p) {
   extern __shared__ __align__(1024) unsigned char raw[];
   PairSmem& s = *reinterpret_cast<PairSmem*>(raw);
   grid_dependency_wait();
@@ -640,27 +721,25 @@ __global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(cons
   const int row_lo = chunk == 0 ? rq.lead : 0;
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
   const __nv_bfloat16* rows = p.qkv + token0 * p.qkv_row;
-  load_rows<kVec>(rows + (p.num_k_heads + kh) * kDim, p.qkv_row, row_lo, row_hi, reinterpret_cast<uint16_t*>(s.k), tid);
-  load_rows<kVec>(rows + kh * kDim, p.qkv_row, row_lo, row_hi, reinterpret_cast<uint16_t*>(s.q), tid);
+  uint16_t* tiles = reinterpret_cast<uint16_t*>(s.kq());
+  load_rows<kVec, kPairThreads, kKeyHalf>(rows + (p.num_k_heads + kh) * kDim, p.qkv_row, row_lo, row_hi, tiles, tid);
+  load_rows<kVec, kPairThreads, kKeyHalf>(rows + kh * kDim, p.qkv_row, row_lo, row_hi, tiles + kHalf, tid);
   const int head0 = kh * p.heads_ratio;
   if (w < p.heads_ratio) chunk_gates(p, s, w, token0, row_lo, row_hi, head0 + w, lane);
   if constexpr (kVec) cp_async_wait();
   __syncthreads();
   if (tid < kChunk) {
-    s.fk[tid] = scale_row(reinterpret_cast<uint16_t*>(s.k), tid);
+    s.fk[tid] = scale_row(tiles, tid);
   } else {
-    s.fq[tid - kChunk] = scale_row(reinterpret_cast<uint16_t*>(s.q), tid - kChunk);
+    s.fq[tid - kChunk] = scale_row(tiles + kHalf, tid - kChunk);
   }
   __syncthreads();
   {
     uint4* to = reinterpret_cast<uint4*>(p.keys + place * p.num_k_heads + kh);
-    const uint4* k = reinterpret_cast<const uint4*>(s.k);
-    const uint4* q = reinterpret_cast<const uint4*>(s.q);
-    constexpr int kPieces = kChunk * kDim / 8;
+    const uint4* from = reinterpret_cast<const uint4*>(s.kq());
 #pragma unroll
-    for (int i = 0; i < kPieces / kPairThreads; ++i) {
-      to[i * kPairThreads + tid] = k[i * kPairThreads + tid];
-      to[kPieces + i * kPairThreads + tid] = q[i * kPairThreads + tid];
+    for (int i = 0; i < static_cast<int>(sizeof(KeyImage)) / (16 * kPairThreads); ++i) {
+      to[i * kPairThreads + tid] = from[i * kPairThreads + tid];
     }
   }
   float kk[4][2][4], qk[4][2][4];
@@ -678,12 +757,12 @@ __global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(cons
     }
     if (tid < kChunk) {
       const float in = exp2_fast(s.g_hi[at][tid] + s.g_lo[at][tid]);
-      s.image.beta[tid] = s.beta[at][tid];
-      s.image.k_in[tid] = in * s.fk[tid];
-      s.image.q_in[tid] = in * s.fq[tid] * p.q_scale;
+      s.work().image.beta[tid] = s.beta[at][tid];
+      s.work().image.k_in[tid] = in * s.fk[tid];
+      s.work().image.q_in[tid] = in * s.fq[tid] * p.q_scale;
       const float left = (s.g_hi[at][kChunk - 1] - s.g_hi[at][tid]) + (s.g_lo[at][kChunk - 1] - s.g_lo[at][tid]);
-      s.image.k_out[tid] = exp2_fast(left) * s.fk[tid];
-      if (tid == kChunk - 1) s.image.decay = in;
+      s.work().image.k_out[tid] = exp2_fast(left) * s.fk[tid];
+      if (tid == kChunk - 1) s.work().image.decay = in;
     }
     decayed_pairs(p, s, at, w, lane, kk, qk);
     __syncwarp();
@@ -692,51 +771,79 @@ __global__ void __launch_bounds__(kPairThreads, 3) gdn_prefill_pairs_kernel(cons
     invert_column(s, w, lane);
     __syncthreads();
     uint4* to = reinterpret_cast<uint4*>(p.pairs + place * p.num_v_heads + head0 + n);
-    const uint4* from = reinterpret_cast<const uint4*>(&s.image);
+    const uint4* from = reinterpret_cast<const uint4*>(&s.work().image);
     for (int i = tid; i < static_cast<int>(sizeof(PairImage) / 16); i += kPairThreads) to[i] = from[i];
   }
 }
 
 // ------------------------------------------------------------------------------------------
-// chain: the state through the chunks, 16 value rows per warp
+// chain: the state through the chunks
 // ------------------------------------------------------------------------------------------
-struct Stage {
-  KeyImage key;
-  __align__(256) __nv_bfloat16 v[kChunk * kDim];  // swizzled
-  PairImage pair;
+struct Factors {
+  float beta[kChunk], k_in[kChunk], q_in[kChunk], k_out[kChunk];
+  float decay;
+};
+constexpr int kFactorPieces = (4 * kChunk * 4 + 16) / 16;  // 16-byte pieces from PairImage::beta on that hold Factors
+static_assert(sizeof(Factors) <= 16 * kFactorPieces && kFactorPieces <= kMoveThreads, "one copy per thread");
+
+struct __align__(1024) Stage {
+  __half kq[2 * kChunk * kDim];
+  __nv_bfloat16 v[kChunk * kDim];
+  __half t_hi[kHalf], t_lo[kHalf], p[kHalf];  // 16 x 16 blocks above the diagonal are never read
+  __align__(16) Factors f;
+  float pad[3];  // the last piece of the factors is copied whole
 };
 
 struct ChainSmem {
-  __align__(256) Stage stage[2];
+  Stage stage[2];
   __align__(16) float o[kChunk * kORow];
+  uint64_t done[2];  // products finished: [0] what the state waits for, [1] what only the outputs do
+  uint32_t tmem;
+  volatile int stop;  // a wait ran out: nothing is stored any more
 };
 
-template <typename Image>
-__device__ __forceinline__ void copy_image(Image& to, const Image* from, int tid) {
-  constexpr int kPieces = sizeof(Image) / 16, kWhole = kPieces / kCopyThreads;
-  const uint32_t dst = smem_u32(&to) + 16 * tid;
-  const unsigned char* src = reinterpret_cast<const unsigned char*>(from) + 16 * tid;
-#pragma unroll
-  for (int i = 0; i < kWhole; ++i) cp_async16(dst + 16 * kCopyThreads * i, src + 16 * kCopyThreads * i);
-  if (tid < kPieces % kCopyThreads) cp_async16(dst + 16 * kCopyThreads * kWhole, src + 16 * kCopyThreads * kWhole);
-}
+// TMEM columns (32 bits x 128 lanes, lane = value row); all 512 are allocated, so they start at 0.  dS takes
+// the place of Y and O, which are in registers by then, and P u that of R.
+constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW = 224, kTmemY = 288, kTmemO = 352,
+                   kTmemDs = 288, kTmemTr = 416, kTmemColumns = 512;
 
 template <bool kVec>
 __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Request& rq, int64_t chunk,
                                            int64_t place, int head, int tid) {
   const int kh = head / p.heads_ratio;
-  copy_image(st.key, p.keys + place * p.num_k_heads + kh, tid);
-  copy_image(st.pair, p.pairs + place * p.num_v_heads + head, tid);
+  const unsigned char* key = reinterpret_cast<const unsigned char*>(p.keys + place * p.num_k_heads + kh) + 16 * tid;
+  const uint32_t key_to = smem_u32(st.kq) + 16 * tid;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(KeyImage)) / (16 * kMoveThreads); ++i) {
+    cp_async16(key_to + 16 * kMoveThreads * i, key + 16 * kMoveThreads * i);
+  }
+  // A warp copies whole packed blocks, 32 pieces each, to their places in the tiles.
+  const PairImage* image = p.pairs + place * p.num_v_heads + head;
+  const unsigned char* packed = reinterpret_cast<const unsigned char*>(image);
+  const int w = tid >> 5, lane = tid & 31;
+  const int row = lane >> 1, part = (lane & 1) ^ ((row >> 2) & 1);
+  const uint32_t tri_to = smem_u32(st.t_hi) + row * 128;
+  constexpr int kWarps = kMoveThreads / 32, kUnits = 3 * kTriBlocks;
+#pragma unroll
+  for (int i = 0; i < (kUnits + kWarps - 1) / kWarps; ++i) {
+    const int unit = w + kWarps * i;
+    if (unit < kUnits) {
+      const int m = unit / kTriBlocks, b = unit - m * kTriBlocks;
+      const int ib = (b >= 1) + (b >= 3) + (b >= 6), jb = b - ib * (ib + 1) / 2;
+      cp_async16(tri_to + m * (2 * kHalf) + ib * 2048 + (((2 * jb + part) ^ (row & 7)) << 4), packed + unit * 512 + lane * 16);
+    }
+  }
+  if (tid < kFactorPieces) cp_async16(smem_u32(&st.f) + 16 * tid, reinterpret_cast<const unsigned char*>(image->beta) + 16 * tid);
   const int64_t local0 = chunk * kChunk - rq.lead;
   const int row_lo = chunk == 0 ? rq.lead : 0;
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
-  load_rows<kVec>(p.qkv + (rq.first + local0) * p.qkv_row + (2 * p.num_k_heads + head) * kDim, p.qkv_row, row_lo,
-                  row_hi, reinterpret_cast<uint16_t*>(st.v), tid);
+  load_rows<kVec, kMoveThreads, kHalf>(p.qkv + (rq.first + local0) * p.qkv_row + (2 * p.num_k_heads + head) * kDim,
+                                       p.qkv_row, row_lo, row_hi, reinterpret_cast<uint16_t*>(st.v), tid);
 }
 
 // Gated RMSNorm of the chunk's outputs.  A warp takes two rows at a time, 16 lanes and twice four values
-// per lane each; gate rows are loaded first, so that they arrive while the chain finishes the tile (`wait`
-// returns then).
+// per lane each.  What the gate and the norm's weight make of a value is computed first, while the chain
+// finishes the tile (`wait` returns then).
 template <bool kVec, typename Wait>
 __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Request& rq,
                                               int64_t chunk, int head, const float (&wt)[8], int tid, Wait wait) {
@@ -744,12 +851,13 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
   const int64_t local0 = chunk * kChunk - rq.lead;
   const int row_lo = chunk == 0 ? rq.lead : 0;
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
-  constexpr int kSteps = kChunk / 8;
+  constexpr int kRows = kMoveThreads / 16, kSteps = kChunk / kRows;
+  const int row0 = 2 * w + (lane >> 4);
   const __nv_bfloat16* gate = p.gate + (rq.first + local0) * p.gate_row + head * kDim + 4 * part;
   uint2 z[kSteps][2];
 #pragma unroll
   for (int n = 0; n < kSteps; ++n) {
-    const int i = 8 * n + 2 * w + (lane >> 4);
+    const int i = kRows * n + row0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       z[n][half] = make_uint2(0, 0);
@@ -764,11 +872,23 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
       }
     }
   }
+  float f[kSteps][8];
+#pragma unroll
+  for (int n = 0; n < kSteps; ++n) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f[n][4 * half + 0] = wt[4 * half + 0] * silu_fast(bf16_low(z[n][half].x));
+      f[n][4 * half + 1] = wt[4 * half + 1] * silu_fast(bf16_high(z[n][half].x));
+      f[n][4 * half + 2] = wt[4 * half + 2] * silu_fast(bf16_low(z[n][half].y));
+      f[n][4 * half + 3] = wt[4 * half + 3] * silu_fast(bf16_high(z[n][half].y));
+    }
+  }
   wait();
+  const bool stop = s.stop != 0;
   __nv_bfloat16* out = p.out + ((rq.first + local0) * p.num_v_heads + head) * kDim + 4 * part;
 #pragma unroll
   for (int n = 0; n < kSteps; ++n) {
-    const int i = 8 * n + 2 * w + (lane >> 4);
+    const int i = kRows * n + row0;
     float4 o[2];
     float sq = 0.0f;
 #pragma unroll
@@ -782,27 +902,22 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     const float rstd = rsqrtf(sq * (1.0f / kDim) + p.eps);
-    const bool live = i >= row_lo && i < row_hi;
+    const bool live = i >= row_lo && i < row_hi && !stop;
     __nv_bfloat16* row = out + static_cast<int64_t>(i) * p.num_v_heads * kDim;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const uint2 zz = z[n][half];
-      const float y0 = o[half].x * rstd * wt[4 * half + 0] * silu(__uint_as_float(zz.x << 16));
-      const float y1 = o[half].y * rstd * wt[4 * half + 1] * silu(__uint_as_float(zz.x & 0xffff0000u));
-      const float y2 = o[half].z * rstd * wt[4 * half + 2] * silu(__uint_as_float(zz.y << 16));
-      const float y3 = o[half].w * rstd * wt[4 * half + 3] * silu(__uint_as_float(zz.y & 0xffff0000u));
+      const uint32_t lo = pack_bf16(o[half].x * rstd * f[n][4 * half], o[half].y * rstd * f[n][4 * half + 1]);
+      const uint32_t hi = pack_bf16(o[half].z * rstd * f[n][4 * half + 2], o[half].w * rstd * f[n][4 * half + 3]);
       __nv_bfloat16* at = row + 64 * half;
-      if constexpr (kVec) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(y0, y1), hi = __floats2bfloat162_rn(y2, y3);
-        if (live) {
-          *reinterpret_cast<uint2*>(at) =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      if (live) {
+        if constexpr (kVec) {
+          *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
+        } else {
+          at[0] = __ushort_as_bfloat16(static_cast<unsigned short>(lo));
+          at[1] = __ushort_as_bfloat16(static_cast<unsigned short>(lo >> 16));
+          at[2] = __ushort_as_bfloat16(static_cast<unsigned short>(hi));
+          at[3] = __ushort_as_bfloat16(static_cast<unsigned short>(hi >> 16));
         }
-      } else if (live) {
-        at[0] = __float2bfloat16_rn(y0);
-        at[1] = __float2bfloat16_rn(y1);
-        at[2] = __float2bfloat16_rn(y2);
-        at[3] = __float2bfloat16_rn(y3);
       }
     }
   }
@@ -825,216 +940,267 @@ __device__ __forceinline__ void store_pair(__nv_bfloat16* at, float x, float y) 
   *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(x, y);
 }
 
-// One chunk on this warp's rows of S.  The output tile is free when `wait_o` says so.
-template <typename WaitO>
-__device__ __forceinline__ void chain_chunk(float (&S)[16][4], const Stage& st, float* o_tile, int v0, int lane,
-                                            WaitO wait_o) {
-  const int g = lane >> 2, t = lane & 3;
-  const uint32_t k_base = lane_addr<kDim, false>(st.key.k, lane), q_base = lane_addr<kDim, false>(st.key.q, lane);
-  const uint32_t k_trans = lane_addr<kDim, true>(st.key.k, lane), v_base = lane_addr<kDim, false>(st.v, lane);
-  const uint32_t th_base = tri_addr(st.pair.t_hi, lane), tl_base = tri_addr(st.pair.t_lo, lane);
-  const uint32_t p_base = tri_addr(st.pair.p, lane);
+// Waits until the barrier's phase has completed, the warp together.  After kWaitNs it gives up for good:
+// it raises the fault, and from then on this warp stores nothing and waits for no product.
+__device__ __forceinline__ void wait_done(uint32_t bar, uint32_t parity, ChainSmem& s, bool& dead) {
+  if (dead) return;
+  uint64_t start = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok != 0)) break;
+    uint64_t now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now)::"memory");
+    if (start == 0) start = now;
+    if (__any_sync(0xffffffffu, now - start > kWaitNs)) {
+      dead = true;
+      s.stop = 1;
+      atomicOr(&g_prefill_faults, LD_FAULT_WAIT_TIMEOUT);
+      break;
+    }
+  }
+  tmem_after();
+}
 
-  // Y = S k~ (two terms) and O = S q~ (hi term), columns = the chunk's rows.
+// Largest magnitudes of the two rows of a fragment array, over the row's four lanes, as row scales.
+template <int kTiles>
+__device__ __forceinline__ void scale_rows(const float (&x)[kTiles][4], float& up0, float& down0, float& up1,
+                                           float& down1) {
   float top0 = 0.0f, top1 = 0.0f;
 #pragma unroll
-  for (int n = 0; n < 16; ++n) {
-    top0 = fmaxf(top0, fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-    top1 = fmaxf(top1, fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
+  for (int n = 0; n < kTiles; ++n) {
+    top0 = max_abs(top0, x[n][0], x[n][1]);
+    top1 = max_abs(top1, x[n][2], x[n][3]);
   }
-  float up0, down0, up1, down1;
   row_scale(quad_max(top0), up0, down0);
   row_scale(quad_max(top1), up1, down1);
-  float Y[8][4], O[8][4];
+}
+
+// Four k-steps (64 columns) of a fragment array, scaled, as hi and lo A operands in TMEM.
+template <int kTiles>
+__device__ __forceinline__ void store_split(const float (&x)[kTiles][4], int first, float up0, float up1,
+                                            uint32_t hi_at, uint32_t lo_at) {
+  uint32_t hi[4][4], lo[4][4];
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) Y[n][e] = O[n][e] = 0.0f;
-  }
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks) {
-    uint32_t hi[4], lo[4];
+  for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      split(S[2 * ks + m][0] * up0, S[2 * ks + m][1] * up0, hi[2 * m], lo[2 * m]);
-      split(S[2 * ks + m][2] * up1, S[2 * ks + m][3] * up1, hi[2 * m + 1], lo[2 * m + 1]);
-    }
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      uint32_t b[4];
-      ldsm4(block<kDim>(k_base, nb, ks), b);
-      mma(Y[2 * nb], lo, b[0], b[1]);
-      mma(Y[2 * nb + 1], lo, b[2], b[3]);
-      mma(Y[2 * nb], hi, b[0], b[1]);
-      mma(Y[2 * nb + 1], hi, b[2], b[3]);
-      ldsm4(block<kDim>(q_base, nb, ks), b);
-      mma(O[2 * nb], hi, b[0], b[1]);
-      mma(O[2 * nb + 1], hi, b[2], b[3]);
+      const float(&f)[4] = x[first + 2 * ks + m];
+      split(mul2(make_float2(f[0], f[1]), make_float2(up0, up0)), hi[ks][2 * m], lo[ks][2 * m]);
+      split(mul2(make_float2(f[2], f[3]), make_float2(up1, up1)), hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
     }
   }
+  tmem_store(hi_at, hi);
+  tmem_store(lo_at, lo);
+}
 
-  // R = beta (v - k_in Y), in place.
-  top0 = top1 = 0.0f;
+// f = a f + b x, a pair of columns of two rows at a time.
+__device__ __forceinline__ void scale_add(float (&f)[4], float2 a0, float2 a1, const float (&x)[4], float2 b0, float2 b1) {
+  const float2 lo = fma2(make_float2(f[0], f[1]), a0, mul2(make_float2(x[0], x[1]), b0));
+  const float2 hi = fma2(make_float2(f[2], f[3]), a1, mul2(make_float2(x[2], x[3]), b1));
+  f[0] = lo.x;
+  f[1] = lo.y;
+  f[2] = hi.x;
+  f[3] = hi.y;
+}
+
+// What the threads that carry the state keep between chunks.
+struct StateWarp {
+  float S[16][4];      // rows v0 + g, v0 + g + 8; columns 8n + 2t, + 1
+  float O[8][4];       // outputs of the chunk in work: columns are the chunk's rows
+  float down0, down1;  // what P u is scaled by
+  uint32_t phase0, phase1;
+  bool dead;
+};
+
+// The chunk's outputs, S q + P u, to the tile, once P u is done.
+__device__ __forceinline__ void finish_outputs(StateWarp& x, ChainSmem& s, uint32_t tmem, int v0, int lane, bool wait) {
+  const int g = lane >> 2, t = lane & 3;
+  float pu[8][4];
+  tmem_load(tmem + kTmemPu, pu);
+  if (wait) bar_sync(kBarOFree);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    float* at = s.o + (8 * n + 2 * t) * kORow + v0 + g;
+    at[0] = fmaf(pu[n][0], x.down0, x.O[n][0]);
+    at[kORow] = fmaf(pu[n][1], x.down0, x.O[n][1]);
+    at[8] = fmaf(pu[n][2], x.down1, x.O[n][2]);
+    at[kORow + 8] = fmaf(pu[n][3], x.down1, x.O[n][3]);
+  }
+  bar_arrive(kBarOReady);
+}
+
+// One chunk.  `tmem` carries this warp's lanes; one warp (`issuer`) issues the products.
+// `before` runs while S k is computed: it finishes the chunk before, if there is one (`more`).
+template <typename Before>
+__device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const Stage& st, uint32_t tmem, int v0, int lane,
+                                            bool issuer, bool more, Before before) {
+  const int t = lane & 3;
+  const uint32_t done0 = smem_u32(&s.done[0]), done1 = smem_u32(&s.done[1]);
+
+  // Y = S k~ (two terms) and O = S q~ (hi term).
+  float up0, down0, up1, down1;
+  scale_rows(x.S, up0, down0, up1, down1);
+  store_split(x.S, 0, up0, up1, tmem + kTmemS, tmem + kTmemS + 64);
+  store_split(x.S, 8, up0, up1, tmem + kTmemS + 32, tmem + kTmemS + 96);
+  tmem_stored();
+  // The chunk before's P u: every warp has seen a barrier's phase before the next one can begin, here and
+  // at the other two joins, so that waiting by parity is sound.
+  if (more) {
+    wait_done(done1, x.phase1, s, x.dead);
+    x.phase1 ^= 1;
+  }
+  tmem_before();
+  bar_state();
+  if (issuer && !x.dead) {
+    tmem_after();
+    const uint32_t elected = elect_lane();
+    const uint64_t kq = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
+    // Rows 0-63 of a half are k's, 64-127 q's: 128 columns of D are Y and O.
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      umma(elected, kTmemY, kTmemS + 8 * ks, kq + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(128, false), ks > 0);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      umma(elected, kTmemY, kTmemS + 64 + 8 * ks, kq + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(64, false), true);
+    }
+    umma_commit(elected, done0);
+  }
+  before();
+
+  // R = beta (v - k_in Y).
+  wait_done(done0, x.phase0, s, x.dead);
+  x.phase0 ^= 1;
+  float Y[8][4];
+  tmem_load(tmem + kTmemY, Y);
+  const uint32_t v_base = lane_addr<false>(st.v, lane);
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
     uint32_t vt[4];  // v transposed: (rows 16nb.., cols v0..), (.., v0 + 8..), (rows 16nb + 8.., ...)
-    ldsm4_t(block<kDim>(v_base, nb, v0 / 16), vt);
+    ldsm4_t(block<kHalf>(v_base, nb, v0 / 16), vt);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const int n = 2 * nb + m;
-      const float2 kin = *reinterpret_cast<const float2*>(&st.pair.k_in[8 * n + 2 * t]);
-      const float2 beta = *reinterpret_cast<const float2*>(&st.pair.beta[8 * n + 2 * t]);
+      float(&f)[4] = Y[2 * nb + m];
+      const float2 kin = *reinterpret_cast<const float2*>(&st.f.k_in[16 * nb + 8 * m + 2 * t]);
+      const float2 beta = *reinterpret_cast<const float2*>(&st.f.beta[16 * nb + 8 * m + 2 * t]);
       const uint32_t r0 = vt[2 * m], r1 = vt[2 * m + 1];
-      Y[n][0] = beta.x * (__uint_as_float(r0 << 16) - kin.x * (Y[n][0] * down0));
-      Y[n][1] = beta.y * (__uint_as_float(r0 & 0xffff0000u) - kin.y * (Y[n][1] * down0));
-      Y[n][2] = beta.x * (__uint_as_float(r1 << 16) - kin.x * (Y[n][2] * down1));
-      Y[n][3] = beta.y * (__uint_as_float(r1 & 0xffff0000u) - kin.y * (Y[n][3] * down1));
-      top0 = fmaxf(top0, fmaxf(fabsf(Y[n][0]), fabsf(Y[n][1])));
-      top1 = fmaxf(top1, fmaxf(fabsf(Y[n][2]), fabsf(Y[n][3])));
+      const float2 y0 = fma2(mul2(kin, make_float2(-down0, -down0)), make_float2(f[0], f[1]),
+                             make_float2(bf16_low(r0), bf16_high(r0)));
+      const float2 y1 = fma2(mul2(kin, make_float2(-down1, -down1)), make_float2(f[2], f[3]),
+                             make_float2(bf16_low(r1), bf16_high(r1)));
+      const float2 z0 = mul2(beta, y0), z1 = mul2(beta, y1);
+      f[0] = z0.x;
+      f[1] = z0.y;
+      f[2] = z1.x;
+      f[3] = z1.y;
     }
   }
-  // O into fp32 units of the first read-out.
+  const float s_down0 = down0, s_down1 = down1;
+  scale_rows(Y, up0, down0, up1, down1);
+  store_split(Y, 0, up0, up1, tmem + kTmemR, tmem + kTmemR + 32);
+  tmem_stored();
+  tmem_before();
+  bar_state();
+  // U = T R (the product of the two lo terms is below fp32's last bit).  Column block ks of T starts at row
+  // block ks.
+  if (issuer && !x.dead) {
+    tmem_after();
+    const uint32_t elected = elect_lane();
+    const uint64_t t_hi = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.t_hi), 0));
+    const uint64_t t_lo = t_hi + (2 * kHalf >> 4);
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const float2 qin = *reinterpret_cast<const float2*>(&st.pair.q_in[8 * n + 2 * t]);
-    O[n][0] *= qin.x * down0;
-    O[n][1] *= qin.y * down0;
-    O[n][2] *= qin.x * down1;
-    O[n][3] *= qin.y * down1;
-  }
-  row_scale(quad_max(top0), up0, down0);
-  row_scale(quad_max(top1), up1, down1);
-
-  // U = T R (both in two terms; the product of the two lo terms is below fp32's last bit).
-  float U[8][4];
-  {
-    uint32_t hi[4][4], lo[4][4];
+    for (int term = 0; term < 3; ++term) {  // hi lo, lo hi, hi hi
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        split(Y[2 * ks + m][0] * up0, Y[2 * ks + m][1] * up0, hi[ks][2 * m], lo[ks][2 * m]);
-        split(Y[2 * ks + m][2] * up1, Y[2 * ks + m][3] * up1, hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
+      for (int ks = 0; ks < 4; ++ks) {
+        umma(elected, kTmemTr + 16 * ks, kTmemR + (term == 1 ? 32 : 0) + 8 * ks,
+             (term == 0 ? t_lo : t_hi) + ks * (2048 >> 4) + ks * 2, mma_shape(64 - 16 * ks, false), term > 0 || ks > 0);
       }
     }
-#pragma unroll
-    for (int ib = 0; ib < 4; ++ib) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) U[2 * ib][e] = U[2 * ib + 1][e] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks <= ib; ++ks) {
-        uint32_t bh[4], bl[4];
-        ldsm4(th_base + tri_block(ib, ks), bh);
-        ldsm4(tl_base + tri_block(ib, ks), bl);
-        mma(U[2 * ib], hi[ks], bl[0], bl[1]);
-        mma(U[2 * ib + 1], hi[ks], bl[2], bl[3]);
-        mma(U[2 * ib], lo[ks], bh[0], bh[1]);
-        mma(U[2 * ib + 1], lo[ks], bh[2], bh[3]);
-        mma(U[2 * ib], hi[ks], bh[0], bh[1]);
-        mma(U[2 * ib + 1], hi[ks], bh[2], bh[3]);
-      }
-    }
+    umma_commit(elected, done0);
   }
-
-  // O += P U (hi term), in units of U's own row scale.
-  top0 = top1 = 0.0f;
+  tmem_load(tmem + kTmemO, x.O);
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    U[n][0] *= down0;
-    U[n][1] *= down0;
-    U[n][2] *= down1;
-    U[n][3] *= down1;
-    top0 = fmaxf(top0, fmaxf(fabsf(U[n][0]), fabsf(U[n][1])));
-    top1 = fmaxf(top1, fmaxf(fabsf(U[n][2]), fabsf(U[n][3])));
+    const float2 qin = *reinterpret_cast<const float2*>(&st.f.q_in[8 * n + 2 * t]);
+    const float2 o0 = mul2(make_float2(x.O[n][0], x.O[n][1]), mul2(qin, make_float2(s_down0, s_down0)));
+    const float2 o1 = mul2(make_float2(x.O[n][2], x.O[n][3]), mul2(qin, make_float2(s_down1, s_down1)));
+    x.O[n][0] = o0.x;
+    x.O[n][1] = o0.y;
+    x.O[n][2] = o1.x;
+    x.O[n][3] = o1.y;
   }
-  row_scale(quad_max(top0), up0, down0);
-  row_scale(quad_max(top1), up1, down1);
+
+  // u, and k_out u in two terms.
+  wait_done(done0, x.phase0, s, x.dead);
+  x.phase0 ^= 1;
+  tmem_load(tmem + kTmemTr, Y);
+  const float r_down0 = down0, r_down1 = down1;
   {
+    scale_rows(Y, up0, down0, up1, down1);
     uint32_t hi[4][4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        hi[ks][2 * m] = pack_half(U[2 * ks + m][0] * up0, U[2 * ks + m][1] * up0);
-        hi[ks][2 * m + 1] = pack_half(U[2 * ks + m][2] * up1, U[2 * ks + m][3] * up1);
+        const float(&f)[4] = Y[2 * ks + m];
+        hi[ks][2 * m] = pack_half(f[0] * up0, f[1] * up0);
+        hi[ks][2 * m + 1] = pack_half(f[2] * up1, f[3] * up1);
       }
     }
-#pragma unroll
-    for (int ib = 0; ib < 4; ++ib) {
-      float acc[2][4] = {};
-#pragma unroll
-      for (int ks = 0; ks <= ib; ++ks) {
-        uint32_t b[4];
-        ldsm4(p_base + tri_block(ib, ks), b);
-        mma(acc[0], hi[ks], b[0], b[1]);
-        mma(acc[1], hi[ks], b[2], b[3]);
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        O[2 * ib + m][0] = fmaf(acc[m][0], down0, O[2 * ib + m][0]);
-        O[2 * ib + m][1] = fmaf(acc[m][1], down0, O[2 * ib + m][1]);
-        O[2 * ib + m][2] = fmaf(acc[m][2], down1, O[2 * ib + m][2]);
-        O[2 * ib + m][3] = fmaf(acc[m][3], down1, O[2 * ib + m][3]);
-      }
-    }
+    tmem_store(tmem + kTmemU, hi);
+    x.down0 = r_down0 * down0;
+    x.down1 = r_down1 * down1;
   }
-  wait_o();
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    float* at = o_tile + (8 * n + 2 * t) * kORow + v0 + g;
-    at[0] = O[n][0];
-    at[kORow] = O[n][1];
-    at[8] = O[n][2];
-    at[kORow + 8] = O[n][3];
+    const float2 kout = *reinterpret_cast<const float2*>(&st.f.k_out[8 * n + 2 * t]);
+    const float2 u0 = mul2(make_float2(Y[n][0], Y[n][1]), kout), u1 = mul2(make_float2(Y[n][2], Y[n][3]), kout);
+    Y[n][0] = u0.x;
+    Y[n][1] = u0.y;
+    Y[n][2] = u1.x;
+    Y[n][3] = u1.y;
   }
-  bar_arrive(kBarOReady);
-
-  // S <- decay S + (k_out u) k~^T, u in two terms.  Each column block sums in fresh accumulators and
-  // meets the state in one fp32 fused multiply-add.
-  top0 = top1 = 0.0f;
+  scale_rows(Y, up0, down0, up1, down1);
+  store_split(Y, 0, up0, up1, tmem + kTmemW, tmem + kTmemW + 32);
+  tmem_stored();
+  tmem_before();
+  bar_state();
+  if (issuer && !x.dead) {
+    tmem_after();
+    const uint32_t elected = elect_lane();
+    const uint64_t k = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
+    const uint64_t pp = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.p), 0));
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const float2 kout = *reinterpret_cast<const float2*>(&st.pair.k_out[8 * n + 2 * t]);
-    U[n][0] *= kout.x;
-    U[n][1] *= kout.y;
-    U[n][2] *= kout.x;
-    U[n][3] *= kout.y;
-    top0 = fmaxf(top0, fmaxf(fabsf(U[n][0]), fabsf(U[n][1])));
-    top1 = fmaxf(top1, fmaxf(fabsf(U[n][2]), fabsf(U[n][3])));
-  }
-  row_scale(quad_max(top0), up0, down0);
-  row_scale(quad_max(top1), up1, down1);
-  {
-    uint32_t hi[4][4], lo[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        split(U[2 * ks + m][0] * up0, U[2 * ks + m][1] * up0, hi[ks][2 * m], lo[ks][2 * m]);
-        split(U[2 * ks + m][2] * up1, U[2 * ks + m][3] * up1, hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
-      }
-    }
-    const float decay = st.pair.decay;
-#pragma unroll
-    for (int nb = 0; nb < 8; ++nb) {
-      float acc[2][4] = {};
+    for (int term = 1; term >= 0; --term) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        uint32_t b[4];  // k~ transposed: (rows 0-7, cols 0-7), (rows 8-15, cols 0-7), (0-7, 8-15), (8-15, 8-15)
-        ldsm4_t(block<kDim>(k_trans, ks, nb), b);
-        mma(acc[0], lo[ks], b[0], b[1]);
-        mma(acc[1], lo[ks], b[2], b[3]);
-        mma(acc[0], hi[ks], b[0], b[1]);
-        mma(acc[1], hi[ks], b[2], b[3]);
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        S[2 * nb + m][0] = fmaf(S[2 * nb + m][0], decay, acc[m][0] * down0);
-        S[2 * nb + m][1] = fmaf(S[2 * nb + m][1], decay, acc[m][1] * down0);
-        S[2 * nb + m][2] = fmaf(S[2 * nb + m][2], decay, acc[m][2] * down1);
-        S[2 * nb + m][3] = fmaf(S[2 * nb + m][3], decay, acc[m][3] * down1);
+        umma(elected, kTmemDs, kTmemW + 32 * term + 8 * ks, k + ks * (2048 >> 4), mma_shape(128, true),
+             term == 0 || ks > 0);
       }
     }
+    umma_commit(elected, done0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, pp + ks * (2048 >> 4) + ks * 2, mma_shape(64 - 16 * ks, false),
+           ks > 0);
+    }
+    umma_commit(elected, done1);
+  }
+  // S <- decay S + dS, one fp32 fused multiply-add per element.
+  const float2 decay = make_float2(st.f.decay, st.f.decay);
+  const float2 w0 = make_float2(r_down0 * down0, r_down0 * down0), w1 = make_float2(r_down1 * down1, r_down1 * down1);
+  wait_done(done0, x.phase0, s, x.dead);
+  x.phase0 ^= 1;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    tmem_load(tmem + kTmemDs + 64 * half, Y);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) scale_add(x.S[8 * half + n], decay, decay, Y[n], w0, w1);
   }
 }
 
@@ -1057,50 +1223,78 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     }
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kStateWarp = kMoveThreads / 32;
 
-  // Launched with 384 x 168 registers; 128 x 88 + 256 x 208 is the same 64,512.
-  if (warp < kCopyThreads / 32) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  // Launched with 512 x 128 registers; 256 x 80 + 256 x 176 is the same 65,536.
+  if (warp < kStateWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int tid = threadIdx.x;
     const int64_t base = chunk_base(rq.first, r);
+    const auto hand_over = [&](int stage) {
+      cp_async_wait();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the products read through the async proxy
+      bar_arrive(kBarFull + stage);
+    };
+    for (int64_t c = 0; c < min(rq.chunks, static_cast<int64_t>(2)); ++c) {
+      copy_chunk<kVec>(p, s.stage[c], rq, c, base + c, head, tid);
+      hand_over(static_cast<int>(c));
+    }
     float wt[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) wt[e] = load_param(p.weight, 64 * (e >> 2) + 4 * (lane & 15) + (e & 3), p.weight_bf16);
-    // Chunk c is copied in while the chain works on chunk c - 1, then chunk c - 1's outputs are stored.
-    for (int64_t c = 0; c <= rq.chunks; ++c) {
-      if (c < rq.chunks) {
-        const int stage = static_cast<int>(c & 1);
-        if (c >= 2) bar_sync(kBarEmpty + stage);
-        copy_chunk<kVec>(p, s.stage[stage], rq, c, base + c, head, tid);
-        cp_async_wait();
-        bar_arrive(kBarFull + stage);
-      }
-      if (c >= 1) {
-        store_outputs<kVec>(p, s, rq, c - 1, head, wt, tid, [] { bar_sync(kBarOReady); });
-        if (c < rq.chunks) bar_arrive(kBarOFree);
-      }
+    for (int64_t c = 0; c < rq.chunks; ++c) {
+      const int stage = static_cast<int>(c & 1);
+      store_outputs<kVec>(p, s, rq, c, head, wt, tid, [&] {
+        // The outputs of chunk c are there, and every product on it is done, so its stage is free.
+        bar_sync(kBarOReady);
+        if (c + 2 < rq.chunks) copy_chunk<kVec>(p, s.stage[stage], rq, c + 2, base + c + 2, head, tid);
+      });
+      if (c + 1 < rq.chunks) bar_arrive(kBarOFree);
+      if (c + 2 < rq.chunks) hand_over(stage);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int g = lane >> 2, t = lane & 3;
-    const int v0 = 16 * (warp - kCopyThreads / 32);
+    // A warp reaches the TMEM lanes of its number mod 4; two warps share them, 16 lanes each.
+    const int v0 = 32 * (warp & 3) + 16 * ((warp - kStateWarp) >> 2);
+    const bool issuer = warp == kStateWarp;
+    if (issuer) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)),
+                   "n"(kTmemColumns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+      if (lane == 0) {
+        s.stop = 0;
+        for (int i = 0; i < 2; ++i) {
+          asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&s.done[i])) : "memory");
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      }
+      __syncwarp();
+      tmem_before();
+    }
     StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(head) * kDim * kDim + (v0 + g) * kDim + 2 * t;
-    float S[16][4];
+    StateWarp x;
+    x.phase0 = x.phase1 = 0;
+    x.dead = false;
     if (rq.source > 0) {
       const StateT* at = pool + rq.source * p.slot_stride;
 #pragma unroll
       for (int n = 0; n < 16; ++n) {
-        load_pair(at + 8 * n, S[n][0], S[n][1]);
-        load_pair(at + 8 * kDim + 8 * n, S[n][2], S[n][3]);
+        load_pair(at + 8 * n, x.S[n][0], x.S[n][1]);
+        load_pair(at + 8 * kDim + 8 * n, x.S[n][2], x.S[n][3]);
       }
     } else {
 #pragma unroll
       for (int n = 0; n < 16; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[n][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) x.S[n][e] = 0.0f;
       }
     }
+    bar_state();
+    tmem_after();
+    const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
     // Chunks end at absolute positions that are multiples of 64, and so do blocks.
     const int64_t per_block = p.block_size / kChunk;
     const int32_t* slot_at = rq.row + rq.context / p.block_size;
@@ -1108,24 +1302,33 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     for (int64_t c = 0; c < rq.chunks; ++c) {
       const int stage = static_cast<int>(c & 1);
       bar_sync(kBarFull + stage);
-      chain_chunk(S, s.stage[stage], s.o, v0, lane, [&] {
-        if (c >= 1) bar_sync(kBarOFree);
+      chain_chunk(x, s, s.stage[stage], tmem, v0, lane, issuer, c >= 1, [&] {
+        if (c >= 1) finish_outputs(x, s, tmem, v0, lane, c >= 2);
       });
-      if (c + 2 < rq.chunks) bar_arrive(kBarEmpty + stage);
       if (c + 1 == rq.chunks || --left == 0) {  // a block or the request ends here: its slot takes the state
         const int32_t slot = *slot_at++;
         left = per_block;
         if (slot > 0 && slot < p.n_slots) {
           StateT* at = pool + slot * p.slot_stride;
+          if (!x.dead) {
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            store_pair(at + 8 * n, S[n][0], S[n][1]);
-            store_pair(at + 8 * kDim + 8 * n, S[n][2], S[n][3]);
+            for (int n = 0; n < 16; ++n) {
+              store_pair(at + 8 * n, x.S[n][0], x.S[n][1]);
+              store_pair(at + 8 * kDim + 8 * n, x.S[n][2], x.S[n][3]);
+            }
           }
         } else if (slot >= p.n_slots && head == 0 && lane == 0) {
           atomicOr(&g_prefill_faults, LD_FAULT_DECODE_SLOT_RANGE);
         }
       }
+    }
+    wait_done(smem_u32(&s.done[1]), x.phase1, s, x.dead);
+    finish_outputs(x, s, tmem, v0, lane, rq.chunks >= 2);
+    tmem_before();
+    bar_state();
+    if (issuer) {
+      tmem_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(kTmemColumns));
     }
   }
 }
