@@ -167,12 +167,15 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Named barriers of the chain kernel: the first three hand buffers between the threads that move data and
-// those that carry the state, kBarState joins the latter.
-constexpr int kBarFull = 1, kBarOReady = 3, kBarOFree = 4, kBarState = 5;
+// Named barriers of the chain kernel: the first ones hand over between the threads that move data and those
+// that carry the state, kBarState and kBarMove join each.
+constexpr int kBarFull = 1, kBarChunkDone = 3, kBarTaken = 4, kBarState = 5, kBarMove = 6;
 __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory");
+}
+__device__ __forceinline__ void bar_move() {
+  asm volatile("bar.sync %0, %1;" ::"n"(kBarMove), "n"(kMoveThreads) : "memory");
 }
 __device__ __forceinline__ void bar_state() {
   asm volatile("bar.sync %0, %1;" ::"n"(kBarState), "n"(kStateThreads) : "memory");
@@ -234,6 +237,19 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&r)[8][4]) {
         "=f"(r[3][2]), "=f"(r[3][3]), "=f"(r[4][0]), "=f"(r[4][1]), "=f"(r[4][2]), "=f"(r[4][3]), "=f"(r[5][0]),
         "=f"(r[5][1]), "=f"(r[5][2]), "=f"(r[5][3]), "=f"(r[6][0]), "=f"(r[6][1]), "=f"(r[6][2]), "=f"(r[6][3]),
         "=f"(r[7][0]), "=f"(r[7][1]), "=f"(r[7][2]), "=f"(r[7][3])
+      : "r"(addr)
+      : "memory");
+}
+
+// 32 columns likewise.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&r)[4][4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0][0]), "=f"(r[0][1]), "=f"(r[0][2]), "=f"(r[0][3]), "=f"(r[1][0]), "=f"(r[1][1]), "=f"(r[1][2]),
+        "=f"(r[1][3]), "=f"(r[2][0]), "=f"(r[2][1]), "=f"(r[2][2]), "=f"(r[2][3]), "=f"(r[3][0]), "=f"(r[3][1]),
+        "=f"(r[3][2]), "=f"(r[3][3])
       : "r"(addr)
       : "memory");
 }
@@ -307,7 +323,7 @@ __device__ __forceinline__ uint32_t pack_half(float x, float y) {
 __device__ __forceinline__ void split(float2 x, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x.x, x.y);
   const float2 f = __half22float2(h);
-  const float2 r = add2(x, make_float2(-f.x, -f.y));
+  const float2 r = fma2(f, make_float2(-1.0f, -1.0f), x);  // exact
   const __half2 l = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
@@ -797,15 +813,16 @@ struct __align__(1024) Stage {
 struct ChainSmem {
   Stage stage[2];
   __align__(16) float o[kChunk * kORow];
+  float s_down[kDim], u_down[kDim];  // what S q and P u of the chunk in work are scaled by, per value row
   uint64_t done[2];  // products finished: [0] what the state waits for, [1] what only the outputs do
   uint32_t tmem;
   volatile int stop;  // a wait ran out: nothing is stored any more
 };
 
 // TMEM columns (32 bits x 128 lanes, lane = value row); all 512 are allocated, so they start at 0.  dS takes
-// the place of Y and O, which are in registers by then, and P u that of R.
-constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW = 224, kTmemY = 288, kTmemO = 352,
-                   kTmemDs = 288, kTmemTr = 416, kTmemColumns = 512;
+// the place of Y and T R, which are in registers by then, and P u that of R.
+constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW = 224, kTmemY = 288, kTmemTr = 352,
+                   kTmemDs = 288, kTmemO = 416, kTmemColumns = 512;
 
 template <bool kVec>
 __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Request& rq, int64_t chunk,
@@ -841,23 +858,57 @@ __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, cons
                                        p.qkv_row, row_lo, row_hi, reinterpret_cast<uint16_t*>(st.v), tid);
 }
 
-// Gated RMSNorm of the chunk's outputs.  A warp takes two rows at a time, 16 lanes and twice four values
-// per lane each.  What the gate and the norm's weight make of a value is computed first, while the chain
-// finishes the tile (`wait` returns then).
-template <bool kVec, typename Wait>
-__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Request& rq,
-                                              int64_t chunk, int head, const float (&wt)[8], int tid, Wait wait) {
-  const int w = tid >> 5, lane = tid & 31, part = lane & 15;
+// The chunk's outputs S q + P u from TMEM to the output tile: this warp's 16 value rows.
+__device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, int v0, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
+  const float s0 = s.s_down[v0 + g], s1 = s.s_down[v0 + g + 8];
+  const float2 u0 = make_float2(s.u_down[v0 + g], s.u_down[v0 + g]);
+  const float2 u1 = make_float2(s.u_down[v0 + g + 8], s.u_down[v0 + g + 8]);
+  float o[8][4];
+  tmem_load(tmem + kTmemO, o);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const float2 qin = *reinterpret_cast<const float2*>(&st.f.q_in[8 * n + 2 * t]);
+    const float2 x0 = mul2(make_float2(o[n][0], o[n][1]), mul2(qin, make_float2(s0, s0)));
+    const float2 x1 = mul2(make_float2(o[n][2], o[n][3]), mul2(qin, make_float2(s1, s1)));
+    o[n][0] = x0.x;
+    o[n][1] = x0.y;
+    o[n][2] = x1.x;
+    o[n][3] = x1.y;
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float pu[4][4];
+    tmem_load(tmem + kTmemPu + 32 * half, pu);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int n = 4 * half + m;
+      const float2 x0 = fma2(make_float2(pu[m][0], pu[m][1]), u0, make_float2(o[n][0], o[n][1]));
+      const float2 x1 = fma2(make_float2(pu[m][2], pu[m][3]), u1, make_float2(o[n][2], o[n][3]));
+      float* at = s.o + (8 * n + 2 * t) * kORow + v0 + g;
+      at[0] = x0.x;
+      at[kORow] = x0.y;
+      at[8] = x1.x;
+      at[kORow + 8] = x1.y;
+    }
+  }
+}
+
+// Gated RMSNorm of the output tile.  A warp takes two rows at a time, 16 lanes and twice four values per lane
+// each.  `load_gates` starts the gate rows' loads early, `store_outputs` uses them.
+constexpr int kOutRows = kMoveThreads / 16, kOutSteps = kChunk / kOutRows;
+
+template <bool kVec>
+__device__ __forceinline__ void load_gates(const PrefillArgs& p, const Request& rq, int64_t chunk, int head, int tid,
+                                           uint2 (&z)[kOutSteps][2]) {
   const int64_t local0 = chunk * kChunk - rq.lead;
   const int row_lo = chunk == 0 ? rq.lead : 0;
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
-  constexpr int kRows = kMoveThreads / 16, kSteps = kChunk / kRows;
-  const int row0 = 2 * w + (lane >> 4);
-  const __nv_bfloat16* gate = p.gate + (rq.first + local0) * p.gate_row + head * kDim + 4 * part;
-  uint2 z[kSteps][2];
+  const __nv_bfloat16* gate = p.gate + (rq.first + local0) * p.gate_row + head * kDim + 4 * (tid & 15);
 #pragma unroll
-  for (int n = 0; n < kSteps; ++n) {
-    const int i = kRows * n + row0;
+  for (int n = 0; n < kOutSteps; ++n) {
+    const int i = kOutRows * n + (tid >> 4);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       z[n][half] = make_uint2(0, 0);
@@ -872,23 +923,21 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
       }
     }
   }
-  float f[kSteps][8];
-#pragma unroll
-  for (int n = 0; n < kSteps; ++n) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      f[n][4 * half + 0] = wt[4 * half + 0] * silu_fast(bf16_low(z[n][half].x));
-      f[n][4 * half + 1] = wt[4 * half + 1] * silu_fast(bf16_high(z[n][half].x));
-      f[n][4 * half + 2] = wt[4 * half + 2] * silu_fast(bf16_low(z[n][half].y));
-      f[n][4 * half + 3] = wt[4 * half + 3] * silu_fast(bf16_high(z[n][half].y));
-    }
-  }
-  wait();
+}
+
+template <bool kVec>
+__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Request& rq,
+                                              int64_t chunk, int head, const float (&wt)[8], int tid,
+                                              const uint2 (&z)[kOutSteps][2]) {
+  const int part = tid & 15;
+  const int64_t local0 = chunk * kChunk - rq.lead;
+  const int row_lo = chunk == 0 ? rq.lead : 0;
+  const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
   const bool stop = s.stop != 0;
   __nv_bfloat16* out = p.out + ((rq.first + local0) * p.num_v_heads + head) * kDim + 4 * part;
 #pragma unroll
-  for (int n = 0; n < kSteps; ++n) {
-    const int i = kRows * n + row0;
+  for (int n = 0; n < kOutSteps; ++n) {
+    const int i = kOutRows * n + (tid >> 4);
     float4 o[2];
     float sq = 0.0f;
 #pragma unroll
@@ -906,8 +955,12 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
     __nv_bfloat16* row = out + static_cast<int64_t>(i) * p.num_v_heads * kDim;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const uint32_t lo = pack_bf16(o[half].x * rstd * f[n][4 * half], o[half].y * rstd * f[n][4 * half + 1]);
-      const uint32_t hi = pack_bf16(o[half].z * rstd * f[n][4 * half + 2], o[half].w * rstd * f[n][4 * half + 3]);
+      const uint2 zz = z[n][half];
+      const float y0 = o[half].x * rstd * (wt[4 * half + 0] * silu_fast(bf16_low(zz.x)));
+      const float y1 = o[half].y * rstd * (wt[4 * half + 1] * silu_fast(bf16_high(zz.x)));
+      const float y2 = o[half].z * rstd * (wt[4 * half + 2] * silu_fast(bf16_low(zz.y)));
+      const float y3 = o[half].w * rstd * (wt[4 * half + 3] * silu_fast(bf16_high(zz.y)));
+      const uint32_t lo = pack_bf16(y0, y1), hi = pack_bf16(y2, y3);
       __nv_bfloat16* at = row + 64 * half;
       if (live) {
         if constexpr (kVec) {
@@ -973,8 +1026,8 @@ __device__ __forceinline__ void scale_rows(const float (&x)[kTiles][4], float& u
   float top0 = 0.0f, top1 = 0.0f;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
-    top0 = max_abs(top0, x[n][0], x[n][1]);
-    top1 = max_abs(top1, x[n][2], x[n][3]);
+    top0 = fmaxf(top0, fmaxf(fabsf(x[n][0]), fabsf(x[n][1])));
+    top1 = fmaxf(top1, fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
   }
   row_scale(quad_max(top0), up0, down0);
   row_scale(quad_max(top1), up1, down1);
@@ -1010,72 +1063,49 @@ __device__ __forceinline__ void scale_add(float (&f)[4], float2 a0, float2 a1, c
 
 // What the threads that carry the state keep between chunks.
 struct StateWarp {
-  float S[16][4];      // rows v0 + g, v0 + g + 8; columns 8n + 2t, + 1
-  float O[8][4];       // outputs of the chunk in work: columns are the chunk's rows
-  float down0, down1;  // what P u is scaled by
-  uint32_t phase0, phase1;
+  float S[16][4];  // rows v0 + g, v0 + g + 8; columns 8n + 2t, + 1
+  uint32_t phase;
   bool dead;
 };
 
-// The chunk's outputs, S q + P u, to the tile, once P u is done.
-__device__ __forceinline__ void finish_outputs(StateWarp& x, ChainSmem& s, uint32_t tmem, int v0, int lane, bool wait) {
-  const int g = lane >> 2, t = lane & 3;
-  float pu[8][4];
-  tmem_load(tmem + kTmemPu, pu);
-  if (wait) bar_sync(kBarOFree);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    float* at = s.o + (8 * n + 2 * t) * kORow + v0 + g;
-    at[0] = fmaf(pu[n][0], x.down0, x.O[n][0]);
-    at[kORow] = fmaf(pu[n][1], x.down0, x.O[n][1]);
-    at[8] = fmaf(pu[n][2], x.down1, x.O[n][2]);
-    at[kORow + 8] = fmaf(pu[n][3], x.down1, x.O[n][3]);
-  }
-  bar_arrive(kBarOReady);
-}
-
-// One chunk.  `tmem` carries this warp's lanes; one warp (`issuer`) issues the products.
-// `before` runs while S k is computed: it finishes the chunk before, if there is one (`more`).
-template <typename Before>
+// One chunk.  `tmem` carries this warp's lanes; one warp (`issuer`) issues the products.  `taken` returns when
+// the outputs of the chunk before have left TMEM.
+//
+// Parity waits are sound because every thread that waits on a barrier has seen a phase before the next one
+// can begin: the state's warps join (bar_state) between a wait on done[0] and the next commit to it, and
+// done[1]'s next commit comes after `taken`, which the waiting threads release.
+template <typename Taken>
 __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const Stage& st, uint32_t tmem, int v0, int lane,
-                                            bool issuer, bool more, Before before) {
-  const int t = lane & 3;
+                                            bool issuer, Taken taken) {
+  const int g = lane >> 2, t = lane & 3;
   const uint32_t done0 = smem_u32(&s.done[0]), done1 = smem_u32(&s.done[1]);
 
-  // Y = S k~ (two terms) and O = S q~ (hi term).
+  // Y = S k~ (two terms).
   float up0, down0, up1, down1;
   scale_rows(x.S, up0, down0, up1, down1);
   store_split(x.S, 0, up0, up1, tmem + kTmemS, tmem + kTmemS + 64);
   store_split(x.S, 8, up0, up1, tmem + kTmemS + 32, tmem + kTmemS + 96);
   tmem_stored();
-  // The chunk before's P u: every warp has seen a barrier's phase before the next one can begin, here and
-  // at the other two joins, so that waiting by parity is sound.
-  if (more) {
-    wait_done(done1, x.phase1, s, x.dead);
-    x.phase1 ^= 1;
-  }
   tmem_before();
   bar_state();
   if (issuer && !x.dead) {
     tmem_after();
     const uint32_t elected = elect_lane();
-    const uint64_t kq = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
-    // Rows 0-63 of a half are k's, 64-127 q's: 128 columns of D are Y and O.
+    const uint64_t k = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      umma(elected, kTmemY, kTmemS + 8 * ks, kq + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(128, false), ks > 0);
-    }
+    for (int term = 1; term >= 0; --term) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      umma(elected, kTmemY, kTmemS + 64 + 8 * ks, kq + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(64, false), true);
+      for (int ks = 0; ks < 8; ++ks) {
+        umma(elected, kTmemY, kTmemS + 64 * term + 8 * ks, k + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2,
+             mma_shape(64, false), term == 0 || ks > 0);
+      }
     }
     umma_commit(elected, done0);
   }
-  before();
 
   // R = beta (v - k_in Y).
-  wait_done(done0, x.phase0, s, x.dead);
-  x.phase0 ^= 1;
+  wait_done(done0, x.phase, s, x.dead);
+  x.phase ^= 1;
   float Y[8][4];
   tmem_load(tmem + kTmemY, Y);
   const uint32_t v_base = lane_addr<false>(st.v, lane);
@@ -1100,7 +1130,11 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
       f[3] = z1.y;
     }
   }
-  const float s_down0 = down0, s_down1 = down1;
+  taken();  // R takes the place of the chunk before's P u
+  if (t == 0) {
+    s.s_down[v0 + g] = down0;
+    s.s_down[v0 + g + 8] = down1;
+  }
   scale_rows(Y, up0, down0, up1, down1);
   store_split(Y, 0, up0, up1, tmem + kTmemR, tmem + kTmemR + 32);
   tmem_stored();
@@ -1122,51 +1156,47 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
       }
     }
     umma_commit(elected, done0);
-  }
-  tmem_load(tmem + kTmemO, x.O);
+    // O = S q~ (hi term), while the others go on.
+    const uint64_t q = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq + kHalf), 0));
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const float2 qin = *reinterpret_cast<const float2*>(&st.f.q_in[8 * n + 2 * t]);
-    const float2 o0 = mul2(make_float2(x.O[n][0], x.O[n][1]), mul2(qin, make_float2(s_down0, s_down0)));
-    const float2 o1 = mul2(make_float2(x.O[n][2], x.O[n][3]), mul2(qin, make_float2(s_down1, s_down1)));
-    x.O[n][0] = o0.x;
-    x.O[n][1] = o0.y;
-    x.O[n][2] = o1.x;
-    x.O[n][3] = o1.y;
+    for (int ks = 0; ks < 8; ++ks) {
+      umma(elected, kTmemO, kTmemS + 8 * ks, q + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(64, false), ks > 0);
+    }
   }
-
-  // u, and k_out u in two terms.
-  wait_done(done0, x.phase0, s, x.dead);
-  x.phase0 ^= 1;
+  // u, and k_out u in two terms.  k_out is at most 1 (the largest k~ of a row is in [1, 2)), so u's row
+  // scale serves both.
+  wait_done(done0, x.phase, s, x.dead);
+  x.phase ^= 1;
   tmem_load(tmem + kTmemTr, Y);
   const float r_down0 = down0, r_down1 = down1;
+  scale_rows(Y, up0, down0, up1, down1);
+  const float w0 = r_down0 * down0, w1 = r_down1 * down1;
+  if (t == 0) {
+    s.u_down[v0 + g] = w0;
+    s.u_down[v0 + g + 8] = w1;
+  }
   {
-    scale_rows(Y, up0, down0, up1, down1);
     uint32_t hi[4][4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float(&f)[4] = Y[2 * ks + m];
-        hi[ks][2 * m] = pack_half(f[0] * up0, f[1] * up0);
-        hi[ks][2 * m + 1] = pack_half(f[2] * up1, f[3] * up1);
+        float(&f)[4] = Y[2 * ks + m];
+        const float2 u0 = mul2(make_float2(f[0], f[1]), make_float2(up0, up0));
+        const float2 u1 = mul2(make_float2(f[2], f[3]), make_float2(up1, up1));
+        hi[ks][2 * m] = pack_half(u0.x, u0.y);
+        hi[ks][2 * m + 1] = pack_half(u1.x, u1.y);
+        const float2 kout = *reinterpret_cast<const float2*>(&st.f.k_out[16 * ks + 8 * m + 2 * t]);
+        const float2 k0 = mul2(u0, kout), k1 = mul2(u1, kout);
+        f[0] = k0.x;
+        f[1] = k0.y;
+        f[2] = k1.x;
+        f[3] = k1.y;
       }
     }
     tmem_store(tmem + kTmemU, hi);
-    x.down0 = r_down0 * down0;
-    x.down1 = r_down1 * down1;
   }
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const float2 kout = *reinterpret_cast<const float2*>(&st.f.k_out[8 * n + 2 * t]);
-    const float2 u0 = mul2(make_float2(Y[n][0], Y[n][1]), kout), u1 = mul2(make_float2(Y[n][2], Y[n][3]), kout);
-    Y[n][0] = u0.x;
-    Y[n][1] = u0.y;
-    Y[n][2] = u1.x;
-    Y[n][3] = u1.y;
-  }
-  scale_rows(Y, up0, down0, up1, down1);
-  store_split(Y, 0, up0, up1, tmem + kTmemW, tmem + kTmemW + 32);
+  store_split(Y, 0, 1.0f, 1.0f, tmem + kTmemW, tmem + kTmemW + 32);
   tmem_stored();
   tmem_before();
   bar_state();
@@ -1193,14 +1223,14 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   }
   // S <- decay S + dS, one fp32 fused multiply-add per element.
   const float2 decay = make_float2(st.f.decay, st.f.decay);
-  const float2 w0 = make_float2(r_down0 * down0, r_down0 * down0), w1 = make_float2(r_down1 * down1, r_down1 * down1);
-  wait_done(done0, x.phase0, s, x.dead);
-  x.phase0 ^= 1;
+  const float2 w02 = make_float2(w0, w0), w12 = make_float2(w1, w1);
+  wait_done(done0, x.phase, s, x.dead);
+  x.phase ^= 1;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     tmem_load(tmem + kTmemDs + 64 * half, Y);
 #pragma unroll
-    for (int n = 0; n < 8; ++n) scale_add(x.S[8 * half + n], decay, decay, Y[n], w0, w1);
+    for (int n = 0; n < 8; ++n) scale_add(x.S[8 * half + n], decay, decay, Y[n], w02, w12);
   }
 }
 
@@ -1226,9 +1256,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kStateWarp = kMoveThreads / 32;
 
-  // Launched with 512 x 128 registers; 256 x 80 + 256 x 176 is the same 65,536.
+  // Launched with 512 x 128 registers; 256 x 96 + 256 x 160 is the same 65,536.
   if (warp < kStateWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int tid = threadIdx.x;
     const int64_t base = chunk_base(rq.first, r);
     const auto hand_over = [&](int stage) {
@@ -1243,18 +1273,27 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     float wt[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) wt[e] = load_param(p.weight, 64 * (e >> 2) + 4 * (lane & 15) + (e & 3), p.weight_bf16);
+    const int v0 = 32 * (warp & 3) + 16 * (warp >> 2);  // the TMEM lanes of a warp, as below
+    uint32_t phase = 0;
+    bool dead = false;
+    uint2 z[kOutSteps][2];
     for (int64_t c = 0; c < rq.chunks; ++c) {
       const int stage = static_cast<int>(c & 1);
-      store_outputs<kVec>(p, s, rq, c, head, wt, tid, [&] {
-        // The outputs of chunk c are there, and every product on it is done, so its stage is free.
-        bar_sync(kBarOReady);
-        if (c + 2 < rq.chunks) copy_chunk<kVec>(p, s.stage[stage], rq, c + 2, base + c + 2, head, tid);
-      });
-      if (c + 1 < rq.chunks) bar_arrive(kBarOFree);
+      load_gates<kVec>(p, rq, c, head, tid, z);
+      bar_sync(kBarChunkDone);
+      wait_done(smem_u32(&s.done[1]), phase, s, dead);
+      phase ^= 1;
+      gather_outputs(s, s.stage[stage], v0, lane);
+      tmem_before();
+      bar_move();  // the tile is whole, and the stage read for the last time
+      if (c + 1 < rq.chunks) bar_arrive(kBarTaken);
+      if (c + 2 < rq.chunks) copy_chunk<kVec>(p, s.stage[stage], rq, c + 2, base + c + 2, head, tid);
+      store_outputs<kVec>(p, s, rq, c, head, wt, tid, z);
       if (c + 2 < rq.chunks) hand_over(stage);
+      bar_move();  // the tile is free again
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     const int g = lane >> 2, t = lane & 3;
     // A warp reaches the TMEM lanes of its number mod 4; two warps share them, 16 lanes each.
     const int v0 = 32 * (warp & 3) + 16 * ((warp - kStateWarp) >> 2);
@@ -1276,7 +1315,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     }
     StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(head) * kDim * kDim + (v0 + g) * kDim + 2 * t;
     StateWarp x;
-    x.phase0 = x.phase1 = 0;
+    x.phase = 0;
     x.dead = false;
     if (rq.source > 0) {
       const StateT* at = pool + rq.source * p.slot_stride;
@@ -1302,9 +1341,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     for (int64_t c = 0; c < rq.chunks; ++c) {
       const int stage = static_cast<int>(c & 1);
       bar_sync(kBarFull + stage);
-      chain_chunk(x, s, s.stage[stage], tmem, v0, lane, issuer, c >= 1, [&] {
-        if (c >= 1) finish_outputs(x, s, tmem, v0, lane, c >= 2);
+      chain_chunk(x, s, s.stage[stage], tmem, v0, lane, issuer, [&] {
+        if (c >= 1) {
+          bar_sync(kBarTaken);
+          tmem_after();
+        }
       });
+      bar_arrive(kBarChunkDone);
       if (c + 1 == rq.chunks || --left == 0) {  // a block or the request ends here: its slot takes the state
         const int32_t slot = *slot_at++;
         left = per_block;
@@ -1322,14 +1365,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         }
       }
     }
-    wait_done(smem_u32(&s.done[1]), x.phase1, s, x.dead);
-    finish_outputs(x, s, tmem, v0, lane, rq.chunks >= 2);
-    tmem_before();
-    bar_state();
-    if (issuer) {
-      tmem_after();
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(kTmemColumns));
-    }
+  }
+  // Everybody has taken what it needs from TMEM.
+  tmem_before();
+  __syncthreads();
+  if (warp == kStateWarp) {
+    tmem_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(kTmemColumns));
   }
 }
 
