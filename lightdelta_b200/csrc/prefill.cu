@@ -41,6 +41,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -111,6 +113,9 @@ struct PrefillArgs {
   int64_t block_size;
   KeyImage* keys;    // [chunk places, num_k_heads]
   PairImage* pairs;  // [chunk places, num_v_heads]
+  int32_t* order;    // requests, longest first
+  uint32_t* next;    // items that the chain's CTAs have taken
+  int64_t places;
   int n_requests;
   int num_k_heads;
   int num_v_heads;
@@ -167,9 +172,9 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Named barriers of the chain kernel: the first ones hand over between the threads that move data and those
-// that carry the state, kBarState and kBarMove join each.
-constexpr int kBarFull = 1, kBarChunkDone = 3, kBarTaken = 4, kBarState = 5, kBarMove = 6;
+// Named barriers of the chain kernel: the first ones and kBarFull hand over between the threads that move data
+// and those that carry the state, kBarState and kBarMove join each.
+constexpr int kBarChunkDone = 1, kBarTaken = 2, kBarState = 3, kBarMove = 4, kBarFull = 5;
 __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kChainThreads) : "memory");
@@ -193,6 +198,13 @@ __host__ __device__ constexpr uint32_t mma_shape(int n, bool b_mn_major) {
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
   return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(2 * kKeyHalf >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// The same of a packed triangular matrix's 16-column block, without swizzle: core matrices 128 bytes apart along
+// the columns, 256 along the rows.
+__device__ __forceinline__ uint64_t tri_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(128 >> 4) << 16) |
+         (static_cast<uint64_t>(256 >> 4) << 32) | (1ull << 46);
 }
 
 __device__ __forceinline__ uint32_t elect_lane() {
@@ -268,10 +280,19 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
   const int bytes = live ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void barrier_init(uint32_t bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
 
 // ------------------------------------------------------------------------------------------
 // swizzled tiles: 64 rows of 64 16-bit columns, 128 bytes a row, whose 16-byte pieces are stored at
@@ -300,19 +321,22 @@ __device__ __forceinline__ uint32_t block(uint32_t addr, int rb, int cb) {
   return (addr ^ ((cb & 3) << 5)) + (cb >> 2) * (2 * kStride) + rb * (16 * 128);
 }
 
-// Packed triangular matrices: block (ib, jb), jb <= ib, of 16 rows of 32 bytes; the two 16-byte pieces of
-// rows 4-7 and 12-15 are exchanged, so that eight rows' pieces lie in different banks.
-__device__ __forceinline__ int tri(int row, int col) {
-  const int ib = row >> 4, jb = col >> 4, r = row & 15, c = col & 15;
-  return (ib * (ib + 1) / 2 + jb) * 256 + r * 16 + ((((c >> 3) ^ ((r >> 2) & 1)) << 3) | (c & 7));
-}
+// Packed triangular matrices: 16-column blocks one after the other, each from its diagonal block down, in 8 x 8
+// core matrices of 128 contiguous bytes, the two of a row group side by side: matrix descriptors without
+// swizzle read a column block's rows from any row group on, and ldmatrix reads core matrices without bank
+// conflicts.
+__host__ __device__ constexpr int tri_block(int ib, int jb) { return 256 * (4 * jb - jb * (jb - 1) / 2 + (ib - jb)); }
 
-// This lane's ldmatrix.x4 address in block 0 of a packed matrix, matrices in the order of lane_addr with
-// kRowsFirst false; block b is 512 bytes on per block.
-__device__ __forceinline__ uint32_t tri_addr(const __half* m, int lane) {
-  return smem_u32(m) + 2 * tri((lane & 7) + 8 * (lane >> 4), 8 * ((lane >> 3) & 1));
+__device__ __forceinline__ int core(int row, int col) {  // within a 16 x 16 block
+  return (row >> 3) * 128 + (col >> 3) * 64 + (row & 7) * 8 + (col & 7);
 }
-__host__ __device__ constexpr int tri_block(int ib, int jb) { return (ib * (ib + 1) / 2 + jb) * 512; }
+__device__ __forceinline__ int tri(int row, int col) { return tri_block(row >> 4, col >> 4) + core(row & 15, col & 15); }
+
+// This lane's ldmatrix.x4 address in the 16 x 16 block at `m`, matrices in the order of lane_addr with
+// kRowsFirst false.
+__device__ __forceinline__ uint32_t core_addr(const __half* m, int lane) {
+  return smem_u32(m) + 2 * core((lane & 7) + 8 * (lane >> 4), 8 * ((lane >> 3) & 1));
+}
 
 __device__ __forceinline__ uint32_t pack_half(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -373,22 +397,21 @@ struct PairSmem {
 };
 static_assert(sizeof(PairWork) <= sizeof(KeyImage), "the work area takes the tiles' place");
 
-// Element (row, col) of a block strictly below the diagonal of the packed L, and the byte offset of a block.
-__host__ __device__ constexpr int low_block(int ib, int jb) { return (ib * (ib - 1) / 2 + jb) * 512; }
-__device__ __forceinline__ int low(int row, int col) {
-  const int r = row & 15, c = col & 15;
-  return low_block(row >> 4, col >> 4) / 2 + r * 16 + ((((c >> 3) ^ ((r >> 2) & 1)) << 3) | (c & 7));
-}
+// L's blocks below the diagonal ones, row by row.
+__host__ __device__ constexpr int low_block(int ib, int jb) { return 256 * (ib * (ib - 1) / 2 + jb); }
+__device__ __forceinline__ int low(int row, int col) { return low_block(row >> 4, col >> 4) + core(row & 15, col & 15); }
 
-template <bool kVec, int kThreads, int kStride>
+// Rows [row_lo, row_hi) of 128 bf16 to shared memory, the others as zeros, 16 bytes a thread at a time; `at` gives
+// the element that (row, column) goes to.
+template <bool kVec, int kThreads, typename At>
 __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row_stride, int row_lo, int row_hi,
-                                          uint16_t* tile, int tid) {
+                                          uint16_t* tile, int tid, At at) {
 #pragma unroll
   for (int pass = 0; pass < kChunk / (kThreads / 16); ++pass) {
     const int i = pass * (kThreads / 16) + (tid >> 4);
     const int col = (tid & 15) * 8;
     const bool live = i >= row_lo && i < row_hi;
-    uint16_t* dst = tile + swz<kStride>(i, col);
+    uint16_t* dst = tile + at(i, col);
     const __nv_bfloat16* src = base + static_cast<int64_t>(live ? i : row_lo) * row_stride + col;
     if constexpr (kVec) {
       cp_async16(smem_u32(dst), src, live);
@@ -606,12 +629,12 @@ __device__ __forceinline__ void invert_diagonal(PairSmem& s, int w, int lane) {
 // The 16 x 16 blocks of T below diagonal block w, top to bottom:
 //   T_iw = -T_ii sum_{k=w}^{i-1} L_ik T_kw,  held transposed so that each result is the next A operand.
 __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
-  const uint32_t t_hi = tri_addr(s.work().image.t_hi, lane), t_lo = tri_addr(s.work().image.t_lo, lane);
-  const uint32_t l_hi = tri_addr(s.work().l_hi, lane), l_lo = tri_addr(s.work().l_lo, lane);
+  const uint32_t t_hi = core_addr(s.work().image.t_hi, lane), t_lo = core_addr(s.work().image.t_lo, lane);
+  const uint32_t l_hi = core_addr(s.work().l_hi, lane), l_lo = core_addr(s.work().l_lo, lane);
   uint32_t x_hi[3][4], x_lo[3][4];  // T_kw^T as A fragments, k = w, w + 1, w + 2
   // ldmatrix.trans of T_ww: matrices (cols 0-7, rows 0-7), (cols 8-15, rows 0-7), (0-7, 8-15), (8-15, 8-15).
-  ldsm4_t(t_hi + tri_block(w, w), x_hi[0]);
-  ldsm4_t(t_lo + tri_block(w, w), x_lo[0]);
+  ldsm4_t(t_hi + 2 * tri_block(w, w), x_hi[0]);
+  ldsm4_t(t_lo + 2 * tri_block(w, w), x_lo[0]);
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int d = 1; d < 4; ++d) {
@@ -621,8 +644,8 @@ __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
 #pragma unroll
       for (int kk = 0; kk < d; ++kk) {
         uint32_t b_hi[4], b_lo[4];
-        ldsm4(l_hi + low_block(i, w + kk), b_hi);
-        ldsm4(l_lo + low_block(i, w + kk), b_lo);
+        ldsm4(l_hi + 2 * low_block(i, w + kk), b_hi);
+        ldsm4(l_lo + 2 * low_block(i, w + kk), b_lo);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           mma(m[n], x_hi[kk], b_lo[2 * n], b_lo[2 * n + 1]);
@@ -638,8 +661,8 @@ __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
       }
       float y[2][4] = {};
       uint32_t b_hi[4], b_lo[4];
-      ldsm4(t_hi + tri_block(i, i), b_hi);
-      ldsm4(t_lo + tri_block(i, i), b_lo);
+      ldsm4(t_hi + 2 * tri_block(i, i), b_hi);
+      ldsm4(t_lo + 2 * tri_block(i, i), b_lo);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         mma(y[n], a_hi, b_lo[2 * n], b_lo[2 * n + 1]);
@@ -704,6 +727,33 @@ __device__ __forceinline__ bool find_request(const PrefillArgs& p, int64_t r, Re
   return true;
 }
 
+// Requests by their chunk counts, longest first (to half an octave), for the chain to take in this order;
+// equal ones in any order.  One CTA.
+__device__ __forceinline__ void order_requests(const PrefillArgs& p, int tid) {
+  __shared__ uint32_t counts[64];
+  if (tid < 64) counts[tid] = 0;
+  if (tid == 0) *p.next = 0;
+  __syncthreads();
+  const auto bucket = [&](int r) {
+    const int tokens = max(p.cu[r + 1] - p.cu[r], 1);
+    const int chunks = tokens / kChunk + 1;  // to one
+    const int octave = 31 - __clz(chunks);
+    return 63 - (2 * octave + (octave > 0 ? (chunks >> (octave - 1)) & 1 : 0));
+  };
+  for (int r = tid; r < p.n_requests; r += kPairThreads) atomicAdd(&counts[bucket(r)], 1u);
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t sum = 0;
+    for (int b = 0; b < 64; ++b) {
+      const uint32_t n = counts[b];
+      counts[b] = sum;
+      sum += n;
+    }
+  }
+  __syncthreads();
+  for (int r = tid; r < p.n_requests; r += kPairThreads) p.order[atomicAdd(&counts[bucket(r)], 1u)] = r;
+}
+
 template <bool kVec>
 __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(const PrefillArgs p) {
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -711,8 +761,12 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   grid_dependency_wait();
   allow_dependent_launch();
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int64_t place = blockIdx.x / p.num_k_heads;
-  const int kh = static_cast<int>(blockIdx.x - place * p.num_k_heads);
+  if (blockIdx.x == 0) {
+    order_requests(p, tid);
+    return;
+  }
+  const int64_t place = (blockIdx.x - 1) / p.num_k_heads;
+  const int kh = static_cast<int>(blockIdx.x - 1 - place * p.num_k_heads);
   // The request of this place: the last r whose places start at or before it, by 32-way bisection.
   int lo = 0, hi = p.n_requests;
   while (hi - lo > 1) {
@@ -738,8 +792,9 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
   const __nv_bfloat16* rows = p.qkv + token0 * p.qkv_row;
   uint16_t* tiles = reinterpret_cast<uint16_t*>(s.kq());
-  load_rows<kVec, kPairThreads, kKeyHalf>(rows + (p.num_k_heads + kh) * kDim, p.qkv_row, row_lo, row_hi, tiles, tid);
-  load_rows<kVec, kPairThreads, kKeyHalf>(rows + kh * kDim, p.qkv_row, row_lo, row_hi, tiles + kHalf, tid);
+  const auto at = [](int row, int col) { return swz<kKeyHalf>(row, col); };
+  load_rows<kVec, kPairThreads>(rows + (p.num_k_heads + kh) * kDim, p.qkv_row, row_lo, row_hi, tiles, tid, at);
+  load_rows<kVec, kPairThreads>(rows + kh * kDim, p.qkv_row, row_lo, row_hi, tiles + kHalf, tid, at);
   const int head0 = kh * p.heads_ratio;
   if (w < p.heads_ratio) chunk_gates(p, s, w, token0, row_lo, row_hi, head0 + w, lane);
   if constexpr (kVec) cp_async_wait();
@@ -795,27 +850,47 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
 // ------------------------------------------------------------------------------------------
 // chain: the state through the chunks
 // ------------------------------------------------------------------------------------------
-struct Factors {
-  float beta[kChunk], k_in[kChunk], q_in[kChunk], k_out[kChunk];
-  float decay;
+constexpr int kVRow = kDim + 8;  // bf16 per row of a stage's v: the 16 bytes spread its rows over the banks
+
+// What a stage holds: one chunk of one item.
+struct Work {
+  int64_t token0;      // the token of row 0 (rows in front of row_lo have none)
+  int64_t place;       // the chunk's place in the workspace; kWorkZero: the item's tokens
+  int32_t row_lo, row_hi;
+  int32_t head;
+  int32_t source;      // -1: the state goes on; else the slot that it starts from (0: from nothing)
+  int32_t slot;        // the slot that takes the state after the chunk (0: none)
+  int32_t kind;
 };
-constexpr int kFactorPieces = (4 * kChunk * 4 + 16) / 16;  // 16-byte pieces from PairImage::beta on that hold Factors
-static_assert(sizeof(Factors) <= 16 * kFactorPieces && kFactorPieces <= kMoveThreads, "one copy per thread");
+constexpr int kWorkChunk = 0, kWorkEnd = 1, kWorkZero = 2;  // a chunk; no more items; an item whose outputs are zeros
+
+// Where the item in work is, kept and used by one thread.
+struct Cursor {
+  int64_t first, tokens, chunks;  // of the item: its first token, its tokens and chunks
+  int64_t base;                   // place of its first chunk
+  int64_t chunk;                  // next chunk
+  int64_t left;                   // chunks to the end of the block that it is in
+  const int32_t* slot_at;
+  uint32_t ahead;                 // the item after this one, already taken
+  int32_t lead, head;
+};
 
 struct __align__(1024) Stage {
   __half kq[2 * kChunk * kDim];
-  __nv_bfloat16 v[kChunk * kDim];
-  __half t_hi[kHalf], t_lo[kHalf], p[kHalf];  // 16 x 16 blocks above the diagonal are never read
-  __align__(16) Factors f;
-  float pad[3];  // the last piece of the factors is copied whole
+  PairImage pair;
+  __align__(16) __nv_bfloat16 v[kChunk * kVRow];
+  Work work;
 };
 
 struct ChainSmem {
   Stage stage[2];
   __align__(16) float o[kChunk * kORow];
   float s_down[kDim], u_down[kDim];  // what S q and P u of the chunk in work are scaled by, per value row
+  uint64_t full[2];  // a stage's copies have landed
   uint64_t done[2];  // products finished: [0] what the state waits for, [1] what only the outputs do
   uint32_t tmem;
+  Cursor at;
+  Work upcoming;      // what the next free stage takes
   volatile int stop;  // a wait ran out: nothing is stored any more
 };
 
@@ -824,38 +899,21 @@ struct ChainSmem {
 constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW = 224, kTmemY = 288, kTmemTr = 352,
                    kTmemDs = 288, kTmemO = 416, kTmemColumns = 512;
 
+// The chunk's images to a stage by two bulk copies, its v rows by the moving threads.
 template <bool kVec>
-__device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Request& rq, int64_t chunk,
-                                           int64_t place, int head, int tid) {
-  const int kh = head / p.heads_ratio;
-  const unsigned char* key = reinterpret_cast<const unsigned char*>(p.keys + place * p.num_k_heads + kh) + 16 * tid;
-  const uint32_t key_to = smem_u32(st.kq) + 16 * tid;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(KeyImage)) / (16 * kMoveThreads); ++i) {
-    cp_async16(key_to + 16 * kMoveThreads * i, key + 16 * kMoveThreads * i);
+__device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid) {
+  // What was read and written in this stage so far comes before the bulk copies, which go through the async
+  // proxy (a barrier lies between that and this thread).
+  if (tid == 0) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    barrier_expect(full, sizeof(KeyImage) + sizeof(PairImage));
+    bulk_copy(smem_u32(st.kq), p.keys + d.place * p.num_k_heads + d.head / p.heads_ratio, sizeof(KeyImage), full);
+    bulk_copy(smem_u32(&st.pair), p.pairs + d.place * p.num_v_heads + d.head, sizeof(PairImage), full);
   }
-  // A warp copies whole packed blocks, 32 pieces each, to their places in the tiles.
-  const PairImage* image = p.pairs + place * p.num_v_heads + head;
-  const unsigned char* packed = reinterpret_cast<const unsigned char*>(image);
-  const int w = tid >> 5, lane = tid & 31;
-  const int row = lane >> 1, part = (lane & 1) ^ ((row >> 2) & 1);
-  const uint32_t tri_to = smem_u32(st.t_hi) + row * 128;
-  constexpr int kWarps = kMoveThreads / 32, kUnits = 3 * kTriBlocks;
-#pragma unroll
-  for (int i = 0; i < (kUnits + kWarps - 1) / kWarps; ++i) {
-    const int unit = w + kWarps * i;
-    if (unit < kUnits) {
-      const int m = unit / kTriBlocks, b = unit - m * kTriBlocks;
-      const int ib = (b >= 1) + (b >= 3) + (b >= 6), jb = b - ib * (ib + 1) / 2;
-      cp_async16(tri_to + m * (2 * kHalf) + ib * 2048 + (((2 * jb + part) ^ (row & 7)) << 4), packed + unit * 512 + lane * 16);
-    }
-  }
-  if (tid < kFactorPieces) cp_async16(smem_u32(&st.f) + 16 * tid, reinterpret_cast<const unsigned char*>(image->beta) + 16 * tid);
-  const int64_t local0 = chunk * kChunk - rq.lead;
-  const int row_lo = chunk == 0 ? rq.lead : 0;
-  const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
-  load_rows<kVec, kMoveThreads, kHalf>(p.qkv + (rq.first + local0) * p.qkv_row + (2 * p.num_k_heads + head) * kDim,
-                                       p.qkv_row, row_lo, row_hi, reinterpret_cast<uint16_t*>(st.v), tid);
+  // Rows of no token are zeros: their beta is 0, but 0 times what lies there need not be 0.
+  load_rows<kVec, kMoveThreads>(p.qkv + d.token0 * p.qkv_row + (2 * p.num_k_heads + d.head) * kDim, p.qkv_row, d.row_lo,
+                                d.row_hi, reinterpret_cast<uint16_t*>(st.v), tid,
+                                [](int row, int col) { return row * kVRow + col; });
 }
 
 // The chunk's outputs S q + P u from TMEM to the output tile: this warp's 16 value rows.
@@ -869,7 +927,7 @@ __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, in
   tmem_load(tmem + kTmemO, o);
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    const float2 qin = *reinterpret_cast<const float2*>(&st.f.q_in[8 * n + 2 * t]);
+    const float2 qin = *reinterpret_cast<const float2*>(&st.pair.q_in[8 * n + 2 * t]);
     const float2 x0 = mul2(make_float2(o[n][0], o[n][1]), mul2(qin, make_float2(s0, s0)));
     const float2 x1 = mul2(make_float2(o[n][2], o[n][3]), mul2(qin, make_float2(s1, s1)));
     o[n][0] = x0.x;
@@ -900,19 +958,15 @@ __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, in
 constexpr int kOutRows = kMoveThreads / 16, kOutSteps = kChunk / kOutRows;
 
 template <bool kVec>
-__device__ __forceinline__ void load_gates(const PrefillArgs& p, const Request& rq, int64_t chunk, int head, int tid,
-                                           uint2 (&z)[kOutSteps][2]) {
-  const int64_t local0 = chunk * kChunk - rq.lead;
-  const int row_lo = chunk == 0 ? rq.lead : 0;
-  const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
-  const __nv_bfloat16* gate = p.gate + (rq.first + local0) * p.gate_row + head * kDim + 4 * (tid & 15);
+__device__ __forceinline__ void load_gates(const PrefillArgs& p, const Work& d, int tid, uint2 (&z)[kOutSteps][2]) {
+  const __nv_bfloat16* gate = p.gate + d.token0 * p.gate_row + d.head * kDim + 4 * (tid & 15);
 #pragma unroll
   for (int n = 0; n < kOutSteps; ++n) {
     const int i = kOutRows * n + (tid >> 4);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       z[n][half] = make_uint2(0, 0);
-      if (i >= row_lo && i < row_hi) {
+      if (i >= d.row_lo && i < d.row_hi) {
         const __nv_bfloat16* at = gate + i * p.gate_row + 64 * half;
         if constexpr (kVec) {
           z[n][half] = *reinterpret_cast<const uint2*>(at);
@@ -926,15 +980,11 @@ __device__ __forceinline__ void load_gates(const PrefillArgs& p, const Request& 
 }
 
 template <bool kVec>
-__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Request& rq,
-                                              int64_t chunk, int head, const float (&wt)[8], int tid,
-                                              const uint2 (&z)[kOutSteps][2]) {
+__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Work& d,
+                                              const float (&wt)[8], int tid, const uint2 (&z)[kOutSteps][2]) {
   const int part = tid & 15;
-  const int64_t local0 = chunk * kChunk - rq.lead;
-  const int row_lo = chunk == 0 ? rq.lead : 0;
-  const int row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), rq.tokens - local0));
   const bool stop = s.stop != 0;
-  __nv_bfloat16* out = p.out + ((rq.first + local0) * p.num_v_heads + head) * kDim + 4 * part;
+  __nv_bfloat16* out = p.out + (d.token0 * p.num_v_heads + d.head) * kDim + 4 * part;
 #pragma unroll
   for (int n = 0; n < kOutSteps; ++n) {
     const int i = kOutRows * n + (tid >> 4);
@@ -951,7 +1001,7 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     const float rstd = rsqrtf(sq * (1.0f / kDim) + p.eps);
-    const bool live = i >= row_lo && i < row_hi && !stop;
+    const bool live = i >= d.row_lo && i < d.row_hi && !stop;
     __nv_bfloat16* row = out + static_cast<int64_t>(i) * p.num_v_heads * kDim;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -1108,16 +1158,17 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   x.phase ^= 1;
   float Y[8][4];
   tmem_load(tmem + kTmemY, Y);
-  const uint32_t v_base = lane_addr<false>(st.v, lane);
+  const uint32_t v_base =
+      smem_u32(st.v) + 2 * (((lane & 7) + 8 * (lane >> 4)) * kVRow + v0 + 8 * ((lane >> 3) & 1));
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
     uint32_t vt[4];  // v transposed: (rows 16nb.., cols v0..), (.., v0 + 8..), (rows 16nb + 8.., ...)
-    ldsm4_t(block<kHalf>(v_base, nb, v0 / 16), vt);
+    ldsm4_t(v_base + nb * (16 * kVRow * 2), vt);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       float(&f)[4] = Y[2 * nb + m];
-      const float2 kin = *reinterpret_cast<const float2*>(&st.f.k_in[16 * nb + 8 * m + 2 * t]);
-      const float2 beta = *reinterpret_cast<const float2*>(&st.f.beta[16 * nb + 8 * m + 2 * t]);
+      const float2 kin = *reinterpret_cast<const float2*>(&st.pair.k_in[16 * nb + 8 * m + 2 * t]);
+      const float2 beta = *reinterpret_cast<const float2*>(&st.pair.beta[16 * nb + 8 * m + 2 * t]);
       const uint32_t r0 = vt[2 * m], r1 = vt[2 * m + 1];
       const float2 y0 = fma2(mul2(kin, make_float2(-down0, -down0)), make_float2(f[0], f[1]),
                              make_float2(bf16_low(r0), bf16_high(r0)));
@@ -1140,19 +1191,19 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   tmem_stored();
   tmem_before();
   bar_state();
-  // U = T R (the product of the two lo terms is below fp32's last bit).  Column block ks of T starts at row
+  // U = T R (the product of the two lo terms is below fp32's last bit).  T's column block ks starts at row
   // block ks.
   if (issuer && !x.dead) {
     tmem_after();
     const uint32_t elected = elect_lane();
-    const uint64_t t_hi = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.t_hi), 0));
-    const uint64_t t_lo = t_hi + (2 * kHalf >> 4);
+    const uint64_t t_hi = tri_desc(__shfl_sync(0xffffffffu, smem_u32(st.pair.t_hi), 0));
+    const uint64_t t_lo = t_hi + (sizeof(st.pair.t_hi) >> 4);
 #pragma unroll
     for (int term = 0; term < 3; ++term) {  // hi lo, lo hi, hi hi
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         umma(elected, kTmemTr + 16 * ks, kTmemR + (term == 1 ? 32 : 0) + 8 * ks,
-             (term == 0 ? t_lo : t_hi) + ks * (2048 >> 4) + ks * 2, mma_shape(64 - 16 * ks, false), term > 0 || ks > 0);
+             (term == 0 ? t_lo : t_hi) + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false), term > 0 || ks > 0);
       }
     }
     umma_commit(elected, done0);
@@ -1186,7 +1237,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
         const float2 u1 = mul2(make_float2(f[2], f[3]), make_float2(up1, up1));
         hi[ks][2 * m] = pack_half(u0.x, u0.y);
         hi[ks][2 * m + 1] = pack_half(u1.x, u1.y);
-        const float2 kout = *reinterpret_cast<const float2*>(&st.f.k_out[16 * ks + 8 * m + 2 * t]);
+        const float2 kout = *reinterpret_cast<const float2*>(&st.pair.k_out[16 * ks + 8 * m + 2 * t]);
         const float2 k0 = mul2(u0, kout), k1 = mul2(u1, kout);
         f[0] = k0.x;
         f[1] = k0.y;
@@ -1204,7 +1255,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
     tmem_after();
     const uint32_t elected = elect_lane();
     const uint64_t k = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
-    const uint64_t pp = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.p), 0));
+    const uint64_t pp = tri_desc(__shfl_sync(0xffffffffu, smem_u32(st.pair.p), 0));
 #pragma unroll
     for (int term = 1; term >= 0; --term) {
 #pragma unroll
@@ -1216,13 +1267,13 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
     umma_commit(elected, done0);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, pp + ks * (2048 >> 4) + ks * 2, mma_shape(64 - 16 * ks, false),
+      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, pp + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false),
            ks > 0);
     }
     umma_commit(elected, done1);
   }
   // S <- decay S + dS, one fp32 fused multiply-add per element.
-  const float2 decay = make_float2(st.f.decay, st.f.decay);
+  const float2 decay = make_float2(st.pair.decay, st.pair.decay);
   const float2 w02 = make_float2(w0, w0), w12 = make_float2(w1, w1);
   wait_done(done0, x.phase, s, x.dead);
   x.phase ^= 1;
@@ -1234,25 +1285,100 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   }
 }
 
+// The next chunk's work, from the next item that has some if the last one is through.  One thread.
+__device__ __forceinline__ void next_work(const PrefillArgs& p, Cursor& at, Work& d) {
+  const int64_t per_block = p.block_size / kChunk;
+  int32_t source = -1;
+  while (at.chunk == at.chunks) {
+    const uint32_t item = at.ahead;
+    if (item >= static_cast<uint32_t>(p.n_requests) * p.num_v_heads) {
+      d.kind = kWorkEnd;
+      return;
+    }
+    at.ahead = atomicAdd(p.next, 1u);
+    const int r = p.order[item / p.num_v_heads];
+    at.head = static_cast<int>(item % p.num_v_heads);
+    at.chunk = at.chunks = 0;
+    Request rq;
+    unsigned int fault;
+    bool skip;
+    if (find_request(p, r, rq, fault, skip)) {
+      at.first = rq.first;
+      at.tokens = rq.tokens;
+      at.chunks = rq.chunks;
+      at.lead = rq.lead;
+      at.base = chunk_base(rq.first, r);
+      // Chunks end at absolute positions that are multiples of 64, and so do blocks.
+      at.left = per_block - (rq.context / kChunk) % per_block;
+      at.slot_at = rq.row + rq.context / p.block_size;
+      source = rq.source;
+    } else {
+      if (fault != 0 && at.head == 0) atomicOr(&g_prefill_faults, fault);
+      if (!skip) {
+        d.token0 = rq.first;
+        d.place = rq.tokens;
+        d.head = at.head;
+        d.kind = kWorkZero;
+        return;
+      }
+    }
+  }
+  const int64_t local0 = at.chunk * kChunk - at.lead;
+  d.token0 = at.first + local0;
+  d.place = at.base + at.chunk;
+  d.row_lo = at.chunk == 0 ? at.lead : 0;
+  d.row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), at.tokens - local0));
+  d.head = at.head;
+  d.source = source;
+  d.slot = 0;
+  d.kind = kWorkChunk;
+  ++at.chunk;
+  if (at.chunk == at.chunks || --at.left == 0) {  // a block or the request ends: its slot takes the state
+    d.slot = *at.slot_at++;
+    at.left = per_block;
+    if (d.slot >= p.n_slots) {
+      if (at.head == 0) atomicOr(&g_prefill_faults, LD_FAULT_DECODE_SLOT_RANGE);
+      d.slot = 0;
+    }
+  }
+}
+
+// Writes the zero outputs of upcoming items that cannot run, until a chunk or the end is next.  The moving
+// threads together.
+__device__ __forceinline__ void skip_items(const PrefillArgs& p, ChainSmem& s, int tid) {
+  while (s.upcoming.kind == kWorkZero) {
+    const int64_t first = s.upcoming.token0, values = s.upcoming.place * kDim;
+    for (int64_t i = tid; i < values; i += kMoveThreads) {
+      p.out[((first + i / kDim) * p.num_v_heads + s.upcoming.head) * kDim + i % kDim] = __float2bfloat16_rn(0.0f);
+    }
+    bar_move();
+    if (tid == 0) next_work(p, s.at, s.upcoming);
+    bar_move();
+  }
+}
+
+// Gives a free stage the upcoming work and starts its copies.  The moving threads together.
+template <typename StateT, bool kVec>
+__device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid) {
+  if (tid == 0) st.work = d;
+  if (d.kind == kWorkEnd) return;
+  if (d.source > 0 && tid < 32) {  // a new item's state: into L2 by the time that it is read
+    const char* state = reinterpret_cast<const char*>(static_cast<const StateT*>(p.state) + d.source * p.slot_stride +
+                                                      static_cast<int64_t>(d.head) * kDim * kDim);
+    constexpr int kBytes = kDim * kDim * sizeof(StateT) / 32;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(state + tid * kBytes), "n"(kBytes) : "memory");
+  }
+  copy_chunk<kVec>(p, st, d, full, tid);
+}
+
+// A persistent CTA per SM: the moving threads take items (a request's value head each), longest first, and
+// feed their chunks through two stages without a gap between items.
 template <typename StateT, bool kVec>
 __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(const PrefillArgs p) {
   extern __shared__ __align__(1024) unsigned char raw[];
   ChainSmem& s = *reinterpret_cast<ChainSmem*>(raw);
   grid_dependency_wait();
   allow_dependent_launch();
-  const int64_t r = blockIdx.x / p.num_v_heads;
-  const int head = static_cast<int>(blockIdx.x - r * p.num_v_heads);
-  Request rq;
-  unsigned int fault;
-  bool skip;
-  if (!find_request(p, r, rq, fault, skip)) {
-    if (fault != 0 && threadIdx.x == 0 && head == 0) atomicOr(&g_prefill_faults, fault);
-    if (skip) return;
-    for (int64_t i = threadIdx.x; i < rq.tokens * kDim; i += kChainThreads) {
-      p.out[((rq.first + i / kDim) * p.num_v_heads + head) * kDim + i % kDim] = __float2bfloat16_rn(0.0f);
-    }
-    return;
-  }
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kStateWarp = kMoveThreads / 32;
 
@@ -1260,15 +1386,41 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
   if (warp < kStateWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int tid = threadIdx.x;
-    const int64_t base = chunk_base(rq.first, r);
-    const auto hand_over = [&](int stage) {
+    const auto full = [&](int stage) { return smem_u32(&s.full[stage]); };
+    // A stage is handed over when its copies have landed: every thread waits for its own, warp 0 for the bulk
+    // copies.
+    uint32_t landed = 0;
+    bool late = false;
+    const auto hand_over = [&](int stage, bool chunk) {
       cp_async_wait();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the products read through the async proxy
+      if (warp == 0 && chunk) {
+        wait_done(full(stage), (landed >> stage) & 1, s, late);
+        landed ^= 1u << stage;
+      }
       bar_arrive(kBarFull + stage);
     };
-    for (int64_t c = 0; c < min(rq.chunks, static_cast<int64_t>(2)); ++c) {
-      copy_chunk<kVec>(p, s.stage[c], rq, c, base + c, head, tid);
-      hand_over(static_cast<int>(c));
+    if (tid == 0) {
+      for (int i = 0; i < 2; ++i) barrier_init(full(i));
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      s.at.ahead = atomicAdd(p.next, 1u);
+      s.at.chunk = s.at.chunks = 0;
+      next_work(p, s.at, s.upcoming);
+    }
+    __syncthreads();  // the barriers are there
+    skip_items(p, s, tid);
+    load_stage<StateT, kVec>(p, s.stage[0], s.upcoming, full(0), tid);
+    bool more = s.upcoming.kind == kWorkChunk;
+    if (more) {
+      bar_move();
+      if (tid == 0) next_work(p, s.at, s.upcoming);
+      bar_move();
+      skip_items(p, s, tid);
+      hand_over(0, true);
+      load_stage<StateT, kVec>(p, s.stage[1], s.upcoming, full(1), tid);
+      more = s.upcoming.kind == kWorkChunk;
+      hand_over(1, more);
+    } else {
+      hand_over(0, false);
     }
     float wt[8];
 #pragma unroll
@@ -1276,21 +1428,31 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     const int v0 = 32 * (warp & 3) + 16 * (warp >> 2);  // the TMEM lanes of a warp, as below
     uint32_t phase = 0;
     bool dead = false;
-    uint2 z[kOutSteps][2];
-    for (int64_t c = 0; c < rq.chunks; ++c) {
-      const int stage = static_cast<int>(c & 1);
-      load_gates<kVec>(p, rq, c, head, tid, z);
+    bar_move();
+    for (int stage = 0;; stage ^= 1) {
+      Stage& st = s.stage[stage];
+      const Work d = st.work;
+      if (d.kind == kWorkEnd) break;
+      uint2 z[kOutSteps][2];
+      load_gates<kVec>(p, d, tid, z);
+      const bool refill = more;
+      if (refill && tid == 0) next_work(p, s.at, s.upcoming);  // while the chain is at work
+      __syncwarp();
       bar_sync(kBarChunkDone);
       wait_done(smem_u32(&s.done[1]), phase, s, dead);
       phase ^= 1;
-      gather_outputs(s, s.stage[stage], v0, lane);
+      gather_outputs(s, st, v0, lane);
       tmem_before();
-      bar_move();  // the tile is whole, and the stage read for the last time
-      if (c + 1 < rq.chunks) bar_arrive(kBarTaken);
-      if (c + 2 < rq.chunks) copy_chunk<kVec>(p, s.stage[stage], rq, c + 2, base + c + 2, head, tid);
-      store_outputs<kVec>(p, s, rq, c, head, wt, tid, z);
-      if (c + 2 < rq.chunks) hand_over(stage);
-      bar_move();  // the tile is free again
+      bar_move();  // the tile is whole, the stage read for the last time, the upcoming work known
+      if (s.stage[stage ^ 1].work.kind == kWorkChunk) bar_arrive(kBarTaken);
+      if (refill) {
+        skip_items(p, s, tid);
+        load_stage<StateT, kVec>(p, st, s.upcoming, full(stage), tid);
+        more = s.upcoming.kind == kWorkChunk;
+      }
+      store_outputs<kVec>(p, s, d, wt, tid, z);
+      if (refill) hand_over(stage, more);
+      bar_move();  // the tile is free again, and the stage's work written
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
@@ -1305,63 +1467,54 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
       if (lane == 0) {
         s.stop = 0;
-        for (int i = 0; i < 2; ++i) {
-          asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&s.done[i])) : "memory");
-        }
+        for (int i = 0; i < 2; ++i) barrier_init(smem_u32(&s.done[i]));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       }
       __syncwarp();
       tmem_before();
     }
-    StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(head) * kDim * kDim + (v0 + g) * kDim + 2 * t;
+    __syncthreads();  // the barriers are there
+    tmem_after();
+    const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
     StateWarp x;
     x.phase = 0;
     x.dead = false;
-    if (rq.source > 0) {
-      const StateT* at = pool + rq.source * p.slot_stride;
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        load_pair(at + 8 * n, x.S[n][0], x.S[n][1]);
-        load_pair(at + 8 * kDim + 8 * n, x.S[n][2], x.S[n][3]);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x.S[n][e] = 0.0f;
-      }
-    }
-    bar_state();
-    tmem_after();
-    const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
-    // Chunks end at absolute positions that are multiples of 64, and so do blocks.
-    const int64_t per_block = p.block_size / kChunk;
-    const int32_t* slot_at = rq.row + rq.context / p.block_size;
-    int64_t left = per_block - (rq.context / kChunk) % per_block;
-    for (int64_t c = 0; c < rq.chunks; ++c) {
-      const int stage = static_cast<int>(c & 1);
+    for (int64_t n = 0;; ++n) {
+      const int stage = static_cast<int>(n & 1);
+      const Stage& st = s.stage[stage];
       bar_sync(kBarFull + stage);
-      chain_chunk(x, s, s.stage[stage], tmem, v0, lane, issuer, [&] {
-        if (c >= 1) {
+      if (st.work.kind == kWorkEnd) break;
+      wait_done(smem_u32(&s.full[stage]), static_cast<uint32_t>(n >> 1) & 1, s, x.dead);  // has landed
+      const int32_t source = st.work.source, slot = st.work.slot;
+      StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(st.work.head) * kDim * kDim +
+                     (v0 + g) * kDim + 2 * t;
+      if (source > 0) {
+        const StateT* at = pool + source * p.slot_stride;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          load_pair(at + 8 * i, x.S[i][0], x.S[i][1]);
+          load_pair(at + 8 * kDim + 8 * i, x.S[i][2], x.S[i][3]);
+        }
+      } else if (source == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.S[i][e] = 0.0f;
+        }
+      }
+      chain_chunk(x, s, st, tmem, v0, lane, issuer, [&] {
+        if (n >= 1) {
           bar_sync(kBarTaken);
           tmem_after();
         }
       });
       bar_arrive(kBarChunkDone);
-      if (c + 1 == rq.chunks || --left == 0) {  // a block or the request ends here: its slot takes the state
-        const int32_t slot = *slot_at++;
-        left = per_block;
-        if (slot > 0 && slot < p.n_slots) {
-          StateT* at = pool + slot * p.slot_stride;
-          if (!x.dead) {
+      if (slot > 0 && !x.dead && s.stop == 0) {
+        StateT* at = pool + slot * p.slot_stride;
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-              store_pair(at + 8 * n, x.S[n][0], x.S[n][1]);
-              store_pair(at + 8 * kDim + 8 * n, x.S[n][2], x.S[n][3]);
-            }
-          }
-        } else if (slot >= p.n_slots && head == 0 && lane == 0) {
-          atomicOr(&g_prefill_faults, LD_FAULT_DECODE_SLOT_RANGE);
+        for (int i = 0; i < 16; ++i) {
+          store_pair(at + 8 * i, x.S[i][0], x.S[i][1]);
+          store_pair(at + 8 * kDim + 8 * i, x.S[i][2], x.S[i][3]);
         }
       }
     }
@@ -1379,14 +1532,34 @@ bool aligned(const void* ptr, uintptr_t bytes) { return (reinterpret_cast<uintpt
 
 int64_t chunk_places(int64_t n_tokens, int64_t n_requests) { return chunk_base(n_tokens, n_requests); }
 
+// The workspace: key images, pair images, then the requests' order and the count of items taken.
+int64_t order_offset(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads) {
+  return chunk_places(n_tokens, n_requests) * (num_k_heads * static_cast<int64_t>(sizeof(KeyImage)) +
+                                               num_v_heads * static_cast<int64_t>(sizeof(PairImage)));
+}
+
 int64_t workspace_bytes(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads) {
-  const int64_t per_place = num_k_heads * static_cast<int64_t>(sizeof(KeyImage)) +
-                            num_v_heads * static_cast<int64_t>(sizeof(PairImage));
-  return chunk_places(n_tokens, n_requests) * per_place;
+  return order_offset(n_tokens, n_requests, num_k_heads, num_v_heads) + 4 * (n_requests + 1);
+}
+
+// Streaming multiprocessors of the current device, asked once per device.
+int sm_count(int& sms) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> known[kMaxDevices];
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess && device >= 0 && device < kMaxDevices) {
+    sms = known[device].load(std::memory_order_relaxed);
+    if (sms > 0) return LD_OK;
+  }
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (err != cudaSuccess) return set_error(LD_ERR_CUDA, "prefill: device query failed: %s", cudaGetErrorString(err));
+  if (device >= 0 && device < kMaxDevices) known[device].store(sms, std::memory_order_relaxed);
+  return LD_OK;
 }
 
 template <typename StateT, bool kVec>
-cudaError_t launch_prefill(const PrefillArgs& args, cudaStream_t stream) {
+cudaError_t launch_prefill(const PrefillArgs& args, int sms, cudaStream_t stream) {
   // Set on every call: the attributes belong to the current device, and setting them is a table write.
   auto pairs = gdn_prefill_pairs_kernel<kVec>;
   cudaError_t err = cudaFuncSetAttribute(pairs, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairSmem));
@@ -1394,11 +1567,11 @@ cudaError_t launch_prefill(const PrefillArgs& args, cudaStream_t stream) {
   auto chain = gdn_prefill_chain_kernel<StateT, kVec>;
   err = cudaFuncSetAttribute(chain, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ChainSmem));
   if (err != cudaSuccess) return err;
-  const int64_t places = chunk_places(args.n_tokens, args.n_requests);
-  err = launch(pairs, dim3(static_cast<unsigned int>(places * args.num_k_heads)), dim3(kPairThreads), sizeof(PairSmem),
-               stream, 1, args);
+  err = launch(pairs, dim3(static_cast<unsigned int>(1 + args.places * args.num_k_heads)), dim3(kPairThreads),
+               sizeof(PairSmem), stream, 1, args);
   if (err != cudaSuccess) return err;
-  return launch(chain, dim3(static_cast<unsigned int>(args.n_requests) * args.num_v_heads), dim3(kChainThreads),
+  const int64_t items = static_cast<int64_t>(args.n_requests) * args.num_v_heads;
+  return launch(chain, dim3(static_cast<unsigned int>(std::min<int64_t>(items, sms))), dim3(kChainThreads),
                 sizeof(ChainSmem), stream, 1, args);
 }
 
@@ -1507,6 +1680,10 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   args.block_size = block_size;
   args.keys = static_cast<KeyImage*>(workspace);
   args.pairs = reinterpret_cast<PairImage*>(args.keys + chunk_places(n_tokens, n_requests) * num_k_heads);
+  unsigned char* order = static_cast<unsigned char*>(workspace) + order_offset(n_tokens, n_requests, num_k_heads, num_v_heads);
+  args.next = reinterpret_cast<uint32_t*>(order);
+  args.order = reinterpret_cast<int32_t*>(order) + 1;
+  args.places = chunk_places(n_tokens, n_requests);
   args.n_requests = static_cast<int>(n_requests);
   args.num_k_heads = static_cast<int>(num_k_heads);
   args.num_v_heads = static_cast<int>(num_v_heads);
@@ -1518,12 +1695,15 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   // 16-byte copies of the q, k, v rows and 8-byte accesses to gate and out where every row allows them.
   const bool vec = aligned(qkv, 16) && qkv_row_stride % 8 == 0 && aligned(gate, 8) && gate_row_stride % 4 == 0 &&
                    aligned(out, 8);
+  int sms = 0;
+  const int rc = sm_count(sms);
+  if (rc != LD_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t err;
   if (bf16_pool) {
-    err = vec ? launch_prefill<__nv_bfloat16, true>(args, s) : launch_prefill<__nv_bfloat16, false>(args, s);
+    err = vec ? launch_prefill<__nv_bfloat16, true>(args, sms, s) : launch_prefill<__nv_bfloat16, false>(args, sms, s);
   } else {
-    err = vec ? launch_prefill<float, true>(args, s) : launch_prefill<float, false>(args, s);
+    err = vec ? launch_prefill<float, true>(args, sms, s) : launch_prefill<float, false>(args, sms, s);
   }
   if (err != cudaSuccess) return set_error(LD_ERR_CUDA, "prefill launch failed: %s", cudaGetErrorString(err));
   return ok();
