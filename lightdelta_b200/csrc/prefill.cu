@@ -1118,12 +1118,24 @@ struct StateWarp {
   bool dead;
 };
 
+// The products that the state waits for are done.  One warp asks the barrier, the others wait for it at a named
+// barrier: asking, eight warps took so many issue slots from the one that issues that a product of 32 cycles
+// (N = 64) was issued every 48.
+__device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool issuer) {
+  if (issuer) {
+    wait_done(smem_u32(&s.done[0]), x.phase, s, x.dead);
+    x.phase ^= 1;
+  }
+  bar_state();
+  tmem_after();
+}
+
 // One chunk.  `tmem` carries this warp's lanes; one warp (`issuer`) issues the products.  `taken` returns when
 // the outputs of the chunk before have left TMEM.
 //
-// Parity waits are sound because every thread that waits on a barrier has seen a phase before the next one
-// can begin: the state's warps join (bar_state) between a wait on done[0] and the next commit to it, and
-// done[1]'s next commit comes after `taken`, which the waiting threads release.
+// Parity waits are sound because the warp that waits on a barrier has seen a phase before the next one can begin:
+// done[0] has one warp that both commits and waits, and done[1]'s next commit comes after `taken`, which the
+// waiting threads release.
 template <typename Taken>
 __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const Stage& st, uint32_t tmem, int v0, int lane,
                                             bool issuer, Taken taken) {
@@ -1154,8 +1166,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   }
 
   // R = beta (v - k_in Y).
-  wait_done(done0, x.phase, s, x.dead);
-  x.phase ^= 1;
+  wait_products(x, s, issuer);
   float Y[8][4];
   tmem_load(tmem + kTmemY, Y);
   const uint32_t v_base =
@@ -1216,8 +1227,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   }
   // u, and k_out u in two terms.  k_out is at most 1 (the largest k~ of a row is in [1, 2)), so u's row
   // scale serves both.
-  wait_done(done0, x.phase, s, x.dead);
-  x.phase ^= 1;
+  wait_products(x, s, issuer);
   tmem_load(tmem + kTmemTr, Y);
   const float r_down0 = down0, r_down1 = down1;
   scale_rows(Y, up0, down0, up1, down1);
@@ -1275,8 +1285,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   // S <- decay S + dS, one fp32 fused multiply-add per element.
   const float2 decay = make_float2(st.pair.decay, st.pair.decay);
   const float2 w02 = make_float2(w0, w0), w12 = make_float2(w1, w1);
-  wait_done(done0, x.phase, s, x.dead);
-  x.phase ^= 1;
+  wait_products(x, s, issuer);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     tmem_load(tmem + kTmemDs + 64 * half, Y);
@@ -1439,8 +1448,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       if (refill && tid == 0) next_work(p, s.at, s.upcoming);  // while the chain is at work
       __syncwarp();
       bar_sync(kBarChunkDone);
-      wait_done(smem_u32(&s.done[1]), phase, s, dead);
-      phase ^= 1;
+      if (warp == 0) {
+        wait_done(smem_u32(&s.done[1]), phase, s, dead);
+        phase ^= 1;
+      }
+      bar_move();
+      tmem_after();
       gather_outputs(s, st, v0, lane);
       tmem_before();
       bar_move();  // the tile is whole, the stage read for the last time, the upcoming work known
@@ -1484,7 +1497,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       const Stage& st = s.stage[stage];
       bar_sync(kBarFull + stage);
       if (st.work.kind == kWorkEnd) break;
-      wait_done(smem_u32(&s.full[stage]), static_cast<uint32_t>(n >> 1) & 1, s, x.dead);  // has landed
       const int32_t source = st.work.source, slot = st.work.slot;
       StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(st.work.head) * kDim * kDim +
                      (v0 + g) * kDim + 2 * t;
@@ -1509,7 +1521,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         }
       });
       bar_arrive(kBarChunkDone);
-      if (slot > 0 && !x.dead && s.stop == 0) {
+      if (slot > 0 && s.stop == 0) {
         StateT* at = pool + slot * p.slot_stride;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
