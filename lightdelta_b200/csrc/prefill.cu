@@ -253,16 +253,16 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&r)[8][4]) {
       : "memory");
 }
 
-// 32 columns likewise.
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&r)[4][4]) {
+// 16 columns from each of two places.
+__device__ __forceinline__ void tmem_load(uint32_t x_at, uint32_t y_at, float (&x)[2][4], float (&y)[2][4]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(r[0][0]), "=f"(r[0][1]), "=f"(r[0][2]), "=f"(r[0][3]), "=f"(r[1][0]), "=f"(r[1][1]), "=f"(r[1][2]),
-        "=f"(r[1][3]), "=f"(r[2][0]), "=f"(r[2][1]), "=f"(r[2][2]), "=f"(r[2][3]), "=f"(r[3][0]), "=f"(r[3][1]),
-        "=f"(r[3][2]), "=f"(r[3][3])
-      : "r"(addr)
+      : "=&f"(x[0][0]), "=&f"(x[0][1]), "=&f"(x[0][2]), "=&f"(x[0][3]), "=&f"(x[1][0]), "=&f"(x[1][1]), "=&f"(x[1][2]),
+        "=&f"(x[1][3]), "=&f"(y[0][0]), "=&f"(y[0][1]), "=&f"(y[0][2]), "=&f"(y[0][3]), "=&f"(y[1][0]), "=&f"(y[1][1]),
+        "=&f"(y[1][2]), "=&f"(y[1][3])
+      : "r"(x_at), "r"(y_at)
       : "memory");
 }
 
@@ -279,6 +279,12 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&a)[4]
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   const int bytes = live ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All groups but the last `kLast`.
+template <int kLast>
+__device__ __forceinline__ void cp_async_wait_groups() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLast) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -406,7 +412,7 @@ __device__ __forceinline__ int low(int row, int col) { return low_block(row >> 4
 template <bool kVec, int kThreads, typename At>
 __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row_stride, int row_lo, int row_hi,
                                           uint16_t* tile, int tid, At at) {
-#pragma unroll
+#pragma unroll 2
   for (int pass = 0; pass < kChunk / (kThreads / 16); ++pass) {
     const int i = pass * (kThreads / 16) + (tid >> 4);
     const int col = (tid & 15) * 8;
@@ -755,7 +761,7 @@ __device__ __forceinline__ void order_requests(const PrefillArgs& p, int tid) {
 }
 
 template <bool kVec>
-__global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(const PrefillArgs p) {
+__global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(const __grid_constant__ PrefillArgs p) {
   extern __shared__ __align__(1024) unsigned char raw[];
   PairSmem& s = *reinterpret_cast<PairSmem*>(raw);
   grid_dependency_wait();
@@ -850,7 +856,7 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
 // ------------------------------------------------------------------------------------------
 // chain: the state through the chunks
 // ------------------------------------------------------------------------------------------
-constexpr int kVRow = kDim + 8;  // bf16 per row of a stage's v: the 16 bytes spread its rows over the banks
+constexpr int kVRow = kDim + 8;  // bf16 per row of a stage's v and gate: the 16 bytes spread their rows over the banks
 
 // What a stage holds: one chunk of one item.
 struct Work {
@@ -866,19 +872,18 @@ constexpr int kWorkChunk = 0, kWorkEnd = 1, kWorkZero = 2;  // a chunk; no more 
 
 // Where the item in work is, kept and used by one thread.
 struct Cursor {
-  int64_t first, tokens, chunks;  // of the item: its first token, its tokens and chunks
-  int64_t base;                   // place of its first chunk
-  int64_t chunk;                  // next chunk
-  int64_t left;                   // chunks to the end of the block that it is in
-  const int32_t* slot_at;
-  uint32_t ahead;                 // the item after this one, already taken
-  int32_t lead, head;
+  const int32_t* slot_at;  // the slot of the block that the next chunk is in
+  uint32_t ahead;          // the item after this one, already taken
+  int32_t rest;            // tokens behind the upcoming chunk
+  int32_t left;            // chunks to the end of the block, the upcoming one not counted
+  int32_t per_block;
 };
 
 struct __align__(1024) Stage {
   __half kq[2 * kChunk * kDim];
   PairImage pair;
   __align__(16) __nv_bfloat16 v[kChunk * kVRow];
+  __align__(16) __nv_bfloat16 gate[kChunk * kVRow];
   Work work;
 };
 
@@ -916,35 +921,36 @@ __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, cons
                                 [](int row, int col) { return row * kVRow + col; });
 }
 
-// The chunk's outputs S q + P u from TMEM to the output tile: this warp's 16 value rows.
+// The chunk's gate rows, which only the moving threads read, when the ones before have been used.
+template <bool kVec>
+__device__ __forceinline__ void copy_gates(const PrefillArgs& p, Stage& st, int tid) {
+  const Work& d = st.work;
+  if (d.kind == kWorkChunk) {
+    load_rows<kVec, kMoveThreads>(p.gate + d.token0 * p.gate_row + d.head * kDim, p.gate_row, d.row_lo, d.row_hi,
+                                  reinterpret_cast<uint16_t*>(st.gate), tid,
+                                  [](int row, int col) { return row * kVRow + col; });
+  }
+}
+
+// The chunk's outputs S q + P u from TMEM to the output tile: this warp's 16 value rows, 16 columns at a time.
 __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, int v0, int lane) {
   const int g = lane >> 2, t = lane & 3;
   const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
-  const float s0 = s.s_down[v0 + g], s1 = s.s_down[v0 + g + 8];
+  const float2 s0 = make_float2(s.s_down[v0 + g], s.s_down[v0 + g]);
+  const float2 s1 = make_float2(s.s_down[v0 + g + 8], s.s_down[v0 + g + 8]);
   const float2 u0 = make_float2(s.u_down[v0 + g], s.u_down[v0 + g]);
   const float2 u1 = make_float2(s.u_down[v0 + g + 8], s.u_down[v0 + g + 8]);
-  float o[8][4];
-  tmem_load(tmem + kTmemO, o);
+#pragma unroll 1
+  for (int nb = 0; nb < 4; ++nb) {
+    float o[2][4], pu[2][4];
+    tmem_load(tmem + kTmemO + 16 * nb, tmem + kTmemPu + 16 * nb, o, pu);
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const float2 qin = *reinterpret_cast<const float2*>(&st.pair.q_in[8 * n + 2 * t]);
-    const float2 x0 = mul2(make_float2(o[n][0], o[n][1]), mul2(qin, make_float2(s0, s0)));
-    const float2 x1 = mul2(make_float2(o[n][2], o[n][3]), mul2(qin, make_float2(s1, s1)));
-    o[n][0] = x0.x;
-    o[n][1] = x0.y;
-    o[n][2] = x1.x;
-    o[n][3] = x1.y;
-  }
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float pu[4][4];
-    tmem_load(tmem + kTmemPu + 32 * half, pu);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int n = 4 * half + m;
-      const float2 x0 = fma2(make_float2(pu[m][0], pu[m][1]), u0, make_float2(o[n][0], o[n][1]));
-      const float2 x1 = fma2(make_float2(pu[m][2], pu[m][3]), u1, make_float2(o[n][2], o[n][3]));
-      float* at = s.o + (8 * n + 2 * t) * kORow + v0 + g;
+    for (int m = 0; m < 2; ++m) {
+      const int col = 16 * nb + 8 * m + 2 * t;
+      const float2 qin = *reinterpret_cast<const float2*>(&st.pair.q_in[col]);
+      const float2 x0 = fma2(make_float2(o[m][0], o[m][1]), mul2(qin, s0), mul2(make_float2(pu[m][0], pu[m][1]), u0));
+      const float2 x1 = fma2(make_float2(o[m][2], o[m][3]), mul2(qin, s1), mul2(make_float2(pu[m][2], pu[m][3]), u1));
+      float* at = s.o + col * kORow + v0 + g;
       at[0] = x0.x;
       at[kORow] = x0.y;
       at[8] = x1.x;
@@ -953,41 +959,17 @@ __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, in
   }
 }
 
-// Gated RMSNorm of the output tile.  A warp takes two rows at a time, 16 lanes and twice four values per lane
-// each.  `load_gates` starts the gate rows' loads early, `store_outputs` uses them.
-constexpr int kOutRows = kMoveThreads / 16, kOutSteps = kChunk / kOutRows;
-
+// Gated RMSNorm of the output tile.  A warp takes two rows at a time, 16 lanes and twice four values per lane each.
+// The loop stays rolled: the chain's warps run through so much straight code that the instruction cache is what
+// they compete for.
 template <bool kVec>
-__device__ __forceinline__ void load_gates(const PrefillArgs& p, const Work& d, int tid, uint2 (&z)[kOutSteps][2]) {
-  const __nv_bfloat16* gate = p.gate + d.token0 * p.gate_row + d.head * kDim + 4 * (tid & 15);
-#pragma unroll
-  for (int n = 0; n < kOutSteps; ++n) {
-    const int i = kOutRows * n + (tid >> 4);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      z[n][half] = make_uint2(0, 0);
-      if (i >= d.row_lo && i < d.row_hi) {
-        const __nv_bfloat16* at = gate + i * p.gate_row + 64 * half;
-        if constexpr (kVec) {
-          z[n][half] = *reinterpret_cast<const uint2*>(at);
-        } else {
-          z[n][half].x = __bfloat16_as_ushort(at[0]) | (static_cast<uint32_t>(__bfloat16_as_ushort(at[1])) << 16);
-          z[n][half].y = __bfloat16_as_ushort(at[2]) | (static_cast<uint32_t>(__bfloat16_as_ushort(at[3])) << 16);
-        }
-      }
-    }
-  }
-}
-
-template <bool kVec>
-__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Work& d,
-                                              const float (&wt)[8], int tid, const uint2 (&z)[kOutSteps][2]) {
+__device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Stage& st, const Work& d,
+                                              const float (&wt)[8], int tid) {
   const int part = tid & 15;
   const bool stop = s.stop != 0;
   __nv_bfloat16* out = p.out + (d.token0 * p.num_v_heads + d.head) * kDim + 4 * part;
-#pragma unroll
-  for (int n = 0; n < kOutSteps; ++n) {
-    const int i = kOutRows * n + (tid >> 4);
+#pragma unroll 1
+  for (int i = tid >> 4; i < kChunk; i += kMoveThreads / 16) {
     float4 o[2];
     float sq = 0.0f;
 #pragma unroll
@@ -1005,11 +987,11 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
     __nv_bfloat16* row = out + static_cast<int64_t>(i) * p.num_v_heads * kDim;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const uint2 zz = z[n][half];
-      const float y0 = o[half].x * rstd * (wt[4 * half + 0] * silu_fast(bf16_low(zz.x)));
-      const float y1 = o[half].y * rstd * (wt[4 * half + 1] * silu_fast(bf16_high(zz.x)));
-      const float y2 = o[half].z * rstd * (wt[4 * half + 2] * silu_fast(bf16_low(zz.y)));
-      const float y3 = o[half].w * rstd * (wt[4 * half + 3] * silu_fast(bf16_high(zz.y)));
+      const uint2 z = *reinterpret_cast<const uint2*>(&st.gate[i * kVRow + 64 * half + 4 * part]);
+      const float y0 = o[half].x * rstd * (wt[4 * half + 0] * silu_fast(bf16_low(z.x)));
+      const float y1 = o[half].y * rstd * (wt[4 * half + 1] * silu_fast(bf16_high(z.x)));
+      const float y2 = o[half].z * rstd * (wt[4 * half + 2] * silu_fast(bf16_low(z.y)));
+      const float y3 = o[half].w * rstd * (wt[4 * half + 3] * silu_fast(bf16_high(z.y)));
       const uint32_t lo = pack_bf16(y0, y1), hi = pack_bf16(y2, y3);
       __nv_bfloat16* at = row + 64 * half;
       if (live) {
@@ -1118,6 +1100,65 @@ struct StateWarp {
   bool dead;
 };
 
+// The products of one chunk, issued by one warp.  Everything here is a constant (the stage is a template argument
+// and shared memory starts at a known address), so operands are immediates: with descriptors from registers a
+// product of 32 cycles (N = 64) was issued every 46, in a rolled loop every 90.
+extern __shared__ __align__(1024) unsigned char chain_raw[];
+
+template <int kStage>
+struct Products {
+  static __device__ __forceinline__ const Stage& stage() { return reinterpret_cast<ChainSmem*>(chain_raw)->stage[kStage]; }
+  static __device__ __forceinline__ uint32_t done(int i) { return smem_u32(&reinterpret_cast<ChainSmem*>(chain_raw)->done[i]); }
+
+  // Y = S k~, two terms.
+  static __device__ __forceinline__ void state_keys(uint32_t elected) {
+    const uint64_t k = tile_desc(smem_u32(stage().kq));
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {  // k-steps of lo, then of hi
+      const uint32_t ks = i & 7;
+      umma(elected, kTmemY, kTmemS + 64 - 8 * (i & 8) + 8 * ks, k + ((ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2),
+           mma_shape(64, false), i > 0);
+    }
+    umma_commit(elected, done(0));
+  }
+
+  // U = T R (the product of the two lo terms is below fp32's last bit), then O = S q~ (hi term), which nobody waits
+  // for yet.  T's column block ks starts at row block ks.
+  static __device__ __forceinline__ void corrections(uint32_t elected) {
+    const uint64_t t_hi = tri_desc(smem_u32(stage().pair.t_hi)), t_lo = tri_desc(smem_u32(stage().pair.t_lo));
+#pragma unroll
+    for (uint32_t ks = 0; ks < 4; ++ks) {  // small terms first in each column block
+      const uint32_t at = 2 * tri_block(ks, ks) >> 4, shape = mma_shape(64 - 16 * ks, false);
+      umma(elected, kTmemTr + 16 * ks, kTmemR + 8 * ks, t_lo + at, shape, ks > 0);
+      umma(elected, kTmemTr + 16 * ks, kTmemR + 32 + 8 * ks, t_hi + at, shape, true);
+      umma(elected, kTmemTr + 16 * ks, kTmemR + 8 * ks, t_hi + at, shape, true);
+    }
+    umma_commit(elected, done(0));
+    const uint64_t q = tile_desc(smem_u32(stage().kq + kHalf));
+#pragma unroll
+    for (uint32_t ks = 0; ks < 8; ++ks) {
+      umma(elected, kTmemO, kTmemS + 8 * ks, q + ((ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2), mma_shape(64, false),
+           ks > 0);
+    }
+  }
+
+  // dS = (k_out u) k~, two terms, then P u, which completes the outputs.
+  static __device__ __forceinline__ void update(uint32_t elected) {
+    const uint64_t k = tile_desc(smem_u32(stage().kq)), p = tri_desc(smem_u32(stage().pair.p));
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {  // k-steps of lo, then of hi
+      umma(elected, kTmemDs, kTmemW + 32 - 8 * (i & 4) + 8 * (i & 3), k + (i & 3) * (2048 >> 4), mma_shape(128, true), i > 0);
+    }
+    umma_commit(elected, done(0));
+#pragma unroll
+    for (uint32_t ks = 0; ks < 4; ++ks) {
+      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, p + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false),
+           ks > 0);
+    }
+    umma_commit(elected, done(1));
+  }
+};
+
 // The products that the state waits for are done.  One warp asks the barrier, the others wait for it at a named
 // barrier: asking, eight warps took so many issue slots from the one that issues that a product of 32 cycles
 // (N = 64) was issued every 48.
@@ -1137,10 +1178,10 @@ __device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool i
 // done[0] has one warp that both commits and waits, and done[1]'s next commit comes after `taken`, which the
 // waiting threads release.
 template <typename Taken>
-__device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const Stage& st, uint32_t tmem, int v0, int lane,
+__device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stage, uint32_t tmem, int v0, int lane,
                                             bool issuer, Taken taken) {
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t done0 = smem_u32(&s.done[0]), done1 = smem_u32(&s.done[1]);
+  const Stage& st = s.stage[stage];
 
   // Y = S k~ (two terms).
   float up0, down0, up1, down1;
@@ -1153,16 +1194,11 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   if (issuer && !x.dead) {
     tmem_after();
     const uint32_t elected = elect_lane();
-    const uint64_t k = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
-#pragma unroll
-    for (int term = 1; term >= 0; --term) {
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        umma(elected, kTmemY, kTmemS + 64 * term + 8 * ks, k + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2,
-             mma_shape(64, false), term == 0 || ks > 0);
-      }
+    if (stage == 0) {
+      Products<0>::state_keys(elected);
+    } else {
+      Products<1>::state_keys(elected);
     }
-    umma_commit(elected, done0);
   }
 
   // R = beta (v - k_in Y).
@@ -1207,24 +1243,13 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   if (issuer && !x.dead) {
     tmem_after();
     const uint32_t elected = elect_lane();
-    const uint64_t t_hi = tri_desc(__shfl_sync(0xffffffffu, smem_u32(st.pair.t_hi), 0));
-    const uint64_t t_lo = t_hi + (sizeof(st.pair.t_hi) >> 4);
-#pragma unroll
-    for (int term = 0; term < 3; ++term) {  // hi lo, lo hi, hi hi
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        umma(elected, kTmemTr + 16 * ks, kTmemR + (term == 1 ? 32 : 0) + 8 * ks,
-             (term == 0 ? t_lo : t_hi) + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false), term > 0 || ks > 0);
-      }
-    }
-    umma_commit(elected, done0);
-    // O = S q~ (hi term), while the others go on.
-    const uint64_t q = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq + kHalf), 0));
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      umma(elected, kTmemO, kTmemS + 8 * ks, q + (ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2, mma_shape(64, false), ks > 0);
+    if (stage == 0) {
+      Products<0>::corrections(elected);
+    } else {
+      Products<1>::corrections(elected);
     }
   }
+
   // u, and k_out u in two terms.  k_out is at most 1 (the largest k~ of a row is in [1, 2)), so u's row
   // scale serves both.
   wait_products(x, s, issuer);
@@ -1264,23 +1289,11 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   if (issuer && !x.dead) {
     tmem_after();
     const uint32_t elected = elect_lane();
-    const uint64_t k = tile_desc(__shfl_sync(0xffffffffu, smem_u32(st.kq), 0));
-    const uint64_t pp = tri_desc(__shfl_sync(0xffffffffu, smem_u32(st.pair.p), 0));
-#pragma unroll
-    for (int term = 1; term >= 0; --term) {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        umma(elected, kTmemDs, kTmemW + 32 * term + 8 * ks, k + ks * (2048 >> 4), mma_shape(128, true),
-             term == 0 || ks > 0);
-      }
+    if (stage == 0) {
+      Products<0>::update(elected);
+    } else {
+      Products<1>::update(elected);
     }
-    umma_commit(elected, done0);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, pp + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false),
-           ks > 0);
-    }
-    umma_commit(elected, done1);
   }
   // S <- decay S + dS, one fp32 fused multiply-add per element.
   const float2 decay = make_float2(st.pair.decay, st.pair.decay);
@@ -1294,11 +1307,24 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, const St
   }
 }
 
-// The next chunk's work, from the next item that has some if the last one is through.  One thread.
-__device__ __forceinline__ void next_work(const PrefillArgs& p, Cursor& at, Work& d) {
+// The slot that takes the state after the upcoming chunk, when a block or the request ends with it.
+__device__ __forceinline__ void work_slot(const PrefillArgs& p, Cursor& at, Work& d) {
+  d.slot = 0;
+  if (at.rest <= 0 || at.left == 0) {
+    d.slot = *at.slot_at++;
+    at.left = at.per_block;
+    if (d.slot >= p.n_slots) {
+      if (d.head == 0) atomicOr(&g_prefill_faults, LD_FAULT_DECODE_SLOT_RANGE);
+      d.slot = 0;
+    }
+  }
+  --at.left;
+}
+
+// The first chunk of the next item that has some, the end, or an item whose outputs are zeros.  One thread.
+__device__ __noinline__ void next_item(const PrefillArgs& p, Cursor& at, Work& d) {
   const int64_t per_block = p.block_size / kChunk;
-  int32_t source = -1;
-  while (at.chunk == at.chunks) {
+  while (true) {
     const uint32_t item = at.ahead;
     if (item >= static_cast<uint32_t>(p.n_requests) * p.num_v_heads) {
       d.kind = kWorkEnd;
@@ -1306,62 +1332,66 @@ __device__ __forceinline__ void next_work(const PrefillArgs& p, Cursor& at, Work
     }
     at.ahead = atomicAdd(p.next, 1u);
     const int r = p.order[item / p.num_v_heads];
-    at.head = static_cast<int>(item % p.num_v_heads);
-    at.chunk = at.chunks = 0;
+    d.head = static_cast<int>(item % p.num_v_heads);
+    at.rest = 0;
     Request rq;
     unsigned int fault;
     bool skip;
     if (find_request(p, r, rq, fault, skip)) {
-      at.first = rq.first;
-      at.tokens = rq.tokens;
-      at.chunks = rq.chunks;
-      at.lead = rq.lead;
-      at.base = chunk_base(rq.first, r);
       // Chunks end at absolute positions that are multiples of 64, and so do blocks.
-      at.left = per_block - (rq.context / kChunk) % per_block;
+      at.per_block = static_cast<int32_t>(min(per_block, static_cast<int64_t>(INT32_MAX)));
+      at.left = static_cast<int32_t>(min(per_block - 1 - (rq.context / kChunk) % per_block, static_cast<int64_t>(INT32_MAX)));
       at.slot_at = rq.row + rq.context / p.block_size;
-      source = rq.source;
-    } else {
-      if (fault != 0 && at.head == 0) atomicOr(&g_prefill_faults, fault);
-      if (!skip) {
-        d.token0 = rq.first;
-        d.place = rq.tokens;
-        d.head = at.head;
-        d.kind = kWorkZero;
-        return;
-      }
+      at.rest = static_cast<int32_t>(rq.tokens) - (kChunk - rq.lead);
+      d.token0 = rq.first - rq.lead;
+      d.place = chunk_base(rq.first, r);
+      d.row_lo = rq.lead;
+      d.row_hi = kChunk + min(at.rest, 0);
+      d.source = rq.source;
+      d.kind = kWorkChunk;
+      work_slot(p, at, d);
+      return;
     }
-  }
-  const int64_t local0 = at.chunk * kChunk - at.lead;
-  d.token0 = at.first + local0;
-  d.place = at.base + at.chunk;
-  d.row_lo = at.chunk == 0 ? at.lead : 0;
-  d.row_hi = static_cast<int>(min(static_cast<int64_t>(kChunk), at.tokens - local0));
-  d.head = at.head;
-  d.source = source;
-  d.slot = 0;
-  d.kind = kWorkChunk;
-  ++at.chunk;
-  if (at.chunk == at.chunks || --at.left == 0) {  // a block or the request ends: its slot takes the state
-    d.slot = *at.slot_at++;
-    at.left = per_block;
-    if (d.slot >= p.n_slots) {
-      if (at.head == 0) atomicOr(&g_prefill_faults, LD_FAULT_DECODE_SLOT_RANGE);
-      d.slot = 0;
+    if (fault != 0 && d.head == 0) atomicOr(&g_prefill_faults, fault);
+    if (!skip) {
+      d.token0 = rq.first;
+      d.place = rq.tokens;
+      d.kind = kWorkZero;
+      return;
     }
   }
 }
 
+// The upcoming work after the one in `d`.  One thread.
+__device__ __forceinline__ void next_work(const PrefillArgs& p, Cursor& at, Work& d) {
+  if (at.rest <= 0) {
+    next_item(p, at, d);
+    return;
+  }
+  d.token0 += kChunk;
+  d.place += 1;
+  d.row_lo = 0;
+  d.row_hi = min(at.rest, kChunk);
+  d.source = -1;
+  at.rest -= kChunk;
+  work_slot(p, at, d);
+}
+
 // Writes the zero outputs of upcoming items that cannot run, until a chunk or the end is next.  The moving
 // threads together.
+__device__ __noinline__ void zero_item(const PrefillArgs& p, const Work& d, int tid) {
+  // `place` rows of 256 bytes, one warp a row.
+  for (int64_t i = tid >> 5; i < d.place; i += kMoveThreads / 32) {
+    __nv_bfloat16* row = p.out + ((d.token0 + i) * p.num_v_heads + d.head) * kDim;
+    for (int c = tid & 31; c < kDim; c += 32) row[c] = __float2bfloat16_rn(0.0f);
+  }
+}
+
 __device__ __forceinline__ void skip_items(const PrefillArgs& p, ChainSmem& s, int tid) {
   while (s.upcoming.kind == kWorkZero) {
-    const int64_t first = s.upcoming.token0, values = s.upcoming.place * kDim;
-    for (int64_t i = tid; i < values; i += kMoveThreads) {
-      p.out[((first + i / kDim) * p.num_v_heads + s.upcoming.head) * kDim + i % kDim] = __float2bfloat16_rn(0.0f);
-    }
+    zero_item(p, s.upcoming, tid);
     bar_move();
-    if (tid == 0) next_work(p, s.at, s.upcoming);
+    if (tid == 0) next_item(p, s.at, s.upcoming);
     bar_move();
   }
 }
@@ -1383,9 +1413,8 @@ __device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, cons
 // A persistent CTA per SM: the moving threads take items (a request's value head each), longest first, and
 // feed their chunks through two stages without a gap between items.
 template <typename StateT, bool kVec>
-__global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(const PrefillArgs p) {
-  extern __shared__ __align__(1024) unsigned char raw[];
-  ChainSmem& s = *reinterpret_cast<ChainSmem*>(raw);
+__global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(const __grid_constant__ PrefillArgs p) {
+  ChainSmem& s = *reinterpret_cast<ChainSmem*>(chain_raw);
   grid_dependency_wait();
   allow_dependent_launch();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -1401,7 +1430,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     uint32_t landed = 0;
     bool late = false;
     const auto hand_over = [&](int stage, bool chunk) {
-      cp_async_wait();
+      cp_async_wait_groups<1>();  // but not for the gates, which were asked for last
       if (warp == 0 && chunk) {
         wait_done(full(stage), (landed >> stage) & 1, s, late);
         landed ^= 1u << stage;
@@ -1412,24 +1441,24 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       for (int i = 0; i < 2; ++i) barrier_init(full(i));
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       s.at.ahead = atomicAdd(p.next, 1u);
-      s.at.chunk = s.at.chunks = 0;
-      next_work(p, s.at, s.upcoming);
+      s.at.rest = 0;
+      next_item(p, s.at, s.upcoming);
     }
     __syncthreads();  // the barriers are there
-    skip_items(p, s, tid);
-    load_stage<StateT, kVec>(p, s.stage[0], s.upcoming, full(0), tid);
-    bool more = s.upcoming.kind == kWorkChunk;
-    if (more) {
-      bar_move();
-      if (tid == 0) next_work(p, s.at, s.upcoming);
-      bar_move();
+    bool more = true;
+#pragma unroll 1
+    for (int stage = 0; stage < 2 && more; ++stage) {
       skip_items(p, s, tid);
-      hand_over(0, true);
-      load_stage<StateT, kVec>(p, s.stage[1], s.upcoming, full(1), tid);
+      load_stage<StateT, kVec>(p, s.stage[stage], s.upcoming, full(stage), tid);
+      cp_async_commit();
       more = s.upcoming.kind == kWorkChunk;
-      hand_over(1, more);
-    } else {
-      hand_over(0, false);
+      bar_move();
+      copy_gates<kVec>(p, s.stage[stage], tid);
+      cp_async_commit();
+      if (stage == 0 && more && tid == 0) next_work(p, s.at, s.upcoming);
+      __syncwarp();
+      hand_over(stage, more);
+      bar_move();
     }
     float wt[8];
 #pragma unroll
@@ -1437,13 +1466,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     const int v0 = 32 * (warp & 3) + 16 * (warp >> 2);  // the TMEM lanes of a warp, as below
     uint32_t phase = 0;
     bool dead = false;
-    bar_move();
     for (int stage = 0;; stage ^= 1) {
       Stage& st = s.stage[stage];
       const Work d = st.work;
       if (d.kind == kWorkEnd) break;
-      uint2 z[kOutSteps][2];
-      load_gates<kVec>(p, d, tid, z);
       const bool refill = more;
       if (refill && tid == 0) next_work(p, s.at, s.upcoming);  // while the chain is at work
       __syncwarp();
@@ -1456,6 +1482,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       tmem_after();
       gather_outputs(s, st, v0, lane);
       tmem_before();
+      cp_async_wait();  // the gates
       bar_move();  // the tile is whole, the stage read for the last time, the upcoming work known
       if (s.stage[stage ^ 1].work.kind == kWorkChunk) bar_arrive(kBarTaken);
       if (refill) {
@@ -1463,9 +1490,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         load_stage<StateT, kVec>(p, st, s.upcoming, full(stage), tid);
         more = s.upcoming.kind == kWorkChunk;
       }
-      store_outputs<kVec>(p, s, d, wt, tid, z);
-      if (refill) hand_over(stage, more);
-      bar_move();  // the tile is free again, and the stage's work written
+      cp_async_commit();
+      store_outputs<kVec>(p, s, st, d, wt, tid);
+      bar_move();  // the tile and the stage's gates are free again, and its work written
+      if (refill) {
+        copy_gates<kVec>(p, st, tid);
+        cp_async_commit();
+        hand_over(stage, more);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
@@ -1514,7 +1546,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
           for (int e = 0; e < 4; ++e) x.S[i][e] = 0.0f;
         }
       }
-      chain_chunk(x, s, st, tmem, v0, lane, issuer, [&] {
+      chain_chunk(x, s, stage, tmem, v0, lane, issuer, [&] {
         if (n >= 1) {
           bar_sync(kBarTaken);
           tmem_after();
@@ -1704,8 +1736,8 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   args.weight_bf16 = weight_dtype == LD_DTYPE_BF16;
   args.q_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(kDim)));
   args.eps = eps;
-  // 16-byte copies of the q, k, v rows and 8-byte accesses to gate and out where every row allows them.
-  const bool vec = aligned(qkv, 16) && qkv_row_stride % 8 == 0 && aligned(gate, 8) && gate_row_stride % 4 == 0 &&
+  // 16-byte copies of the q, k, v and gate rows and 8-byte stores to out where every row allows them.
+  const bool vec = aligned(qkv, 16) && qkv_row_stride % 8 == 0 && aligned(gate, 16) && gate_row_stride % 8 == 0 &&
                    aligned(out, 8);
   int sms = 0;
   const int rc = sm_count(sms);
