@@ -136,7 +136,7 @@ def build_torch_path(reference: Path = DEFAULT_REFERENCE, force: bool = False) -
 def build_if_available() -> Path | None:
     """Builds oracle/_ref/_C.so (and the harness and the torch path's bytecode) when the reference
     sources are present (this container); on the GPU box the prebuilt files are used as shipped."""
-    if not DEFAULT_REFERENCE.exists():
+    if not (DEFAULT_REFERENCE / "csrc" / "gdn_decode.cu").exists():
         return OUT if OUT.exists() else None
     build_harness(DEFAULT_REFERENCE)
     build_torch_path(DEFAULT_REFERENCE)
