@@ -242,8 +242,8 @@ int ld_decode_kernel_override(int variant);
  * or output of the item whose wait ran out or of any later item, waits (bounded) for the copies it
  * issued and returns.  extra_tx_bytes > 0 (at most 1024) makes every state load announce that many
  * bytes more than it copies, so the waits for it run out although every copy lands: a launch then
- * changes no pool slot and no output of a request it runs.  Settings apply to launches made after
- * the call.  Returns LD_OK, or LD_ERR_INVALID for arguments out of range.
+ * changes no pool slot and no output of a request it runs.  ld_prefill's waits and copies take both
+ * settings too, with the same effect.  Settings apply to launches made after the call.  Returns LD_OK, or LD_ERR_INVALID for arguments out of range.
  */
 int ld_decode_wait_test(int64_t limit_ns, int32_t extra_tx_bytes);
 

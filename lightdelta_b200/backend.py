@@ -19,6 +19,10 @@ project's parity oracle and is not offered as a product path.  The config may be
 
 A bf16 pool (an extension; the reference's pool is fp32) runs in indexed mode through
 ``lightdelta::decode_bf16_state``.  Packed mode keeps the reference's fp32-only state copies.
+
+``prefill`` (an extension; the reference leaves prompts to its host engine's kernel) runs whole prompts, or pieces of
+them, on the pool through a block table; it reads and writes the pool in place, so it needs
+``state_io = "indexed"``.
 """
 
 from __future__ import annotations
@@ -43,6 +47,15 @@ class GDNBackend:
         self.config = config
         self.calls = Counter()
         self._packed: dict = {}
+
+    def prefill(self, qkv, a, b, a_log, dt_bias, table, context, cu, pool, gate, weight, out, block_size, eps=1e-6):
+        """Prompts through ``lightdelta::prefill``: request r brings tokens cu[r]..cu[r+1] behind context[r] held ones and
+        finds its states in the slots of its table row, one per ``block_size`` positions."""
+        if self.config.state_io != "indexed":
+            raise ValueError("prefill works on the pool in place: use state_io='indexed'")
+        self.calls["prefill"] += 1
+        torch.ops.lightdelta.prefill(qkv, a, b, a_log, dt_bias, table, context, cu, pool, gate, weight, out, block_size,
+                                     eps)
 
     def __call__(self, qkv, a, b, a_log, dt_bias, slots, cu, accepted, pool, gate, weight, out, eps=1e-6):
         batch, width = slots.shape

@@ -1587,6 +1587,9 @@ extern "C" int ld_decode_kernel_override(int variant) {
 
 namespace ldb {
 
+uint64_t wait_limit_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
+uint32_t wait_test_extra_bytes() { return g_extra_tx.load(std::memory_order_relaxed); }
+
 int check_decode_args(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a_row_stride, const void* b,
                       int64_t b_row_stride, const float* a_log, const void* dt_bias, int dt_bias_dtype,
                       const int32_t* indices, int64_t n_requests, int64_t width, const int32_t* cu,

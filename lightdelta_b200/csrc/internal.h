@@ -18,6 +18,11 @@ int check_decode_args(const void* qkv, int64_t qkv_row_stride, const void* a, in
                       int64_t gate_row_stride, const void* weight, int weight_dtype, void* out, int64_t n_tokens,
                       int64_t num_k_heads, int64_t num_v_heads, float eps);
 
+// What ld_decode_wait_test has set: the bound of in-kernel waits in nanoseconds, and the bytes that loads announce
+// beyond what they copy (0 outside tests).
+uint64_t wait_limit_ns();
+uint32_t wait_test_extra_bytes();
+
 // Whether kernels launch with programmatic dependent launch (ld_programmatic_launch).
 bool programmatic_launch_enabled();
 

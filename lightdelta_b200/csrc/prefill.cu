@@ -60,7 +60,6 @@ constexpr int kPairThreads = 128;
 constexpr int kMoveThreads = 256;   // chain kernel: warps 0-7 copy chunks in and store outputs,
 constexpr int kStateThreads = 256;  // warps 8-15 carry the state
 constexpr int kChainThreads = kMoveThreads + kStateThreads;
-constexpr uint64_t kWaitNs = 1000000000;  // bound of every in-kernel wait
 constexpr int kORow = kDim + 4;  // floats per row of the output tile: the +4 spreads its rows over the banks
 static_assert(kChunk == 64, "fragment loops below are written for chunks of 64 tokens");
 
@@ -83,8 +82,10 @@ struct __align__(128) PairImage {  // per (chunk, value head)
   float beta[kChunk];
   float k_in[kChunk];   // e^{G_i} fk_i: scales S k~
   float q_in[kChunk];   // e^{G_i} fq_i 128^-1/2: scales S q~
-  float k_out[kChunk];  // e^{G_C - G_j} fk_j: scales u_j on its way into the state
+  float k_out[kChunk];  // e^{G_C - G_j} fk_j / k_scale: scales u_j on its way into the state
   float decay;          // e^{G_C}
+  float k_scale;        // the power of two that brings the largest of k_out to [1, 2)
+  float p_scale;        // the powers of two that P was divided by, for the chunk's largest fk and fq
 };
 static_assert(sizeof(KeyImage) % 16 == 0 && sizeof(PairImage) % 16 == 0, "images are copied 16 bytes at a time");
 
@@ -124,6 +125,8 @@ struct PrefillArgs {
   int weight_bf16;
   float q_scale;
   float eps;
+  uint64_t wait_ns;   // bound of every in-kernel wait (ld_decode_wait_test)
+  uint32_t extra_tx;  // test only: bytes that a chunk's copies announce beyond what they copy (normally 0)
 };
 
 // Chunk c of request r is kept at place chunk_base(cu[r], r) + c.  A request of n tokens has at most
@@ -397,6 +400,8 @@ struct PairSmem {
   __align__(1024) unsigned char tiles[sizeof(KeyImage)];  // the key image, then, its products in registers, PairWork
   float g_hi[kGroup][kChunk], g_lo[kGroup][kChunk], beta[kGroup][kChunk];
   float fk[kChunk], fq[kChunk];
+  float fk_unit[kChunk], fq_unit[kChunk];  // divided by their largest's power of two
+  float fk_power, fq_power;
 
   __device__ __forceinline__ __half* kq() { return reinterpret_cast<__half*>(tiles); }
   __device__ __forceinline__ PairWork& work() { return *reinterpret_cast<PairWork*>(tiles); }
@@ -454,6 +459,17 @@ __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
     *at = make_uint4(y[0], y[1], y[2], y[3]);
   }
   return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
+// The power of two at or below the largest of 64 positive floats, of which each lane of a warp has two.  Operands that
+// become fp16 are divided by it, so that keys or queries of any size (the L2 norm's 1e-6 lets short ones stay short)
+// have the same bits there.
+__device__ __forceinline__ float largest_power(float x, float y) {
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(__float_as_uint(x), __float_as_uint(y)));
+  return __uint_as_float(min(max(top >> 23, 1u), 253u) << 23);
+}
+__device__ __forceinline__ float inverse_power(float power) {
+  return __uint_as_float(0x7f000000u - __float_as_uint(power));  // 2^(254 - e - 127)
 }
 
 // g and beta of the chunk's tokens for one value head and G's running sums (in powers of two), by one
@@ -569,8 +585,8 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
     const int i = 16 * w + g + 8 * half;
     g_hi[half] = s.g_hi[place][i];
     g_lo[half] = s.g_lo[place][i];
-    row_k[half] = s.beta[place][i] * s.fk[i];
-    row_q[half] = p.q_scale * s.fq[i];
+    row_k[half] = s.beta[place][i] * s.fk[i] * s.fk_power;
+    row_q[half] = p.q_scale * s.fq_unit[i];
   }
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
@@ -580,7 +596,7 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
       const int j = 16 * nb + 8 * m + 2 * t;
       const float2 hj = *reinterpret_cast<const float2*>(&s.g_hi[place][j]);
       const float2 lj = *reinterpret_cast<const float2*>(&s.g_lo[place][j]);
-      const float2 fj = *reinterpret_cast<const float2*>(&s.fk[j]);
+      const float2 fj = *reinterpret_cast<const float2*>(&s.fk_unit[j]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = 16 * w + g + 8 * half;
@@ -822,6 +838,16 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   float kk[4][2][4], qk[4][2][4];
   row_products(s, w, lane, kk, qk);
   __syncthreads();
+  if (w < 2) {
+    const float* f = w == 0 ? s.fk : s.fq;
+    float* unit = w == 0 ? s.fk_unit : s.fq_unit;
+    const float x = f[lane], y = f[lane + 32];
+    const float power = largest_power(x, y), down = inverse_power(power);
+    unit[lane] = x * down;
+    unit[lane + 32] = y * down;
+    if (lane == 0) (w == 0 ? s.fk_power : s.fq_power) = power;
+  }
+  __syncthreads();
 #pragma unroll 1
   for (int n = 0; n < p.heads_ratio; ++n) {
     const int at = n % kGroup;
@@ -837,9 +863,17 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
       s.work().image.beta[tid] = s.beta[at][tid];
       s.work().image.k_in[tid] = in * s.fk[tid];
       s.work().image.q_in[tid] = in * s.fq[tid] * p.q_scale;
-      const float left = (s.g_hi[at][kChunk - 1] - s.g_hi[at][tid]) + (s.g_lo[at][kChunk - 1] - s.g_lo[at][tid]);
-      s.work().image.k_out[tid] = exp2_fast(left) * s.fk[tid];
-      if (tid == kChunk - 1) s.work().image.decay = in;
+      const auto out = [&](int i) {
+        const float left = (s.g_hi[at][kChunk - 1] - s.g_hi[at][i]) + (s.g_lo[at][kChunk - 1] - s.g_lo[at][i]);
+        return exp2_fast(left) * s.fk[i];
+      };
+      const float k_out = out(tid), power = largest_power(k_out, out(tid ^ 32));
+      s.work().image.k_out[tid] = k_out * inverse_power(power);
+      if (tid == kChunk - 1) {
+        s.work().image.decay = in;
+        s.work().image.k_scale = power;
+        s.work().image.p_scale = s.fk_power * s.fq_power;
+      }
     }
     decayed_pairs(p, s, at, w, lane, kk, qk);
     __syncwarp();
@@ -906,12 +940,12 @@ constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW
 
 // The chunk's images to a stage by two bulk copies, its v rows by the moving threads.
 template <bool kVec>
-__device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid) {
+__device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid, bool late) {
   // What was read and written in this stage so far comes before the bulk copies, which go through the async
   // proxy (a barrier lies between that and this thread).
-  if (tid == 0) {
+  if (tid == 0 && !late) {  // after a wait that ran out there are no more of them, and the ones before have landed
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    barrier_expect(full, sizeof(KeyImage) + sizeof(PairImage));
+    barrier_expect(full, sizeof(KeyImage) + sizeof(PairImage) + p.extra_tx);
     bulk_copy(smem_u32(st.kq), p.keys + d.place * p.num_k_heads + d.head / p.heads_ratio, sizeof(KeyImage), full);
     bulk_copy(smem_u32(&st.pair), p.pairs + d.place * p.num_v_heads + d.head, sizeof(PairImage), full);
   }
@@ -1025,9 +1059,9 @@ __device__ __forceinline__ void store_pair(__nv_bfloat16* at, float x, float y) 
   *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(x, y);
 }
 
-// Waits until the barrier's phase has completed, the warp together.  After kWaitNs it gives up for good:
+// Waits until the barrier's phase has completed, the warp together.  After limit_ns it gives up for good:
 // it raises the fault, and from then on this warp stores nothing and waits for no product.
-__device__ __forceinline__ void wait_done(uint32_t bar, uint32_t parity, ChainSmem& s, bool& dead) {
+__device__ __forceinline__ void wait_done(uint32_t bar, uint32_t parity, ChainSmem& s, bool& dead, uint64_t limit_ns) {
   if (dead) return;
   uint64_t start = 0;
   while (true) {
@@ -1041,7 +1075,7 @@ __device__ __forceinline__ void wait_done(uint32_t bar, uint32_t parity, ChainSm
     uint64_t now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now)::"memory");
     if (start == 0) start = now;
-    if (__any_sync(0xffffffffu, now - start > kWaitNs)) {
+    if (__any_sync(0xffffffffu, now - start > limit_ns)) {
       dead = true;
       s.stop = 1;
       atomicOr(&g_prefill_faults, LD_FAULT_WAIT_TIMEOUT);
@@ -1162,9 +1196,9 @@ struct Products {
 // The products that the state waits for are done.  One warp asks the barrier, the others wait for it at a named
 // barrier: asking, eight warps took so many issue slots from the one that issues that a product of 32 cycles
 // (N = 64) was issued every 48.
-__device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool issuer) {
+__device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool issuer, uint64_t limit_ns) {
   if (issuer) {
-    wait_done(smem_u32(&s.done[0]), x.phase, s, x.dead);
+    wait_done(smem_u32(&s.done[0]), x.phase, s, x.dead, limit_ns);
     x.phase ^= 1;
   }
   bar_state();
@@ -1179,7 +1213,7 @@ __device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool i
 // waiting threads release.
 template <typename Taken>
 __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stage, uint32_t tmem, int v0, int lane,
-                                            bool issuer, Taken taken) {
+                                            bool issuer, uint64_t limit_ns, Taken taken) {
   const int g = lane >> 2, t = lane & 3;
   const Stage& st = s.stage[stage];
 
@@ -1202,7 +1236,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   }
 
   // R = beta (v - k_in Y).
-  wait_products(x, s, issuer);
+  wait_products(x, s, issuer, limit_ns);
   float Y[8][4];
   tmem_load(tmem + kTmemY, Y);
   const uint32_t v_base =
@@ -1250,16 +1284,15 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
     }
   }
 
-  // u, and k_out u in two terms.  k_out is at most 1 (the largest k~ of a row is in [1, 2)), so u's row
-  // scale serves both.
-  wait_products(x, s, issuer);
+  // u, and k_out u in two terms.  The largest k_out is in [1, 2), so u's row scale serves both.
+  wait_products(x, s, issuer, limit_ns);
   tmem_load(tmem + kTmemTr, Y);
   const float r_down0 = down0, r_down1 = down1;
   scale_rows(Y, up0, down0, up1, down1);
   const float w0 = r_down0 * down0, w1 = r_down1 * down1;
   if (t == 0) {
-    s.u_down[v0 + g] = w0;
-    s.u_down[v0 + g + 8] = w1;
+    s.u_down[v0 + g] = w0 * st.pair.p_scale;
+    s.u_down[v0 + g + 8] = w1 * st.pair.p_scale;
   }
   {
     uint32_t hi[4][4];
@@ -1297,8 +1330,9 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   }
   // S <- decay S + dS, one fp32 fused multiply-add per element.
   const float2 decay = make_float2(st.pair.decay, st.pair.decay);
-  const float2 w02 = make_float2(w0, w0), w12 = make_float2(w1, w1);
-  wait_products(x, s, issuer);
+  const float k0 = w0 * st.pair.k_scale, k1 = w1 * st.pair.k_scale;
+  const float2 w02 = make_float2(k0, k0), w12 = make_float2(k1, k1);
+  wait_products(x, s, issuer, limit_ns);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     tmem_load(tmem + kTmemDs + 64 * half, Y);
@@ -1398,7 +1432,7 @@ __device__ __forceinline__ void skip_items(const PrefillArgs& p, ChainSmem& s, i
 
 // Gives a free stage the upcoming work and starts its copies.  The moving threads together.
 template <typename StateT, bool kVec>
-__device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid) {
+__device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid, bool late) {
   if (tid == 0) st.work = d;
   if (d.kind == kWorkEnd) return;
   if (d.source > 0 && tid < 32) {  // a new item's state: into L2 by the time that it is read
@@ -1407,7 +1441,7 @@ __device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, cons
     constexpr int kBytes = kDim * kDim * sizeof(StateT) / 32;
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(state + tid * kBytes), "n"(kBytes) : "memory");
   }
-  copy_chunk<kVec>(p, st, d, full, tid);
+  copy_chunk<kVec>(p, st, d, full, tid, late);
 }
 
 // A persistent CTA per SM: the moving threads take items (a request's value head each), longest first, and
@@ -1432,7 +1466,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     const auto hand_over = [&](int stage, bool chunk) {
       cp_async_wait_groups<1>();  // but not for the gates, which were asked for last
       if (warp == 0 && chunk) {
-        wait_done(full(stage), (landed >> stage) & 1, s, late);
+        wait_done(full(stage), (landed >> stage) & 1, s, late, p.wait_ns);
         landed ^= 1u << stage;
       }
       bar_arrive(kBarFull + stage);
@@ -1449,7 +1483,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
 #pragma unroll 1
     for (int stage = 0; stage < 2 && more; ++stage) {
       skip_items(p, s, tid);
-      load_stage<StateT, kVec>(p, s.stage[stage], s.upcoming, full(stage), tid);
+      load_stage<StateT, kVec>(p, s.stage[stage], s.upcoming, full(stage), tid, late);
       cp_async_commit();
       more = s.upcoming.kind == kWorkChunk;
       bar_move();
@@ -1475,7 +1509,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       __syncwarp();
       bar_sync(kBarChunkDone);
       if (warp == 0) {
-        wait_done(smem_u32(&s.done[1]), phase, s, dead);
+        wait_done(smem_u32(&s.done[1]), phase, s, dead, p.wait_ns);
         phase ^= 1;
       }
       bar_move();
@@ -1487,7 +1521,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       if (s.stage[stage ^ 1].work.kind == kWorkChunk) bar_arrive(kBarTaken);
       if (refill) {
         skip_items(p, s, tid);
-        load_stage<StateT, kVec>(p, st, s.upcoming, full(stage), tid);
+        load_stage<StateT, kVec>(p, st, s.upcoming, full(stage), tid, late);
         more = s.upcoming.kind == kWorkChunk;
       }
       cp_async_commit();
@@ -1546,7 +1580,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
           for (int e = 0; e < 4; ++e) x.S[i][e] = 0.0f;
         }
       }
-      chain_chunk(x, s, stage, tmem, v0, lane, issuer, [&] {
+      chain_chunk(x, s, stage, tmem, v0, lane, issuer, p.wait_ns, [&] {
         if (n >= 1) {
           bar_sync(kBarTaken);
           tmem_after();
@@ -1736,6 +1770,8 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   args.weight_bf16 = weight_dtype == LD_DTYPE_BF16;
   args.q_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(kDim)));
   args.eps = eps;
+  args.wait_ns = wait_limit_ns();
+  args.extra_tx = wait_test_extra_bytes();
   // 16-byte copies of the q, k, v and gate rows and 8-byte stores to out where every row allows them.
   const bool vec = aligned(qkv, 16) && qkv_row_stride % 8 == 0 && aligned(gate, 16) && gate_row_stride % 8 == 0 &&
                    aligned(out, 8);
