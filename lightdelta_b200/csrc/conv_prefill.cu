@@ -158,6 +158,47 @@ __device__ __forceinline__ Row<kVec> earlier(const ConvPrefillArgs& p, const Pla
   return load_window<kVec>(p, at.source, channel, static_cast<int>(kWidth - 1 + (i - at.begin)));
 }
 
+// Outputs of `count` tokens, whose loads go out together, and the window behind them.  A full batch is straight code
+// in which every input is unpacked once.
+template <int kVec, int kWidth, bool kFull>
+__device__ __forceinline__ void convolve(const __nv_bfloat16* x, int64_t x_row, __nv_bfloat16* out, int64_t out_row,
+                                         int count, const float2 (&wt)[kWidth][Row<kVec>::kWords],
+                                         const float2 (&bias)[Row<kVec>::kWords], Row<kVec> (&window)[kWidth - 1]) {
+  constexpr int kWords = Row<kVec>::kWords;
+  Row<kVec> rows[kWidth - 1 + kBatch];
+#pragma unroll
+  for (int j = 0; j < kWidth - 1; ++j) rows[j] = window[j];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if (kFull || i < count) rows[kWidth - 1 + i] = load_row<kVec>(x + i * x_row);
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if (kFull || i < count) {
+      Row<kVec> y;
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        float2 acc = bias[c];
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) {
+          acc = fma2(make_float2(bf16_low(rows[i + j].w[c]), bf16_high(rows[i + j].w[c])), wt[j][c], acc);
+        }
+        const float2 z = silu_fast(acc);
+        y.w[c] = pack_bf16(z.x, z.y);
+      }
+      store_row<kVec>(out + i * out_row, y);
+      if (!kFull) {
+#pragma unroll
+        for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[i + 1 + j];
+      }
+    }
+  }
+  if (kFull) {
+#pragma unroll
+    for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[kBatch + j];
+  }
+}
+
 template <int kVec, int kWidth>
 __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefillArgs p) {
   grid_dependency_wait();
@@ -245,30 +286,10 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
       t += count;
       continue;
     }
-    Row<kVec> rows[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (i < count) rows[i] = load_row<kVec>(x + i * p.x_row);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (i < count) {
-        Row<kVec> y;
-#pragma unroll
-        for (int c = 0; c < kWords; ++c) {
-          float2 acc = bias[c];
-#pragma unroll
-          for (int j = 0; j < kWidth - 1; ++j) {
-            acc = fma2(make_float2(bf16_low(window[j].w[c]), bf16_high(window[j].w[c])), wt[j][c], acc);
-          }
-          acc = fma2(make_float2(bf16_low(rows[i].w[c]), bf16_high(rows[i].w[c])), wt[kWidth - 1][c], acc);
-          y.w[c] = pack_bf16(silu_fast(acc.x), silu_fast(acc.y));
-        }
-        store_row<kVec>(out + i * p.dim, y);
-#pragma unroll
-        for (int j = 0; j + 1 < kWidth - 1; ++j) window[j] = window[j + 1];
-        window[kWidth - 2] = rows[i];
-      }
+    if (count == kBatch) {
+      convolve<kVec, kWidth, true>(x, p.x_row, out, p.dim, count, wt, bias, window);
+    } else {
+      convolve<kVec, kWidth, false>(x, p.x_row, out, p.dim, count, wt, bias, window);
     }
     t += count;
     if (t == at.next_end) {
