@@ -10,8 +10,12 @@
 //
 // One pass bound by HBM: 2 bytes read and 2 written per (token, channel).  A thread owns 4 channels of a
 // tile of consecutive tokens, whatever requests they belong to, and slides the window along, so a tile
-// reads w - 1 rows beyond its own; rows come in batches of 8 loads before the first is used.  silu costs
-// two special-function operations per value, 0.7 of the time HBM needs, which the batches overlap.
+// reads w - 1 rows beyond its own; rows come in batches of 8 loads before the first is used, and a whole
+// batch is straight code.  Six CTAs on an SM (80 registers a thread) keep enough batches in flight: 24
+// prompts of 16,000 tokens in all with 8,192 channels take 108.7 us, 4.84 TB/s; without that bound (96
+// registers, five CTAs) 124 us, with seven or eight and spills 120 and 125, and batches of 4 rows at eight
+// CTAs 111.  8 channels a thread took 222 registers and 299 us.  What is left is instructions: silu's two
+// special-function operations per value and the tile's start.
 // A request's first w - 1 tokens all go to the thread that has its first one: only that thread reads the
 // history, so it can also write the slot when a request goes on inside a block and its source slot is
 // its first destination.
@@ -45,7 +49,8 @@ struct ConvPrefillArgs {
   const __nv_bfloat16* weight;
   const __nv_bfloat16* bias;
   const int32_t* table;
-  int64_t table_row, table_width, block_size;
+  int64_t table_row, table_width;
+  uint32_t block_size;  // larger ones as the largest of these: every position is below it
   const int32_t* context;
   const int32_t* cu;
   int n_requests;
@@ -115,7 +120,7 @@ __device__ __forceinline__ void store_window(const ConvPrefillArgs& p, int32_t s
 // The request that a thread is in.
 struct Place {
   int64_t begin, end;   // its tokens
-  int64_t context;
+  uint32_t context;     // a position, context + token, is below 2^32 - 1
   int64_t next_end;     // the next token after which a block or the request ends
   const int32_t* row;
   int32_t source;       // slot of the history (0: none)
@@ -126,24 +131,28 @@ struct Place {
 __device__ __forceinline__ void enter(const ConvPrefillArgs& p, int r, int64_t token, bool report, Place& at) {
   at.begin = p.cu[r];
   at.end = p.cu[r + 1];
-  at.context = p.context[r];
+  const int32_t context = p.context[r];
+  at.context = static_cast<uint32_t>(context);
   at.row = p.table + r * p.table_row;
   at.source = 0;
   at.kept = -1;
   at.next_end = at.end;
   unsigned int fault = 0;
-  at.ok = at.context >= 0 && (at.context + (at.end - at.begin) - 1) / p.block_size < p.table_width;
+  at.ok = context >= 0 && (at.context + static_cast<uint32_t>(at.end - at.begin) - 1) / p.block_size < p.table_width;
   if (!at.ok) {
     fault = LD_FAULT_TABLE_BLOCKS;
   } else {
-    if (at.context > 0) {
-      at.source = at.row[(at.context - 1) / p.block_size];
+    uint32_t block = 0;
+    if (context > 0) {
+      block = (at.context - 1) / p.block_size;
+      at.source = at.row[block];
       if (at.source >= p.n_slots) fault = LD_FAULT_CONV_SLOT_RANGE;
       at.ok = at.source > 0 && at.source < p.n_slots;
-      if (at.context % p.block_size != 0) at.kept = static_cast<int32_t>(at.context / p.block_size);
+      if (at.context - block * p.block_size < p.block_size) at.kept = static_cast<int32_t>(block);
     }
-    const int64_t position = at.context + (token - at.begin);
-    at.next_end = min(at.end, at.begin + (position / p.block_size + 1) * p.block_size - at.context);
+    if (token != at.begin) block = (at.context + static_cast<uint32_t>(token - at.begin)) / p.block_size;
+    if (token == at.begin && context > 0 && at.kept < 0) ++block;  // the context fills its block
+    at.next_end = min(at.end, at.begin + (static_cast<int64_t>(block) + 1) * p.block_size - at.context);
   }
   if (fault != 0 && report) atomicOr(&g_conv_prefill_faults, fault);
 }
@@ -170,7 +179,8 @@ __device__ __forceinline__ void convolve(const __nv_bfloat16* x, int64_t x_row, 
   for (int j = 0; j < kWidth - 1; ++j) rows[j] = window[j];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    if (kFull || i < count) rows[kWidth - 1 + i] = load_row<kVec>(x + i * x_row);
+    if (kFull || i < count) rows[kWidth - 1 + i] = load_row<kVec>(x);
+    x += x_row;
   }
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
@@ -186,7 +196,8 @@ __device__ __forceinline__ void convolve(const __nv_bfloat16* x, int64_t x_row, 
         const float2 z = silu_fast(acc);
         y.w[c] = pack_bf16(z.x, z.y);
       }
-      store_row<kVec>(out + i * out_row, y);
+      store_row<kVec>(out, y);
+      out += out_row;
       if (!kFull) {
 #pragma unroll
         for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[i + 1 + j];
@@ -200,7 +211,7 @@ __device__ __forceinline__ void convolve(const __nv_bfloat16* x, int64_t x_row, 
 }
 
 template <int kVec, int kWidth>
-__global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefillArgs p) {
+__global__ void __launch_bounds__(kThreads, 6) conv_prefill_kernel(const ConvPrefillArgs p) {
   grid_dependency_wait();
   allow_dependent_launch();
   const int64_t channel = (static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x) * kVec;
@@ -293,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const ConvPrefil
     }
     t += count;
     if (t == at.next_end) {
-      const int64_t block = (at.context + (t - 1 - at.begin)) / p.block_size;
+      const int64_t block = (at.context + static_cast<uint32_t>(t - 1 - at.begin)) / p.block_size;
       if (block != at.kept) {
         const int32_t slot = at.row[block];
         if (slot > 0 && slot < p.n_slots) {
@@ -314,8 +325,11 @@ template <int kWidth>
 cudaError_t launch_width(ConvPrefillArgs& args, bool vec, cudaStream_t stream) {
   const int channels = (vec ? kVector : 1) * kThreads;
   const int64_t groups = (args.dim + channels - 1) / channels;
-  // 32 tokens per thread read 3 rows of 35 twice; 8 tokens per thread spread short batches over the SMs.
-  args.tile = args.n_tokens * groups >= 32 * 4 * 148 ? 32 : 8;
+  // A tile's thread reads 3 rows that the tile before reads too, and finds its request and its weights: 24 prompts of
+  // 16,000 tokens in all (8,192 channels) take 108.7 us at 64 tokens per thread, 110.5 at 32.  Smaller batches are
+  // spread over the SMs (six CTAs each) before their tiles grow.
+  const int64_t work = args.n_tokens * groups;
+  args.tile = work >= 64 * 6 * 148 ? 64 : work >= 32 * 4 * 148 ? 32 : 8;
   const dim3 grid(static_cast<unsigned int>((args.n_tokens + args.tile - 1) / args.tile),
                   static_cast<unsigned int>(groups));
   if (vec) return launch(conv_prefill_kernel<kVector, kWidth>, grid, dim3(kThreads), 0, stream, 1, args);
@@ -399,7 +413,7 @@ extern "C" int ld_conv_prefill(const void* x, int64_t x_row_stride, int64_t n_to
   args.table = table;
   args.table_row = table_row_stride;
   args.table_width = table_width;
-  args.block_size = block_size;
+  args.block_size = static_cast<uint32_t>(std::min<int64_t>(block_size, UINT32_MAX));
   args.context = context;
   args.cu = cu;
   args.n_requests = static_cast<int>(n_requests);

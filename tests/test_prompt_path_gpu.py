@@ -444,6 +444,17 @@ def test_conv_prefill_long_batch():
     Conv([2500, 31, 2, 1200], [0, 64, 100, 3], dim=2560, block=512, seed=31).check()
 
 
+@pytest.mark.parametrize("dim,tokens", [(2560, 4000), (8192, 3700)])
+def test_conv_prefill_batches_that_take_long_tiles(dim, tokens):
+    """Batches large enough for tiles of 32 and of 64 tokens, with requests that begin and end anywhere in them."""
+    rng = np.random.default_rng(dim)
+    lens = []
+    while sum(lens) < tokens:
+        lens.append(int(rng.choice([1, 2, 3, 5, 31, 32, 33, 62, 63, 64, 65, 200])))
+    contexts = rng.integers(0, 100, len(lens)).tolist()
+    Conv(lens, contexts, dim=dim, block=64, seed=dim).check()
+
+
 def test_conv_prefill_invalid_requests():
     case = Conv([10, 20, 30, 5], [64, 64, -1, 0], seed=32)
     case.table[0, 0], case.table[1, 0], case.table[3, 0] = 0, 1000, 1001
