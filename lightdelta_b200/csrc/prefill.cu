@@ -998,22 +998,22 @@ __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, in
 // they compete for.
 template <bool kVec>
 __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Stage& st, const Work& d,
-                                              const float (&wt)[8], int tid) {
+                                              const float2 (&wt)[4], int tid) {
   const int part = tid & 15;
   const bool stop = s.stop != 0;
   __nv_bfloat16* out = p.out + (d.token0 * p.num_v_heads + d.head) * kDim + 4 * part;
 #pragma unroll 1
   for (int i = tid >> 4; i < kChunk; i += kMoveThreads / 16) {
-    float4 o[2];
-    float sq = 0.0f;
+    float2 o[2][2], sum = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      o[half] = *reinterpret_cast<const float4*>(&s.o[i * kORow + 64 * half + 4 * part]);
-      sq = fmaf(o[half].x, o[half].x, sq);
-      sq = fmaf(o[half].y, o[half].y, sq);
-      sq = fmaf(o[half].z, o[half].z, sq);
-      sq = fmaf(o[half].w, o[half].w, sq);
+      const float4 x = *reinterpret_cast<const float4*>(&s.o[i * kORow + 64 * half + 4 * part]);
+      o[half][0] = make_float2(x.x, x.y);
+      o[half][1] = make_float2(x.z, x.w);
+      sum = fma2(o[half][0], o[half][0], sum);
+      sum = fma2(o[half][1], o[half][1], sum);
     }
+    float sq = sum.x + sum.y;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     const float rstd = rsqrtf(sq * (1.0f / kDim) + p.eps);
@@ -1022,11 +1022,11 @@ __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainS
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const uint2 z = *reinterpret_cast<const uint2*>(&st.gate[i * kVRow + 64 * half + 4 * part]);
-      const float y0 = o[half].x * rstd * (wt[4 * half + 0] * silu_fast(bf16_low(z.x)));
-      const float y1 = o[half].y * rstd * (wt[4 * half + 1] * silu_fast(bf16_high(z.x)));
-      const float y2 = o[half].z * rstd * (wt[4 * half + 2] * silu_fast(bf16_low(z.y)));
-      const float y3 = o[half].w * rstd * (wt[4 * half + 3] * silu_fast(bf16_high(z.y)));
-      const uint32_t lo = pack_bf16(y0, y1), hi = pack_bf16(y2, y3);
+      const float2 r = make_float2(rstd, rstd);
+      const float2 y0 = mul2(mul2(o[half][0], r), mul2(wt[2 * half], silu_fast(make_float2(bf16_low(z.x), bf16_high(z.x)))));
+      const float2 y1 =
+          mul2(mul2(o[half][1], r), mul2(wt[2 * half + 1], silu_fast(make_float2(bf16_low(z.y), bf16_high(z.y)))));
+      const uint32_t lo = pack_bf16(y0.x, y0.y), hi = pack_bf16(y1.x, y1.y);
       __nv_bfloat16* at = row + 64 * half;
       if (live) {
         if constexpr (kVec) {
@@ -1085,18 +1085,24 @@ __device__ __forceinline__ void wait_done(uint32_t bar, uint32_t parity, ChainSm
   tmem_after();
 }
 
+__device__ __forceinline__ float largest(float x, float y, float z) {  // of the magnitudes
+  float m;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
+
 // Largest magnitudes of the two rows of a fragment array, over the row's four lanes, as row scales.
 template <int kTiles>
 __device__ __forceinline__ void scale_rows(const float (&x)[kTiles][4], float& up0, float& down0, float& up1,
                                            float& down1) {
-  float top0 = 0.0f, top1 = 0.0f;
+  float top0[2] = {}, top1[2] = {};  // of even and odd tiles: shorter chains
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
-    top0 = fmaxf(top0, fmaxf(fabsf(x[n][0]), fabsf(x[n][1])));
-    top1 = fmaxf(top1, fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+    top0[n & 1] = largest(top0[n & 1], x[n][0], x[n][1]);
+    top1[n & 1] = largest(top1[n & 1], x[n][2], x[n][3]);
   }
-  row_scale(quad_max(top0), up0, down0);
-  row_scale(quad_max(top1), up1, down1);
+  row_scale(quad_max(fmaxf(top0[0], top0[1])), up0, down0);
+  row_scale(quad_max(fmaxf(top1[0], top1[1])), up1, down1);
 }
 
 // Four k-steps (64 columns) of a fragment array, scaled, as hi and lo A operands in TMEM.
@@ -1494,9 +1500,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       hand_over(stage, more);
       bar_move();
     }
-    float wt[8];
+    float2 wt[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wt[e] = load_param(p.weight, 64 * (e >> 2) + 4 * (lane & 15) + (e & 3), p.weight_bf16);
+    for (int e = 0; e < 4; ++e) {
+      const int at = 64 * (e >> 1) + 4 * (lane & 15) + 2 * (e & 1);
+      wt[e] = make_float2(load_param(p.weight, at, p.weight_bf16), load_param(p.weight, at + 1, p.weight_bf16));
+    }
     const int v0 = 32 * (warp & 3) + 16 * (warp >> 2);  // the TMEM lanes of a warp, as below
     uint32_t phase = 0;
     bool dead = false;
