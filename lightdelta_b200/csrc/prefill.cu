@@ -389,24 +389,44 @@ __device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1
 // ------------------------------------------------------------------------------------------
 constexpr int kGroup = 4;  // value heads whose gates are computed together, one per warp
 
-struct PairWork {
-  PairImage image;
-  __align__(128) __half l_hi[6 * 256];   // L's blocks below the diagonal ones, packed row by row
-  __align__(128) __half l_lo[6 * 256];
-  __align__(16) float diag[4][16 * 16];  // L's diagonal blocks
+// What a value head's inverse is made in; heads are worked on two at a time.
+struct PairHead {
+  __align__(16) __half t_hi[kTriBlocks * 256];
+  __half t_lo[kTriBlocks * 256];
+  __half l_hi[6 * 256];   // L's blocks below the diagonal ones, packed row by row
+  __half l_lo[6 * 256];
+  float diag[4][16 * 16];  // L's diagonal blocks
+  float pad[16];           // the two heads' diagonal blocks, read side by side, lie in different banks
 };
 
 struct PairSmem {
-  __align__(1024) unsigned char tiles[sizeof(KeyImage)];  // the key image, then, its products in registers, PairWork
+  union {
+    __align__(128) unsigned char tiles[sizeof(KeyImage)];  // the key image, then, its products in registers,
+    unsigned char heads[2 * sizeof(PairHead)];
+    uint32_t counts[64];  // of order_requests
+  };
   float g_hi[kGroup][kChunk], g_lo[kGroup][kChunk], beta[kGroup][kChunk];
   float fk[kChunk], fq[kChunk];
   float fk_unit[kChunk], fq_unit[kChunk];  // divided by their largest's power of two
   float fk_power, fq_power;
 
   __device__ __forceinline__ __half* kq() { return reinterpret_cast<__half*>(tiles); }
-  __device__ __forceinline__ PairWork& work() { return *reinterpret_cast<PairWork*>(tiles); }
+  __device__ __forceinline__ PairHead& head(int i) { return reinterpret_cast<PairHead*>(heads)[i]; }
 };
-static_assert(sizeof(PairWork) <= sizeof(KeyImage), "the work area takes the tiles' place");
+static_assert(sizeof(PairHead) % 128 == 64, "heads differ in banks, and matrices stay 16-byte aligned");
+
+// The 16 x 16 blocks on and below the diagonal that a warp has: the diagonal one of its number and one or two side by
+// side below, so that no warp has more than three of the ten.
+struct Blocks {
+  int w;      // diagonal block
+  int row;    // row block of the others
+  int col;    // column block of the first
+  bool two;   // and of a second, col + 1
+  __device__ __forceinline__ explicit Blocks(int warp)
+      : w(warp), row(warp == 1 ? 2 : warp == 3 ? 1 : 3), col(warp == 2 ? 2 : 0), two(warp < 2) {}
+  __device__ __forceinline__ int ib(int b) const { return b == 0 ? w : row; }
+  __device__ __forceinline__ int jb(int b) const { return b == 0 ? w : col + b - 1; }
+};
 
 // L's blocks below the diagonal ones, row by row.
 __host__ __device__ constexpr int low_block(int ib, int jb) { return 256 * (ib * (ib - 1) / 2 + jb); }
@@ -437,13 +457,15 @@ __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row
 // largest magnitude to [1, 2).  Returns that power's inverse.
 __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
   uint16_t* row = tile + i * 64;
-  uint32_t top2 = 0;  // the largest magnitudes so far of even and odd columns; bf16 magnitudes order as integers
+  __nv_bfloat162 top = __floats2bfloat162_rn(0.0f, 0.0f);  // the largest magnitudes so far of even and odd columns
 #pragma unroll
   for (int piece = 0; piece < kDim / 8; ++piece) {
     const uint4 raw = *reinterpret_cast<const uint4*>(row + (piece >> 3) * kKeyHalf + (((piece & 7) ^ (i & 7)) << 3));
-    top2 = __vmaxu2(__vmaxu2(top2, raw.x & 0x7fff7fffu), raw.y & 0x7fff7fffu);
-    top2 = __vmaxu2(__vmaxu2(top2, raw.z & 0x7fff7fffu), raw.w & 0x7fff7fffu);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[n])));
   }
+  const uint32_t top2 = *reinterpret_cast<const uint32_t*>(&top);  // bf16 magnitudes order as integers
   const int e = min(max(static_cast<int>(max(top2 >> 16, top2 & 0xffffu) >> 7), 1), 253);
   const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
 #pragma unroll
@@ -454,7 +476,8 @@ __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
     uint32_t y[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      y[n] = pack_half(__uint_as_float(w[n] << 16) * down, __uint_as_float(w[n] & 0xffff0000u) * down);
+      const float2 x = mul2(make_float2(bf16_low(w[n]), bf16_high(w[n])), make_float2(down, down));
+      y[n] = pack_half(x.x, x.y);
     }
     *at = make_uint4(y[0], y[1], y[2], y[3]);
   }
@@ -518,40 +541,43 @@ __device__ __forceinline__ void chunk_gates(const PrefillArgs& p, PairSmem& s, i
   }
 }
 
-// Products of this warp's 16 rows of k~ and q~ with the rows of k~ up to its own, and the rows' factors
-// (the L2 norm's reciprocal times the power of two that the scaling took) from the diagonals of k~ k~^T
-// and q~ q~^T.
-__device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float (&kk)[4][2][4],
-                                             float (&qk)[4][2][4]) {
-  const uint32_t k_a = lane_addr<true>(s.kq(), lane) + w * 16 * 128;
-  const uint32_t q_a = lane_addr<true>(s.kq() + kHalf, lane) + w * 16 * 128;
+// This warp's blocks of k~ k~^T and q~ k~^T, and its rows' factors (the L2 norm's reciprocal times the power of two that
+// the scaling took) from the diagonals of k~ k~^T and q~ q~^T.
+__device__ __forceinline__ void row_products(PairSmem& s, const Blocks& mine, int lane, float (&kk)[3][2][4],
+                                             float (&qk)[3][2][4]) {
+  const uint32_t k_a = lane_addr<true>(s.kq(), lane), q_a = lane_addr<true>(s.kq() + kHalf, lane);
   const uint32_t k_b = lane_addr<false>(s.kq(), lane);
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb) {
+  for (int b = 0; b < 3; ++b) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) kk[nb][m][e] = qk[nb][m][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) kk[b][m][e] = qk[b][m][e] = 0.0f;
     }
   }
   float qq[2][4] = {};
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) {
-    uint32_t ak[4], aq[4];
-    ldsm4(block<kKeyHalf>(k_a, 0, ks), ak);
-    ldsm4(block<kKeyHalf>(q_a, 0, ks), aq);
+    uint32_t ak[4], aq[4], b[4];
+    ldsm4(block<kKeyHalf>(k_a, mine.w, ks), ak);
+    ldsm4(block<kKeyHalf>(q_a, mine.w, ks), aq);
     // A fragments are (rows 0-7, cols 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15): as B, rows 0-7 are 0, 2.
-    mma(qq[0], aq, aq[0], aq[2]);
-    mma(qq[1], aq, aq[1], aq[3]);
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      if (nb <= w) {
-        uint32_t b[4];
-        ldsm4(block<kKeyHalf>(k_b, nb, ks), b);
+    for (int m = 0; m < 2; ++m) {
+      mma(kk[0][m], ak, ak[m], ak[2 + m]);
+      mma(qk[0][m], aq, ak[m], ak[2 + m]);
+      mma(qq[m], aq, aq[m], aq[2 + m]);
+    }
+    ldsm4(block<kKeyHalf>(k_a, mine.row, ks), ak);
+    ldsm4(block<kKeyHalf>(q_a, mine.row, ks), aq);
+#pragma unroll
+    for (int n = 1; n < 3; ++n) {
+      if (n == 1 || mine.two) {
+        ldsm4(block<kKeyHalf>(k_b, mine.jb(n), ks), b);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          mma(kk[nb][m], ak, b[2 * m], b[2 * m + 1]);
-          mma(qk[nb][m], aq, b[2 * m], b[2 * m + 1]);
+          mma(kk[n][m], ak, b[2 * m], b[2 * m + 1]);
+          mma(qk[n][m], aq, b[2 * m], b[2 * m + 1]);
         }
       }
     }
@@ -560,14 +586,10 @@ __device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    float k2 = 0.0f;
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      if (nb == w) k2 = (g & 1) ? kk[nb][half][2 * half + 1] : kk[nb][half][2 * half];
-    }
+    const float k2 = (g & 1) ? kk[0][half][2 * half + 1] : kk[0][half][2 * half];
     const float q2 = (g & 1) ? qq[half][2 * half + 1] : qq[half][2 * half];
     if (t == g / 2) {
-      const int i = 16 * w + g + 8 * half;
+      const int i = 16 * mine.w + g + 8 * half;
       const float up_k = s.fk[i], up_q = s.fq[i];
       s.fk[i] = up_k * rsqrtf(k2 * up_k * up_k + 1e-6f);
       s.fq[i] = up_q * rsqrtf(q2 * up_q * up_q + 1e-6f);
@@ -575,84 +597,107 @@ __device__ __forceinline__ void row_products(PairSmem& s, int w, int lane, float
   }
 }
 
-// L and P of this warp's rows for one value head.
-__device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s, int place, int w, int lane,
-                                              const float (&kk)[4][2][4], const float (&qk)[4][2][4]) {
-  const int g = lane >> 2, t = lane & 3;
-  float g_hi[2], g_lo[2], row_k[2], row_q[2];
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int i = 16 * w + g + 8 * half;
-    g_hi[half] = s.g_hi[place][i];
-    g_lo[half] = s.g_lo[place][i];
-    row_k[half] = s.beta[place][i] * s.fk[i] * s.fk_power;
-    row_q[half] = p.q_scale * s.fq_unit[i];
+// The factors of the chunk's rows for one value head, row i = 0..63 by two warps, straight to its image.
+__device__ __forceinline__ void row_factors(const PrefillArgs& p, PairSmem& s, int place, int i, PairImage& image) {
+  const float in = exp2_fast(s.g_hi[place][i] + s.g_lo[place][i]);
+  image.beta[i] = s.beta[place][i];
+  image.k_in[i] = in * s.fk[i];
+  image.q_in[i] = in * s.fq[i] * p.q_scale;
+  const auto out = [&](int j) {
+    const float left = (s.g_hi[place][kChunk - 1] - s.g_hi[place][j]) + (s.g_lo[place][kChunk - 1] - s.g_lo[place][j]);
+    return exp2_fast(left) * s.fk[j];
+  };
+  const float k_out = out(i), power = largest_power(k_out, out(i ^ 32));
+  image.k_out[i] = k_out * inverse_power(power);
+  if (i == kChunk - 1) {
+    image.decay = in;
+    image.k_scale = power;
+    image.p_scale = s.fk_power * s.fq_power;
   }
+}
+
+// L and P of this warp's blocks for one value head; P goes straight to the image, 128 bytes a store.
+__device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s, PairHead& head, int place,
+                                              const Blocks& mine, int lane, const float (&kk)[3][2][4],
+                                              const float (&qk)[3][2][4], __half* p_image) {
+  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb) {
-    if (nb > w) continue;
+  for (int b = 0; b < 3; ++b) {
+    if (b == 2 && !mine.two) continue;
+    const int row0 = 16 * mine.ib(b) + g, col0 = 16 * mine.jb(b) + 2 * t;
+    float g_hi[2], g_lo[2], row_k[2], row_q[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int i = row0 + 8 * half;
+      g_hi[half] = s.g_hi[place][i];
+      g_lo[half] = s.g_lo[place][i];
+      row_k[half] = s.beta[place][i] * s.fk[i] * s.fk_power;
+      row_q[half] = p.q_scale * s.fq_unit[i];
+    }
+    __half* to_p = p_image + tri_block(mine.ib(b), mine.jb(b)) + core(g, 2 * t);
+    const int to_l = low_block(mine.row, mine.jb(b)) + core(g, 2 * t);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const int j = 16 * nb + 8 * m + 2 * t;
+      const int j = col0 + 8 * m;
       const float2 hj = *reinterpret_cast<const float2*>(&s.g_hi[place][j]);
       const float2 lj = *reinterpret_cast<const float2*>(&s.g_lo[place][j]);
       const float2 fj = *reinterpret_cast<const float2*>(&s.fk_unit[j]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int i = 16 * w + g + 8 * half;
         const float d0 = fj.x * exp2_fast((g_hi[half] - hj.x) + (g_lo[half] - lj.x));
         const float d1 = fj.y * exp2_fast((g_hi[half] - hj.y) + (g_lo[half] - lj.y));
-        const float l0 = j < i ? row_k[half] * d0 * kk[nb][m][2 * half] : 0.0f;
-        const float l1 = j + 1 < i ? row_k[half] * d1 * kk[nb][m][2 * half + 1] : 0.0f;
-        const float p0 = j <= i ? row_q[half] * d0 * qk[nb][m][2 * half] : 0.0f;
-        const float p1 = j + 1 <= i ? row_q[half] * d1 * qk[nb][m][2 * half + 1] : 0.0f;
-        *reinterpret_cast<uint32_t*>(&s.work().image.p[tri(i, j)]) = pack_half(p0, p1);
-        if (nb == w) {
-          *reinterpret_cast<float2*>(&s.work().diag[w][(g + 8 * half) * 16 + (j & 15)]) = make_float2(l0, l1);
+        float l0 = row_k[half] * d0 * kk[b][m][2 * half], l1 = row_k[half] * d1 * kk[b][m][2 * half + 1];
+        float p0 = row_q[half] * d0 * qk[b][m][2 * half], p1 = row_q[half] * d1 * qk[b][m][2 * half + 1];
+        if (b == 0) {
+          const int i = row0 + 8 * half;
+          l0 = j < i ? l0 : 0.0f;
+          l1 = j + 1 < i ? l1 : 0.0f;
+          p0 = j <= i ? p0 : 0.0f;
+          p1 = j + 1 <= i ? p1 : 0.0f;
+          *reinterpret_cast<float2*>(&head.diag[mine.w][(g + 8 * half) * 16 + 8 * m + 2 * t]) = make_float2(l0, l1);
         } else {
           uint32_t hi, lo;
           split(make_float2(l0, l1), hi, lo);
-          *reinterpret_cast<uint32_t*>(&s.work().l_hi[low(i, j)]) = hi;
-          *reinterpret_cast<uint32_t*>(&s.work().l_lo[low(i, j)]) = lo;
+          *reinterpret_cast<uint32_t*>(&head.l_hi[to_l + core(8 * half, 8 * m)]) = hi;
+          *reinterpret_cast<uint32_t*>(&head.l_lo[to_l + core(8 * half, 8 * m)]) = lo;
         }
+        *reinterpret_cast<uint32_t*>(&to_p[core(8 * half, 8 * m)]) = pack_half(p0, p1);
       }
     }
   }
 }
 
-// Inverse of this warp's diagonal block of I + L by forward substitution, one column per lane.
-__device__ __forceinline__ void invert_diagonal(PairSmem& s, int w, int lane) {
-  const int c = lane & 15;
+// Inverse of a diagonal block of I + L by forward substitution: one column per lane, a head per half warp.
+__device__ __forceinline__ void invert_diagonal(PairHead& head, int w, int c) {
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float sum0 = i == c ? 1.0f : 0.0f, sum1 = 0.0f;
 #pragma unroll
-    for (int j = 0; j < i; ++j) {
-      const float l = s.work().diag[w][i * 16 + j];
-      if (j & 1) {
-        sum1 = fmaf(-l, x[j], sum1);
-      } else {
-        sum0 = fmaf(-l, x[j], sum0);
-      }
+    for (int j = 0; j < i; j += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(&head.diag[w][i * 16 + j]);
+      sum0 = fmaf(-l.x, x[j], sum0);
+      if (j + 1 < i) sum1 = fmaf(-l.y, x[j + 1], sum1);
+      if (j + 2 < i) sum0 = fmaf(-l.z, x[j + 2], sum0);
+      if (j + 3 < i) sum1 = fmaf(-l.w, x[j + 3], sum1);
     }
     x[i] = sum0 + sum1;
   }
-  if (lane < 16) {
+  __half* to_hi = head.t_hi + tri_block(w, w) + core(0, c);
+  __half* to_lo = head.t_lo + tri_block(w, w) + core(0, c);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const __half hi = __float2half_rn(x[i]);
-      s.work().image.t_hi[tri(16 * w + i, 16 * w + c)] = hi;
-      s.work().image.t_lo[tri(16 * w + i, 16 * w + c)] = __float2half_rn(x[i] - __half2float(hi));
-    }
+  for (int i = 0; i < 16; ++i) {
+    const __half hi = __float2half_rn(x[i]);
+    to_hi[core(i, 0)] = hi;
+    to_lo[core(i, 0)] = __float2half_rn(x[i] - __half2float(hi));
   }
 }
 
 // The 16 x 16 blocks of T below diagonal block w, top to bottom:
 //   T_iw = -T_ii sum_{k=w}^{i-1} L_ik T_kw,  held transposed so that each result is the next A operand.
-__device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
-  const uint32_t t_hi = core_addr(s.work().image.t_hi, lane), t_lo = core_addr(s.work().image.t_lo, lane);
-  const uint32_t l_hi = core_addr(s.work().l_hi, lane), l_lo = core_addr(s.work().l_lo, lane);
+__device__ __forceinline__ void invert_column(PairHead& head, int w, int lane) {
+  const uint32_t t_hi = core_addr(head.t_hi, lane), t_lo = core_addr(head.t_lo, lane);
+  const uint32_t l_hi = core_addr(head.l_hi, lane), l_lo = core_addr(head.l_lo, lane);
   uint32_t x_hi[3][4], x_lo[3][4];  // T_kw^T as A fragments, k = w, w + 1, w + 2
   // ldmatrix.trans of T_ww: matrices (cols 0-7, rows 0-7), (cols 8-15, rows 0-7), (0-7, 8-15), (8-15, 8-15).
   ldsm4_t(t_hi + 2 * tri_block(w, w), x_hi[0]);
@@ -692,19 +737,20 @@ __device__ __forceinline__ void invert_column(PairSmem& s, int w, int lane) {
         mma(y[n], a_hi, b_hi[2 * n], b_hi[2 * n + 1]);
       }
       // y[n] is -T_iw^T: row m = column of T_iw (g, g + 8), column = row of T_iw (8n + 2t, + 1).
+      __half* to_hi = head.t_hi + tri_block(i, w) + core(2 * t, g);
+      __half* to_lo = head.t_lo + tri_block(i, w) + core(2 * t, g);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           split(make_float2(-y[n][2 * half], -y[n][2 * half + 1]), hi[half], lo[half]);
-          const int col = 16 * w + g + 8 * half, row = 16 * i + 8 * n + 2 * t;
           const __half2 h = *reinterpret_cast<const __half2*>(&hi[half]);
           const __half2 l = *reinterpret_cast<const __half2*>(&lo[half]);
-          s.work().image.t_hi[tri(row, col)] = __low2half(h);
-          s.work().image.t_hi[tri(row + 1, col)] = __high2half(h);
-          s.work().image.t_lo[tri(row, col)] = __low2half(l);
-          s.work().image.t_lo[tri(row + 1, col)] = __high2half(l);
+          to_hi[core(8 * n, 8 * half)] = __low2half(h);
+          to_hi[core(8 * n + 1, 8 * half)] = __high2half(h);
+          to_lo[core(8 * n, 8 * half)] = __low2half(l);
+          to_lo[core(8 * n + 1, 8 * half)] = __high2half(l);
         }
         if (d < 3) {
           x_hi[d < 3 ? d : 0][2 * n] = hi[0];
@@ -751,8 +797,7 @@ __device__ __forceinline__ bool find_request(const PrefillArgs& p, int64_t r, Re
 
 // Requests by their chunk counts, longest first (to half an octave), for the chain to take in this order;
 // equal ones in any order.  One CTA.
-__device__ __forceinline__ void order_requests(const PrefillArgs& p, int tid) {
-  __shared__ uint32_t counts[64];
+__device__ __forceinline__ void order_requests(const PrefillArgs& p, uint32_t (&counts)[64], int tid) {
   if (tid < 64) counts[tid] = 0;
   if (tid == 0) *p.next = 0;
   __syncthreads();
@@ -784,7 +829,7 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   allow_dependent_launch();
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   if (blockIdx.x == 0) {
-    order_requests(p, tid);
+    order_requests(p, s.counts, tid);
     return;
   }
   const int64_t place = (blockIdx.x - 1) / p.num_k_heads;
@@ -835,8 +880,9 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
       to[i * kPairThreads + tid] = from[i * kPairThreads + tid];
     }
   }
-  float kk[4][2][4], qk[4][2][4];
-  row_products(s, w, lane, kk, qk);
+  const Blocks mine(w);
+  float kk[3][2][4], qk[3][2][4];
+  row_products(s, mine, lane, kk, qk);
   __syncthreads();
   if (w < 2) {
     const float* f = w == 0 ? s.fk : s.fq;
@@ -849,41 +895,36 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   }
   __syncthreads();
 #pragma unroll 1
-  for (int n = 0; n < p.heads_ratio; ++n) {
+  for (int n = 0; n < p.heads_ratio; n += 2) {
     const int at = n % kGroup;
+    const int heads = min(p.heads_ratio - n, 2);
+    PairImage* images = p.pairs + place * p.num_v_heads + head0 + n;
     if (n > 0) {
-      __syncthreads();  // the image and, every fourth head, the gates are taken over
+      __syncthreads();  // the heads' inverses and, every fourth head, the gates are taken over
       if (at == 0) {
         if (n + w < p.heads_ratio) chunk_gates(p, s, w, token0, row_lo, row_hi, head0 + n + w, lane);
         __syncthreads();
       }
     }
-    if (tid < kChunk) {
-      const float in = exp2_fast(s.g_hi[at][tid] + s.g_lo[at][tid]);
-      s.work().image.beta[tid] = s.beta[at][tid];
-      s.work().image.k_in[tid] = in * s.fk[tid];
-      s.work().image.q_in[tid] = in * s.fq[tid] * p.q_scale;
-      const auto out = [&](int i) {
-        const float left = (s.g_hi[at][kChunk - 1] - s.g_hi[at][i]) + (s.g_lo[at][kChunk - 1] - s.g_lo[at][i]);
-        return exp2_fast(left) * s.fk[i];
-      };
-      const float k_out = out(tid), power = largest_power(k_out, out(tid ^ 32));
-      s.work().image.k_out[tid] = k_out * inverse_power(power);
-      if (tid == kChunk - 1) {
-        s.work().image.decay = in;
-        s.work().image.k_scale = power;
-        s.work().image.p_scale = s.fk_power * s.fq_power;
-      }
-    }
-    decayed_pairs(p, s, at, w, lane, kk, qk);
+    if ((w >> 1) < heads) row_factors(p, s, at + (w >> 1), tid & (kChunk - 1), images[w >> 1]);
+#pragma unroll 1
+    for (int i = 0; i < heads; ++i) decayed_pairs(p, s, s.head(i), at + i, mine, lane, kk, qk, images[i].p);
     __syncwarp();
-    invert_diagonal(s, w, lane);
+    if ((lane >> 4) < heads) invert_diagonal(s.head(lane >> 4), w, lane & 15);
     __syncthreads();
-    invert_column(s, w, lane);
+    // Columns 0, 1 and 2 have 3, 2 and 1 blocks: a warp takes the first, another the other two.
+    if ((w & 1) < heads) {
+      for (int col = w >> 1; col <= (w & 2); ++col) invert_column(s.head(w & 1), col, lane);
+    }
     __syncthreads();
-    uint4* to = reinterpret_cast<uint4*>(p.pairs + place * p.num_v_heads + head0 + n);
-    const uint4* from = reinterpret_cast<const uint4*>(&s.work().image);
-    for (int i = tid; i < static_cast<int>(sizeof(PairImage) / 16); i += kPairThreads) to[i] = from[i];
+#pragma unroll 1
+    for (int i = 0; i < heads; ++i) {
+      uint4* to = reinterpret_cast<uint4*>(images + i);  // t_hi and t_lo come first
+      const uint4* from = reinterpret_cast<const uint4*>(&s.head(i));
+      constexpr int kPieces = 2 * sizeof(PairHead::t_hi) / 16;
+#pragma unroll
+      for (int k = 0; k < kPieces / kPairThreads; ++k) to[k * kPairThreads + tid] = from[k * kPairThreads + tid];
+    }
   }
 }
 
