@@ -45,6 +45,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.h"
 #include "launch.cuh"
@@ -89,6 +90,38 @@ struct __align__(128) PairImage {  // per (chunk, value head)
 };
 static_assert(sizeof(KeyImage) % 16 == 0 && sizeof(PairImage) % 16 == 0, "images are copied 16 bytes at a time");
 
+// Splitting a long prompt.  The chain takes a value head's chunks one after the other, so few requests with few heads
+// leave most SMs idle.  A chunk's step is linear in the state, S <- S M + B, and so is a run of chunks: M is what it
+// makes of the identity with all v taken as zero, B what it makes of zero.  A request in pieces is run in two passes:
+// the first runs piece 0 for good and carries M_k and B_k through each middle piece k, all at once; then
+// S_1 = the end of piece 0 and S_{k+1} = S_k M_k + B_k are joined, and the second pass runs the pieces from 1 on from
+// their states, all at once.  That is three times the work for the middle pieces, in the time of two pieces.
+// With room for `slots` CTAs per value head there are (slots - 1) / 2 middle pieces, and one more of half their length,
+// whose M and B share a CTA, where a slot is left over: 16,384 tokens of one request with 32 value heads (4 slots,
+// 4 pieces, 2 of 3.5 parts of the time) take 739 us, unsplit 1,104.
+struct Pieces {
+  int count;       // 1: no request is split
+  bool half_last;  // the last middle piece has half the length of the others
+
+  // Piece k begins with chunk chunks * cut(k) / cut(count).
+  __host__ __device__ int64_t cut(int k) const { return 2 * k - (half_last && k >= count - 1 ? 1 : 0); }
+  // What the first pass runs per request and value head, a matrix each: piece 0, then M_k and B_k, k = 1 .. count - 2.
+  __host__ __device__ int first_parts() const { return count > 1 ? 2 * count - 3 : 1; }
+};
+
+constexpr int kPieceChunks = 12;  // a whole piece has at least so many: below, two launches more cost what they save
+constexpr int kPiecesMost = 8;
+constexpr int kPieceSms = 148;
+
+Pieces pieces_of(int64_t n_tokens, int64_t n_requests, int64_t num_v_heads) {
+  const int64_t slots = kPieceSms / std::max<int64_t>(n_requests * num_v_heads, 1);
+  const int64_t most = std::min<int64_t>(kPiecesMost, n_tokens / kChunk / kPieceChunks);
+  if (slots < 2 || most < 3) return {1, false};
+  const int64_t whole = 2 + (slots - 1) / 2;
+  if (slots % 2 == 0 && whole < most) return {static_cast<int>(whole + 1), true};
+  return {static_cast<int>(std::min(whole, most)), false};
+}
+
 struct PrefillArgs {
   const __nv_bfloat16* qkv;
   int64_t qkv_row;
@@ -115,7 +148,10 @@ struct PrefillArgs {
   KeyImage* keys;    // [chunk places, num_k_heads]
   PairImage* pairs;  // [chunk places, num_v_heads]
   int32_t* order;    // requests, longest first
-  uint32_t* next;    // items that the chain's CTAs have taken
+  uint32_t* next;    // items that the chain's CTAs have taken, per pass, and whether a wait has run out
+  float* states;     // fp32 states between the pieces of split requests, first_parts() per request and value head
+  Pieces pieces;     // of long requests
+  int pass;          // of the chain kernel: 1 for the pieces that begin with a joined state
   int64_t places;
   int n_requests;
   int num_k_heads;
@@ -145,6 +181,10 @@ struct Request {
   int32_t source;   // state slot to start from (0: from nothing)
   const int32_t* row;
 };
+
+__device__ __forceinline__ bool is_split(const PrefillArgs& p, int64_t chunks) {
+  return p.pieces.count > 1 && chunks >= kPieceChunks * p.pieces.count;
+}
 
 // ------------------------------------------------------------------------------------------
 // instructions
@@ -799,7 +839,7 @@ __device__ __forceinline__ bool find_request(const PrefillArgs& p, int64_t r, Re
 // equal ones in any order.  One CTA.
 __device__ __forceinline__ void order_requests(const PrefillArgs& p, uint32_t (&counts)[64], int tid) {
   if (tid < 64) counts[tid] = 0;
-  if (tid == 0) *p.next = 0;
+  if (tid < 3) p.next[tid] = 0;
   __syncthreads();
   const auto bucket = [&](int r) {
     const int tokens = max(p.cu[r + 1] - p.cu[r], 1);
@@ -939,19 +979,26 @@ struct Work {
   int64_t place;       // the chunk's place in the workspace; kWorkZero: the item's tokens
   int32_t row_lo, row_hi;
   int32_t head;
-  int32_t source;      // -1: the state goes on; else the slot that it starts from (0: from nothing)
+  int32_t source;      // the slot that the state starts from (0: from nothing), or one of these:
+  int32_t matrix;      // kSourceMatrix: the matrix of `states`
+  int32_t save;        // the matrix of `states` that takes the state after the chunk (-1: none)
+  int32_t quiet;       // no outputs
   int32_t slot;        // the slot that takes the state after the chunk (0: none)
   int32_t kind;
 };
+constexpr int kSourceOn = -1, kSourceIdentity = -2, kSourceMatrix = -3;  // the state goes on; identity; a matrix
 constexpr int kWorkChunk = 0, kWorkEnd = 1, kWorkZero = 2;  // a chunk; no more items; an item whose outputs are zeros
 
 // Where the item in work is, kept and used by one thread.
 struct Cursor {
   const int32_t* slot_at;  // the slot of the block that the next chunk is in
-  uint32_t ahead;          // the item after this one, already taken
+  uint32_t ahead;          // the item after this one, taken with this one's last chunk
   int32_t rest;            // tokens behind the upcoming chunk
   int32_t left;            // chunks to the end of the block, the upcoming one not counted
   int32_t per_block;
+  int32_t save;            // the matrix of `states` that takes the item's last state (-1: none)
+  bool last;               // the item ends with its request
+  bool blind;              // no v: every row counts as one of no token
 };
 
 struct __align__(1024) Stage {
@@ -1000,7 +1047,7 @@ __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, cons
 template <bool kVec>
 __device__ __forceinline__ void copy_gates(const PrefillArgs& p, Stage& st, int tid) {
   const Work& d = st.work;
-  if (d.kind == kWorkChunk) {
+  if (d.kind == kWorkChunk && !d.quiet) {
     load_rows<kVec, kMoveThreads>(p.gate + d.token0 * p.gate_row + d.head * kDim, p.gate_row, d.row_lo, d.row_hi,
                                   reinterpret_cast<uint16_t*>(st.gate), tid,
                                   [](int row, int col) { return row * kVRow + col; });
@@ -1041,7 +1088,7 @@ template <bool kVec>
 __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Stage& st, const Work& d,
                                               const float2 (&wt)[4], int tid) {
   const int part = tid & 15;
-  const bool stop = s.stop != 0;
+  const bool stop = s.stop != 0 || d.quiet;
   __nv_bfloat16* out = p.out + (d.token0 * p.num_v_heads + d.head) * kDim + 4 * part;
 #pragma unroll 1
   for (int i = tid >> 4; i < kChunk; i += kMoveThreads / 16) {
@@ -1388,10 +1435,17 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   }
 }
 
-// The slot that takes the state after the upcoming chunk, when a block or the request ends with it.
-__device__ __forceinline__ void work_slot(const PrefillArgs& p, Cursor& at, Work& d) {
+// Where the state goes after the upcoming chunk: to a slot when a block or the request ends with it, and to a matrix
+// when a split request's piece does.
+template <bool kSplit>
+__device__ __forceinline__ void work_ends(const PrefillArgs& p, Cursor& at, Work& d) {
   d.slot = 0;
-  if (at.rest <= 0 || at.left == 0) {
+  if constexpr (kSplit) {
+    d.save = at.rest <= 0 ? at.save : -1;
+    if (at.blind) d.row_lo = d.row_hi = 0;
+  }
+  const bool last = !kSplit || at.last, quiet = kSplit && d.quiet;
+  if (!quiet && (at.left == 0 || (at.rest <= 0 && last))) {
     d.slot = *at.slot_at++;
     at.left = at.per_block;
     if (d.slot >= p.n_slots) {
@@ -1403,36 +1457,61 @@ __device__ __forceinline__ void work_slot(const PrefillArgs& p, Cursor& at, Work
 }
 
 // The first chunk of the next item that has some, the end, or an item whose outputs are zeros.  One thread.
+template <bool kSplit>
 __device__ __noinline__ void next_item(const PrefillArgs& p, Cursor& at, Work& d) {
   const int64_t per_block = p.block_size / kChunk;
+  const uint32_t heads = p.num_v_heads, parts = !kSplit ? 1 : p.pass == 0 ? p.pieces.first_parts() : p.pieces.count - 1;
   while (true) {
     const uint32_t item = at.ahead;
-    if (item >= static_cast<uint32_t>(p.n_requests) * p.num_v_heads) {
+    if (item >= p.n_requests * parts * heads) {
       d.kind = kWorkEnd;
       return;
     }
-    at.ahead = atomicAdd(p.next, 1u);
-    const int r = p.order[item / p.num_v_heads];
-    d.head = static_cast<int>(item % p.num_v_heads);
+    const auto take = [&] { at.ahead = atomicAdd(p.next + p.pass, 1u); };
+    const int part = static_cast<int>(item / heads % parts);
+    const int r = p.order[item / heads / parts];
+    const bool first = !kSplit || (p.pass == 0 && part == 0);
+    d.head = static_cast<int>(item % heads);
     at.rest = 0;
     Request rq;
     unsigned int fault;
     bool skip;
     if (find_request(p, r, rq, fault, skip)) {
+      // Chunks [lo, hi) of the request.
+      const bool split = kSplit && is_split(p, rq.chunks);
+      if (!split && !first) {
+        take();
+        continue;
+      }
+      const int piece = p.pass == 0 ? (part + 1) / 2 : part + 1;
+      const int64_t cuts = p.pieces.cut(p.pieces.count);
+      const int64_t lo = split ? rq.chunks * p.pieces.cut(piece) / cuts : 0;
+      const int64_t hi = split ? rq.chunks * p.pieces.cut(piece + 1) / cuts : rq.chunks;
       // Chunks end at absolute positions that are multiples of 64, and so do blocks.
+      const int64_t position = rq.context / kChunk + lo;
       at.per_block = static_cast<int32_t>(min(per_block, static_cast<int64_t>(INT32_MAX)));
-      at.left = static_cast<int32_t>(min(per_block - 1 - (rq.context / kChunk) % per_block, static_cast<int64_t>(INT32_MAX)));
-      at.slot_at = rq.row + rq.context / p.block_size;
-      at.rest = static_cast<int32_t>(rq.tokens) - (kChunk - rq.lead);
-      d.token0 = rq.first - rq.lead;
-      d.place = chunk_base(rq.first, r);
-      d.row_lo = rq.lead;
+      at.left = static_cast<int32_t>(min(per_block - 1 - position % per_block, static_cast<int64_t>(INT32_MAX)));
+      at.slot_at = rq.row + position / per_block;
+      at.last = hi == rq.chunks;
+      const int64_t before = lo * kChunk - rq.lead;  // tokens in front of row 0
+      at.rest = static_cast<int32_t>((at.last ? rq.tokens : hi * kChunk - rq.lead) - before - kChunk);
+      const int32_t matrices = static_cast<int32_t>(r * heads + d.head) * p.pieces.first_parts();
+      at.save = split && p.pass == 0 ? matrices + part : -1;
+      at.blind = p.pass == 0 && (part & 1) != 0;
+      d.quiet = p.pass == 0 && part != 0;
+      d.token0 = rq.first + before;
+      d.place = chunk_base(rq.first, r) + lo;
+      d.row_lo = lo == 0 ? rq.lead : 0;
       d.row_hi = kChunk + min(at.rest, 0);
-      d.source = rq.source;
+      d.source = first ? rq.source : p.pass != 0 ? kSourceMatrix : at.blind ? kSourceIdentity : 0;
+      d.matrix = matrices + 2 * part;  // S_1 is where piece 0 left it, S_{k+1} in the place of B_k
       d.kind = kWorkChunk;
-      work_slot(p, at, d);
+      work_ends<kSplit>(p, at, d);
+      if (at.rest <= 0) take();
       return;
     }
+    take();
+    if (!first) continue;
     if (fault != 0 && d.head == 0) atomicOr(&g_prefill_faults, fault);
     if (!skip) {
       d.token0 = rq.first;
@@ -1444,18 +1523,20 @@ __device__ __noinline__ void next_item(const PrefillArgs& p, Cursor& at, Work& d
 }
 
 // The upcoming work after the one in `d`.  One thread.
+template <bool kSplit>
 __device__ __forceinline__ void next_work(const PrefillArgs& p, Cursor& at, Work& d) {
   if (at.rest <= 0) {
-    next_item(p, at, d);
+    next_item<kSplit>(p, at, d);
     return;
   }
   d.token0 += kChunk;
   d.place += 1;
   d.row_lo = 0;
   d.row_hi = min(at.rest, kChunk);
-  d.source = -1;
+  d.source = kSourceOn;
   at.rest -= kChunk;
-  work_slot(p, at, d);
+  work_ends<kSplit>(p, at, d);
+  if (at.rest <= 0) at.ahead = atomicAdd(p.next + p.pass, 1u);
 }
 
 // Writes the zero outputs of upcoming items that cannot run, until a chunk or the end is next.  The moving
@@ -1468,11 +1549,12 @@ __device__ __noinline__ void zero_item(const PrefillArgs& p, const Work& d, int 
   }
 }
 
+template <bool kSplit>
 __device__ __forceinline__ void skip_items(const PrefillArgs& p, ChainSmem& s, int tid) {
   while (s.upcoming.kind == kWorkZero) {
     zero_item(p, s.upcoming, tid);
     bar_move();
-    if (tid == 0) next_item(p, s.at, s.upcoming);
+    if (tid == 0) next_item<kSplit>(p, s.at, s.upcoming);
     bar_move();
   }
 }
@@ -1493,11 +1575,9 @@ __device__ __forceinline__ void load_stage(const PrefillArgs& p, Stage& st, cons
 
 // A persistent CTA per SM: the moving threads take items (a request's value head each), longest first, and
 // feed their chunks through two stages without a gap between items.
-template <typename StateT, bool kVec>
+template <typename StateT, bool kVec, bool kSplit>
 __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(const __grid_constant__ PrefillArgs p) {
   ChainSmem& s = *reinterpret_cast<ChainSmem*>(chain_raw);
-  grid_dependency_wait();
-  allow_dependent_launch();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kStateWarp = kMoveThreads / 32;
 
@@ -1521,22 +1601,26 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     if (tid == 0) {
       for (int i = 0; i < 2; ++i) barrier_init(full(i));
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      s.at.ahead = atomicAdd(p.next, 1u);
+    }
+    grid_dependency_wait();
+    allow_dependent_launch();
+    if (tid == 0) {
+      s.at.ahead = atomicAdd(p.next + p.pass, 1u);
       s.at.rest = 0;
-      next_item(p, s.at, s.upcoming);
+      next_item<kSplit>(p, s.at, s.upcoming);
     }
     __syncthreads();  // the barriers are there
     bool more = true;
 #pragma unroll 1
     for (int stage = 0; stage < 2 && more; ++stage) {
-      skip_items(p, s, tid);
+      skip_items<kSplit>(p, s, tid);
       load_stage<StateT, kVec>(p, s.stage[stage], s.upcoming, full(stage), tid, late);
       cp_async_commit();
       more = s.upcoming.kind == kWorkChunk;
       bar_move();
       copy_gates<kVec>(p, s.stage[stage], tid);
       cp_async_commit();
-      if (stage == 0 && more && tid == 0) next_work(p, s.at, s.upcoming);
+      if (stage == 0 && more && tid == 0) next_work<kSplit>(p, s.at, s.upcoming);
       __syncwarp();
       hand_over(stage, more);
       bar_move();
@@ -1555,7 +1639,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       const Work d = st.work;
       if (d.kind == kWorkEnd) break;
       const bool refill = more;
-      if (refill && tid == 0) next_work(p, s.at, s.upcoming);  // while the chain is at work
+      if (refill && tid == 0) next_work<kSplit>(p, s.at, s.upcoming);  // while the chain is at work
       __syncwarp();
       bar_sync(kBarChunkDone);
       if (warp == 0) {
@@ -1570,7 +1654,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       bar_move();  // the tile is whole, the stage read for the last time, the upcoming work known
       if (s.stage[stage ^ 1].work.kind == kWorkChunk) bar_arrive(kBarTaken);
       if (refill) {
-        skip_items(p, s, tid);
+        skip_items<kSplit>(p, s, tid);
         load_stage<StateT, kVec>(p, st, s.upcoming, full(stage), tid, late);
         more = s.upcoming.kind == kWorkChunk;
       }
@@ -1595,13 +1679,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
       if (lane == 0) {
-        s.stop = 0;
         for (int i = 0; i < 2; ++i) barrier_init(smem_u32(&s.done[i]));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       }
       __syncwarp();
       tmem_before();
     }
+    grid_dependency_wait();
+    if (issuer && lane == 0) s.stop = p.pass == 0 ? 0 : static_cast<int>(p.next[2]);  // ran out in the first pass
     __syncthreads();  // the barriers are there
     tmem_after();
     const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
@@ -1614,20 +1699,44 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       bar_sync(kBarFull + stage);
       if (st.work.kind == kWorkEnd) break;
       const int32_t source = st.work.source, slot = st.work.slot;
-      StateT* pool = static_cast<StateT*>(p.state) + static_cast<int64_t>(st.work.head) * kDim * kDim +
-                     (v0 + g) * kDim + 2 * t;
-      if (source > 0) {
-        const StateT* at = pool + source * p.slot_stride;
+      [[maybe_unused]] int32_t save = st.work.save;
+      const int64_t element = (v0 + g) * kDim + 2 * t;
+      const auto pool_at = [&](int32_t i) {
+        return static_cast<StateT*>(p.state) + i * p.slot_stride + static_cast<int64_t>(st.work.head) * kDim * kDim + element;
+      };
+      const auto matrix_at = [&](int32_t i) { return p.states + static_cast<int64_t>(i) * kDim * kDim + element; };
+      const auto load = [&](const auto* at) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           load_pair(at + 8 * i, x.S[i][0], x.S[i][1]);
           load_pair(at + 8 * kDim + 8 * i, x.S[i][2], x.S[i][3]);
         }
-      } else if (source == 0) {
+      };
+      const auto store = [&](auto* at) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          store_pair(at + 8 * i, x.S[i][0], x.S[i][1]);
+          store_pair(at + 8 * kDim + 8 * i, x.S[i][2], x.S[i][3]);
+        }
+      };
+      // Where the pool has the matrices' type they share its code: instructions are what the chain's warps compete for.
+      constexpr bool kShared = kSplit && std::is_same<StateT, float>::value;
+      if (source > 0 || (kShared && source == kSourceMatrix)) {
+        if constexpr (kShared) {
+          load(source > 0 ? pool_at(source) : matrix_at(st.work.matrix));
+        } else {
+          load(pool_at(source));
+        }
+      } else if (kSplit && !kShared && source == kSourceMatrix) {
+        load(matrix_at(st.work.matrix));
+      } else if (source != kSourceOn) {  // zeros, or the identity
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x.S[i][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) {
+            const bool one = kSplit && source == kSourceIdentity && v0 + g + 8 * (e >> 1) == 8 * i + 2 * t + (e & 1);
+            x.S[i][e] = one ? 1.0f : 0.0f;
+          }
         }
       }
       chain_chunk(x, s, stage, tmem, v0, lane, issuer, p.wait_ns, [&] {
@@ -1637,22 +1746,95 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         }
       });
       bar_arrive(kBarChunkDone);
-      if (slot > 0 && s.stop == 0) {
-        StateT* at = pool + slot * p.slot_stride;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          store_pair(at + 8 * i, x.S[i][0], x.S[i][1]);
-          store_pair(at + 8 * kDim + 8 * i, x.S[i][2], x.S[i][3]);
+      const bool to_pool = slot > 0 && s.stop == 0;
+      if constexpr (kShared) {
+        float* at = to_pool ? pool_at(slot) : nullptr;
+#pragma unroll 1
+        while (at != nullptr || save >= 0) {
+          if (at == nullptr) {
+            at = matrix_at(save);
+            save = -1;
+          }
+          store(at);
+          at = nullptr;
         }
+      } else {
+        if (to_pool) store(pool_at(slot));
+        if (kSplit && save >= 0) store(matrix_at(save));
       }
     }
   }
   // Everybody has taken what it needs from TMEM.
   tmem_before();
   __syncthreads();
+  if (threadIdx.x == 0 && s.stop != 0) p.next[2] = 1;
   if (warp == kStateWarp) {
     tmem_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(kTmemColumns));
+  }
+}
+
+// S_{k+1} = S_k M_k + B_k for a split request's value head, 32 rows of S per CTA, which takes them through all its pieces.
+constexpr int kJoinRows = 32, kJoinThreads = 256;
+struct JoinSmem {
+  __align__(16) float m[kDim * kDim];
+  __align__(16) float rows[kJoinRows * kDim];
+};
+
+__global__ void __launch_bounds__(kJoinThreads) gdn_prefill_join_kernel(const __grid_constant__ PrefillArgs p) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  JoinSmem& s = *reinterpret_cast<JoinSmem*>(raw);
+  grid_dependency_wait();
+  allow_dependent_launch();
+  constexpr int kBlocks = kDim / kJoinRows;
+  const int item = blockIdx.x / kBlocks, row0 = static_cast<int>(blockIdx.x % kBlocks) * kJoinRows;
+  Request rq;
+  unsigned int fault;
+  bool skip;
+  if (!find_request(p, item / p.num_v_heads, rq, fault, skip) || !is_split(p, rq.chunks)) return;
+  float* states = p.states + static_cast<int64_t>(item) * p.pieces.first_parts() * kDim * kDim;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < kJoinRows * kDim / 4; i += kJoinThreads) {
+    reinterpret_cast<float4*>(s.rows)[i] = reinterpret_cast<const float4*>(states + row0 * kDim)[i];
+  }
+  const int col = 4 * (tid & 31), row = 4 * (tid >> 5);  // 4 x 4 results a thread
+  for (int k = 1; k < p.pieces.count - 1; ++k) {
+    const float4* m = reinterpret_cast<const float4*>(states + (2 * k - 1) * kDim * kDim);
+    float* b = states + 2 * k * kDim * kDim + (row0 + row) * kDim + col;
+#pragma unroll 8
+    for (int i = 0; i < kDim * kDim / 4 / kJoinThreads; ++i) {
+      reinterpret_cast<float4*>(s.m)[i * kJoinThreads + tid] = m[i * kJoinThreads + tid];
+    }
+    float4 sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = *reinterpret_cast<const float4*>(b + i * kDim);
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < kDim; j += 4) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = *reinterpret_cast<const float4*>(&s.rows[(row + i) * kDim + j]);
+        y[i] = *reinterpret_cast<const float4*>(&s.m[(j + i) * kDim + col]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          sum[i].x = fmaf(f[n], y[n].x, sum[i].x);
+          sum[i].y = fmaf(f[n], y[n].y, sum[i].y);
+          sum[i].z = fmaf(f[n], y[n].z, sum[i].z);
+          sum[i].w = fmaf(f[n], y[n].w, sum[i].w);
+        }
+      }
+    }
+    __syncthreads();  // rows and M have been read
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<float4*>(b + i * kDim) = sum[i];
+      *reinterpret_cast<float4*>(&s.rows[(row + i) * kDim + col]) = sum[i];
+    }
   }
 }
 
@@ -1660,14 +1842,23 @@ bool aligned(const void* ptr, uintptr_t bytes) { return (reinterpret_cast<uintpt
 
 int64_t chunk_places(int64_t n_tokens, int64_t n_requests) { return chunk_base(n_tokens, n_requests); }
 
-// The workspace: key images, pair images, then the requests' order and the count of items taken.
+// The workspace: key images, pair images, the chain's counters and the requests' order, then split requests' states.
 int64_t order_offset(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads) {
   return chunk_places(n_tokens, n_requests) * (num_k_heads * static_cast<int64_t>(sizeof(KeyImage)) +
                                                num_v_heads * static_cast<int64_t>(sizeof(PairImage)));
 }
 
+constexpr int kCounters = 3;
+
+int64_t states_offset(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads) {
+  return (order_offset(n_tokens, n_requests, num_k_heads, num_v_heads) + 4 * (n_requests + kCounters) + 127) / 128 * 128;
+}
+
 int64_t workspace_bytes(int64_t n_tokens, int64_t n_requests, int64_t num_k_heads, int64_t num_v_heads) {
-  return order_offset(n_tokens, n_requests, num_k_heads, num_v_heads) + 4 * (n_requests + 1);
+  const Pieces pieces = pieces_of(n_tokens, n_requests, num_v_heads);
+  const int64_t matrices = pieces.count > 1 ? n_requests * num_v_heads * pieces.first_parts() : 0;
+  return states_offset(n_tokens, n_requests, num_k_heads, num_v_heads) +
+         matrices * kDim * kDim * static_cast<int64_t>(sizeof(float));
 }
 
 // Streaming multiprocessors of the current device, asked once per device.
@@ -1687,20 +1878,32 @@ int sm_count(int& sms) {
 }
 
 template <typename StateT, bool kVec>
-cudaError_t launch_prefill(const PrefillArgs& args, int sms, cudaStream_t stream) {
+cudaError_t launch_prefill(PrefillArgs& args, int sms, cudaStream_t stream) {
   // Set on every call: the attributes belong to the current device, and setting them is a table write.
   auto pairs = gdn_prefill_pairs_kernel<kVec>;
   cudaError_t err = cudaFuncSetAttribute(pairs, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairSmem));
   if (err != cudaSuccess) return err;
-  auto chain = gdn_prefill_chain_kernel<StateT, kVec>;
+  const auto chain = args.pieces.count > 1 ? gdn_prefill_chain_kernel<StateT, kVec, true> : gdn_prefill_chain_kernel<StateT, kVec, false>;
   err = cudaFuncSetAttribute(chain, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ChainSmem));
   if (err != cudaSuccess) return err;
   err = launch(pairs, dim3(static_cast<unsigned int>(1 + args.places * args.num_k_heads)), dim3(kPairThreads),
                sizeof(PairSmem), stream, 1, args);
   if (err != cudaSuccess) return err;
-  const int64_t items = static_cast<int64_t>(args.n_requests) * args.num_v_heads;
-  return launch(chain, dim3(static_cast<unsigned int>(std::min<int64_t>(items, sms))), dim3(kChainThreads),
-                sizeof(ChainSmem), stream, 1, args);
+  const int64_t heads = static_cast<int64_t>(args.n_requests) * args.num_v_heads;
+  const auto run_chain = [&](int64_t items) {
+    return launch(chain, dim3(static_cast<unsigned int>(std::min<int64_t>(items, sms))), dim3(kChainThreads),
+                  sizeof(ChainSmem), stream, 1, args);
+  };
+  args.pass = 0;
+  err = run_chain(heads * args.pieces.first_parts());
+  if (err != cudaSuccess || args.pieces.count == 1) return err;
+  err = cudaFuncSetAttribute(gdn_prefill_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(JoinSmem));
+  if (err != cudaSuccess) return err;
+  err = launch(gdn_prefill_join_kernel, dim3(static_cast<unsigned int>(heads * (kDim / kJoinRows))), dim3(kJoinThreads),
+               sizeof(JoinSmem), stream, 1, args);
+  if (err != cudaSuccess) return err;
+  args.pass = 1;
+  return run_chain(heads * (args.pieces.count - 1));
 }
 
 }  // namespace
@@ -1810,7 +2013,10 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   args.pairs = reinterpret_cast<PairImage*>(args.keys + chunk_places(n_tokens, n_requests) * num_k_heads);
   unsigned char* order = static_cast<unsigned char*>(workspace) + order_offset(n_tokens, n_requests, num_k_heads, num_v_heads);
   args.next = reinterpret_cast<uint32_t*>(order);
-  args.order = reinterpret_cast<int32_t*>(order) + 1;
+  args.order = reinterpret_cast<int32_t*>(order) + kCounters;
+  args.pieces = pieces_of(n_tokens, n_requests, num_v_heads);
+  args.states = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+                                         states_offset(n_tokens, n_requests, num_k_heads, num_v_heads));
   args.places = chunk_places(n_tokens, n_requests);
   args.n_requests = static_cast<int>(n_requests);
   args.num_k_heads = static_cast<int>(num_k_heads);

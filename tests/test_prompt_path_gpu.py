@@ -230,6 +230,49 @@ def test_prefill_offsets_out_of_range_skip_the_request(cu, faults):
     case.check(faults=faults)
 
 
+@pytest.mark.parametrize("lens,contexts,heads,block,pool", [
+    ([2500], [70], (1, 2), 64, torch.float32),
+    ([6200], [0], (1, 1), 128, torch.bfloat16),
+    ([7000, 100, 0, 300], [64, 3, 0, 64], (1, 2), 64, torch.float32),
+    ([3100, 3100], [100, 0], (2, 12), 1024, torch.float32),
+    ([2700], [1000], (1, 37), 64, torch.float32),
+])
+def test_prefill_long_prompts_in_pieces_at_once(lens, contexts, heads, block, pool):
+    """Long prompts of few heads, which run in pieces side by side whose states are joined, beside short ones."""
+    Prompt(lens, contexts, *heads, block=block, pool=pool, seed=len(lens)).check()
+
+
+def test_prefill_long_prompts_that_cannot_run_or_keep_nothing():
+    """Pieces of a request with a null source give zeros and raise nothing, and blocks without a slot are not stored."""
+    case = Prompt([2400, 2400], [64, 0], h=1, hv=2, seed=41)
+    case.table[0, 0] = 0
+    case.table[1, ::2] = 0
+    case.check()
+    case = Prompt([2400], [64], h=1, hv=2, seed=42)
+    case.table[0, 0] = case.slots
+    case.check(faults=capi.LD_FAULT_DECODE_SLOT_RANGE)
+
+
+def test_prefill_long_prompt_repeats_and_stops():
+    """Bit for bit, and a wait that runs out in the first pass keeps the second from storing anything."""
+    results = []
+    for _ in range(2):
+        case = Prompt([3000], [30], h=1, hv=2, seed=43)
+        case.run()
+        torch.cuda.synchronize()
+        results.append((bits(case.out), case.state.cpu().numpy().view(np.uint32)))
+    assert np.array_equal(results[0][0], results[1][0]) and np.array_equal(results[0][1], results[1][1])
+    before, out = case.state.clone(), case.out.clone()
+    capi.set_decode_wait_test(200_000, 64)
+    try:
+        case.run()
+        torch.cuda.synchronize()
+    finally:
+        capi.set_decode_wait_test()
+    assert capi.fault_flags() == capi.LD_FAULT_WAIT_TIMEOUT
+    assert torch.equal(case.state, before) and torch.equal(case.out, out)
+
+
 def test_prefill_many_requests():
     """Single tokens and empty requests by the hundred, in an order that the queue of items changes."""
     lens = [(7 * i) % 3 for i in range(300)]
