@@ -98,7 +98,8 @@ static_assert(sizeof(KeyImage) % 16 == 0 && sizeof(PairImage) % 16 == 0, "images
 // their states, all at once.  That is three times the work for the middle pieces, in the time of two pieces.
 // With room for `slots` CTAs per value head there are (slots - 1) / 2 middle pieces, and one more of half their length,
 // whose M and B share a CTA, where a slot is left over: 16,384 tokens of one request with 32 value heads (4 slots,
-// 4 pieces, 2 of 3.5 parts of the time) take 739 us, unsplit 1,104.
+// 4 pieces, 2 of 3.5 parts of the chain's time) take 732 us, unsplit 1,104; with 4 value heads (16 pieces) 215 instead of
+// 1,010, and 1,600 tokens with 8 value heads 91 instead of 122.
 struct Pieces {
   int count;       // 1: no request is split
   bool half_last;  // the last middle piece has half the length of the others
@@ -109,17 +110,24 @@ struct Pieces {
   __host__ __device__ int first_parts() const { return count > 1 ? 2 * count - 3 : 1; }
 };
 
-constexpr int kPieceChunks = 12;  // a whole piece has at least so many: below, two launches more cost what they save
-constexpr int kPiecesMost = 8;
+constexpr int kPieceChunks = 5;   // a whole piece has at least so many: every piece adds 2 us to the joins
+constexpr int kSavedChunks = 10;  // chunk times that splitting saves at least: the launches cost about nine
+constexpr int kPiecesMost = 16;
 constexpr int kPieceSms = 148;
 
+// Splitting pays for a request of so many chunks: 2 whole pieces' time, 4 of cut's units, instead of all.
+__host__ __device__ __forceinline__ bool worth_splitting(const Pieces& pieces, int64_t chunks) {
+  const int64_t units = pieces.cut(pieces.count);
+  return pieces.count > 1 && chunks >= kPieceChunks * pieces.count && chunks * (units - 4) >= kSavedChunks * units;
+}
+
 Pieces pieces_of(int64_t n_tokens, int64_t n_requests, int64_t num_v_heads) {
-  const int64_t slots = kPieceSms / std::max<int64_t>(n_requests * num_v_heads, 1);
-  const int64_t most = std::min<int64_t>(kPiecesMost, n_tokens / kChunk / kPieceChunks);
+  const int64_t slots = kPieceSms / std::max<int64_t>(n_requests * num_v_heads, 1), chunks = n_tokens / kChunk;
+  const int64_t most = std::min<int64_t>(kPiecesMost, chunks / kPieceChunks), whole = 2 + (slots - 1) / 2;
   if (slots < 2 || most < 3) return {1, false};
-  const int64_t whole = 2 + (slots - 1) / 2;
-  if (slots % 2 == 0 && whole < most) return {static_cast<int>(whole + 1), true};
-  return {static_cast<int>(std::min(whole, most)), false};
+  const bool half = slots % 2 == 0 && whole < most;
+  const Pieces pieces{static_cast<int>(half ? whole + 1 : std::min(whole, most)), half};
+  return worth_splitting(pieces, chunks) ? pieces : Pieces{1, false};
 }
 
 struct PrefillArgs {
@@ -181,10 +189,6 @@ struct Request {
   int32_t source;   // state slot to start from (0: from nothing)
   const int32_t* row;
 };
-
-__device__ __forceinline__ bool is_split(const PrefillArgs& p, int64_t chunks) {
-  return p.pieces.count > 1 && chunks >= kPieceChunks * p.pieces.count;
-}
 
 // ------------------------------------------------------------------------------------------
 // instructions
@@ -1478,7 +1482,7 @@ __device__ __noinline__ void next_item(const PrefillArgs& p, Cursor& at, Work& d
     bool skip;
     if (find_request(p, r, rq, fault, skip)) {
       // Chunks [lo, hi) of the request.
-      const bool split = kSplit && is_split(p, rq.chunks);
+      const bool split = kSplit && worth_splitting(p.pieces, rq.chunks);
       if (!split && !first) {
         take();
         continue;
@@ -1774,67 +1778,65 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
   }
 }
 
-// S_{k+1} = S_k M_k + B_k for a split request's value head, 32 rows of S per CTA, which takes them through all its pieces.
-constexpr int kJoinRows = 32, kJoinThreads = 256;
-struct JoinSmem {
-  __align__(16) float m[kDim * kDim];
-  __align__(16) float rows[kJoinRows * kDim];
-};
+// S_{k+1} = S_k M_k + B_k for a split request's value head, 8 rows of S per CTA, which takes them through all its pieces.
+// A warp multiplies 16 columns of S_k by M_k's rows of their numbers, which it alone reads and which go from global
+// memory to registers while the piece before is at work; the warps' partial sums meet in shared memory.
+constexpr int kJoinRows = 8, kJoinThreads = 256;
 
 __global__ void __launch_bounds__(kJoinThreads) gdn_prefill_join_kernel(const __grid_constant__ PrefillArgs p) {
-  extern __shared__ __align__(1024) unsigned char raw[];
-  JoinSmem& s = *reinterpret_cast<JoinSmem*>(raw);
+  constexpr int kWarps = kJoinThreads / 32, kDepth = kDim / kWarps, kBlocks = kDim / kJoinRows;
+  __shared__ __align__(16) float rows[kJoinRows][kDim];
+  __shared__ __align__(16) float4 part[kWarps][kJoinRows][32];
+  static_assert(kWarps == kJoinRows, "the warps add up a row each");
   grid_dependency_wait();
   allow_dependent_launch();
-  constexpr int kBlocks = kDim / kJoinRows;
   const int item = blockIdx.x / kBlocks, row0 = static_cast<int>(blockIdx.x % kBlocks) * kJoinRows;
   Request rq;
   unsigned int fault;
   bool skip;
-  if (!find_request(p, item / p.num_v_heads, rq, fault, skip) || !is_split(p, rq.chunks)) return;
+  if (!find_request(p, item / p.num_v_heads, rq, fault, skip) || !worth_splitting(p.pieces, rq.chunks)) return;
   float* states = p.states + static_cast<int64_t>(item) * p.pieces.first_parts() * kDim * kDim;
-  const int tid = threadIdx.x;
-  for (int i = tid; i < kJoinRows * kDim / 4; i += kJoinThreads) {
-    reinterpret_cast<float4*>(s.rows)[i] = reinterpret_cast<const float4*>(states + row0 * kDim)[i];
-  }
-  const int col = 4 * (tid & 31), row = 4 * (tid >> 5);  // 4 x 4 results a thread
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto matrix = [&](int i, int row) { return reinterpret_cast<float4*>(states + (i * kDim + row) * kDim) + lane; };
+  reinterpret_cast<float4*>(rows[w])[lane] = *matrix(0, row0 + w);
+  float4 m[kDepth], b = *matrix(2, row0 + w);
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) m[i] = *matrix(1, kDepth * w + i);
+  __syncthreads();
   for (int k = 1; k < p.pieces.count - 1; ++k) {
-    const float4* m = reinterpret_cast<const float4*>(states + (2 * k - 1) * kDim * kDim);
-    float* b = states + 2 * k * kDim * kDim + (row0 + row) * kDim + col;
-#pragma unroll 8
-    for (int i = 0; i < kDim * kDim / 4 / kJoinThreads; ++i) {
-      reinterpret_cast<float4*>(s.m)[i * kJoinThreads + tid] = m[i * kJoinThreads + tid];
-    }
-    float4 sum[4];
+    float4 sum[kJoinRows];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = *reinterpret_cast<const float4*>(b + i * kDim);
+    for (int r = 0; r < kJoinRows; ++r) {
+      sum[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        const float x = rows[r][kDepth * w + i];
+        sum[r].x = fmaf(x, m[i].x, sum[r].x);
+        sum[r].y = fmaf(x, m[i].y, sum[r].y);
+        sum[r].z = fmaf(x, m[i].z, sum[r].z);
+        sum[r].w = fmaf(x, m[i].w, sum[r].w);
+      }
+    }
+    float4 total = b;
+    if (k + 1 < p.pieces.count - 1) {
+      b = *matrix(2 * k + 2, row0 + w);
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) m[i] = *matrix(2 * k + 1, kDepth * w + i);
+    }
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r) part[w][r][lane] = sum[r];
     __syncthreads();
-#pragma unroll 4
-    for (int j = 0; j < kDim; j += 4) {
-      float4 x[4], y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = *reinterpret_cast<const float4*>(&s.rows[(row + i) * kDim + j]);
-        y[i] = *reinterpret_cast<const float4*>(&s.m[(j + i) * kDim + col]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          sum[i].x = fmaf(f[n], y[n].x, sum[i].x);
-          sum[i].y = fmaf(f[n], y[n].y, sum[i].y);
-          sum[i].z = fmaf(f[n], y[n].z, sum[i].z);
-          sum[i].w = fmaf(f[n], y[n].w, sum[i].w);
-        }
-      }
+    for (int i = 0; i < kWarps; ++i) {
+      const float4 x = part[i][w][lane];
+      total.x += x.x;
+      total.y += x.y;
+      total.z += x.z;
+      total.w += x.w;
     }
-    __syncthreads();  // rows and M have been read
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<float4*>(b + i * kDim) = sum[i];
-      *reinterpret_cast<float4*>(&s.rows[(row + i) * kDim + col]) = sum[i];
-    }
+    *matrix(2 * k, row0 + w) = total;
+    reinterpret_cast<float4*>(rows[w])[lane] = total;
+    __syncthreads();
   }
 }
 
@@ -1897,10 +1899,8 @@ cudaError_t launch_prefill(PrefillArgs& args, int sms, cudaStream_t stream) {
   args.pass = 0;
   err = run_chain(heads * args.pieces.first_parts());
   if (err != cudaSuccess || args.pieces.count == 1) return err;
-  err = cudaFuncSetAttribute(gdn_prefill_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(JoinSmem));
-  if (err != cudaSuccess) return err;
   err = launch(gdn_prefill_join_kernel, dim3(static_cast<unsigned int>(heads * (kDim / kJoinRows))), dim3(kJoinThreads),
-               sizeof(JoinSmem), stream, 1, args);
+               0, stream, 1, args);
   if (err != cudaSuccess) return err;
   args.pass = 1;
   return run_chain(heads * (args.pieces.count - 1));

@@ -66,8 +66,8 @@ def test_prefill_workspace_size(native):
     size = native.prefill_workspace
     assert size(64, 1, 16, 32) < size(6400, 1, 16, 32) < size(6400, 100, 16, 32) < size(6400, 100, 16, 48)
     # Per chunk: q and k of a key head (32 KiB), triangular factors of a value head (16.1 KiB); requests share chunks
-    # at most at two places each.  One head's long prompt runs in 8 pieces with 13 states of 64 KiB between them.
-    assert size(64 * 1000, 1, 1, 1) <= 1002 * (32768 + 16640) + 13 * 65536 + 256
+    # at most at two places each.  One head's long prompt runs in 16 pieces with 29 states of 64 KiB between them.
+    assert size(64 * 1000, 1, 1, 1) <= 1002 * (32768 + 16640) + 29 * 65536 + 256
     assert size(64 * 1000, 1, 1, 149) <= 1002 * (32768 + 149 * 16640) + 256
     for bad in ((-1, 1, 1, 1), (1, -1, 1, 1), (1, 1, 0, 1), (1, 1, 1, 1 << 20)):
         with pytest.raises(native.LightDeltaError):
