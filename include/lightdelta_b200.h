@@ -243,7 +243,8 @@ int ld_decode_kernel_override(int variant);
  * issued and returns.  extra_tx_bytes > 0 (at most 1024) makes every state load announce that many
  * bytes more than it copies, so the waits for it run out although every copy lands: a launch then
  * changes no pool slot and no output of a request it runs.  ld_prefill's waits and copies take both
- * settings too, with the same effect.  Settings apply to launches made after the call.  Returns LD_OK, or LD_ERR_INVALID for arguments out of range.
+ * settings too, with the same effect.  Settings apply to launches made after the call.  Returns LD_OK,
+ * or LD_ERR_INVALID for arguments out of range.
  */
 int ld_decode_wait_test(int64_t limit_ns, int32_t extra_tx_bytes);
 
@@ -377,6 +378,14 @@ int ld_decode_packed_noalloc(const void* qkv, int64_t qkv_row_stride, const void
  * [0, n_tokens) skip the request (LD_FAULT_DECODE_TOKENS).  A destination slot >= n_slots is not
  * written (LD_FAULT_DECODE_SLOT_RANGE).  A token whose inputs are not finite spoils its request
  * from the start of its chunk (positions are cut into chunks at multiples of LD_PREFILL_CHUNK).
+ * An in-kernel wait that runs out (LD_FAULT_WAIT_TIMEOUT) leaves what its CTA has not stored yet as it
+ * was, as in ld_decode.
+ *
+ * Products take fp16 operands with fp32 sums: two terms each (22 bits) on the way to the state, which
+ * so follows the fp32 recurrence to a few 1e-7 of a state row's largest value, and one term (11 bits)
+ * for what only reaches the bf16 outputs.  Results do not depend on the order of execution, but their
+ * last bits may on n_requests and n_tokens: few long prompts of few heads run in pieces whose states
+ * are joined.
  */
 int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a_row_stride, const void* b,
                int64_t b_row_stride, const float* a_log, const void* dt_bias, int dt_bias_dtype, const int32_t* table,
@@ -388,7 +397,7 @@ int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a
 
 /*
  * Bytes of device memory that ld_prefill needs as `workspace` (128-byte aligned) for a call of these sizes:
- * about 16 KiB per token at 16 key and 32 value heads.  It is written and read by the call alone, needs no
+ * about 16 KiB per token at 16 key and 32 value heads, and up to 10 MiB for prompts in pieces.  It is written and read by the call alone, needs no
  * clearing, and may be used again by work behind the call on the same stream; calls that may overlap (other
  * streams, graphs that run side by side) need one each.  Negative: -LD_ERR_INVALID.
  */
