@@ -397,7 +397,7 @@ int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a
 
 /*
  * Bytes of device memory that ld_prefill needs as `workspace` (128-byte aligned) for a call of these sizes:
- * about 16 KiB per token at 16 key and 32 value heads, and up to 10 MiB for prompts in pieces.  It is written and read by the call alone, needs no
+ * about 16 KiB per token at 16 key and 32 value heads, and up to 15 MiB for prompts in pieces.  It is written and read by the call alone, needs no
  * clearing, and may be used again by work behind the call on the same stream; calls that may overlap (other
  * streams, graphs that run side by side) need one each.  Negative: -LD_ERR_INVALID.
  */

@@ -10,12 +10,12 @@
 //
 // One pass bound by HBM: 2 bytes read and 2 written per (token, channel).  A thread owns 4 channels of a
 // tile of consecutive tokens, whatever requests they belong to, and slides the window along, so a tile
-// reads w - 1 rows beyond its own; rows come in batches of 8 loads before the first is used, and a whole
-// batch is straight code.  Six CTAs on an SM (80 registers a thread) keep enough batches in flight: 24
-// prompts of 16,000 tokens in all with 8,192 channels take 108.7 us, 4.84 TB/s; without that bound (96
-// registers, five CTAs) 124 us, with seven or eight and spills 120 and 125, and batches of 4 rows at eight
-// CTAs 111.  8 channels a thread took 222 registers and 299 us.  What is left is instructions: silu's two
-// special-function operations per value and the tile's start.
+// reads w - 1 rows beyond its own.  Rows come in batches of 8, a batch's loads while the one before is at
+// work, and a whole batch is straight code.  24 prompts of 16,000 tokens in all with 8,192 channels take
+// 97.8 us, 5.4 TB/s, at six CTAs on an SM (80 registers a thread); five (96 registers) take 101.4, four
+// 103.3, batches of 4 rows at eight CTAs 101.  Without loads ahead six CTAs took 108.5 and five 124; 8
+// channels a thread took 222 registers and 299 us.  What is left is instructions, silu's two
+// special-function operations per value above all, and the tile's start.
 // A request's first w - 1 tokens all go to the thread that has its first one: only that thread reads the
 // history, so it can also write the slot when a request goes on inside a block and its source slot is
 // its first destination.
@@ -167,47 +167,72 @@ __device__ __forceinline__ Row<kVec> earlier(const ConvPrefillArgs& p, const Pla
   return load_window<kVec>(p, at.source, channel, static_cast<int>(kWidth - 1 + (i - at.begin)));
 }
 
-// Outputs of `count` tokens, whose loads go out together, and the window behind them.  A full batch is straight code
-// in which every input is unpacked once.
-template <int kVec, int kWidth, bool kFull>
-__device__ __forceinline__ void convolve(const __nv_bfloat16* x, int64_t x_row, __nv_bfloat16* out, int64_t out_row,
-                                         int count, const float2 (&wt)[kWidth][Row<kVec>::kWords],
-                                         const float2 (&bias)[Row<kVec>::kWords], Row<kVec> (&window)[kWidth - 1]) {
-  constexpr int kWords = Row<kVec>::kWords;
-  Row<kVec> rows[kWidth - 1 + kBatch];
+// Outputs of one token from it and the inputs before it.
+template <int kVec, int kWidth>
+__device__ __forceinline__ Row<kVec> convolve(const Row<kVec>* rows, const float2 (&wt)[kWidth][Row<kVec>::kWords],
+                                              const float2 (&bias)[Row<kVec>::kWords]) {
+  Row<kVec> y;
+#pragma unroll
+  for (int c = 0; c < Row<kVec>::kWords; ++c) {
+    float2 acc = bias[c];
+#pragma unroll
+    for (int j = 0; j < kWidth; ++j) {
+      acc = fma2(make_float2(bf16_low(rows[j].w[c]), bf16_high(rows[j].w[c])), wt[j][c], acc);
+    }
+    const float2 z = silu_fast(acc);
+    y.w[c] = pack_bf16(z.x, z.y);
+  }
+  return y;
+}
+
+// Outputs of `count` tokens and the window behind them.  Whole batches are straight code in which every input is
+// unpacked once, and a batch's rows are loaded while the one before is at work.
+template <int kVec, int kWidth>
+__device__ __forceinline__ void convolve_run(const __nv_bfloat16* x, int64_t x_row, __nv_bfloat16* out, int64_t out_row,
+                                             int count, const float2 (&wt)[kWidth][Row<kVec>::kWords],
+                                             const float2 (&bias)[Row<kVec>::kWords], Row<kVec> (&window)[kWidth - 1]) {
+  Row<kVec> rows[kWidth - 1 + kBatch], next[kBatch];
 #pragma unroll
   for (int j = 0; j < kWidth - 1; ++j) rows[j] = window[j];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    if (kFull || i < count) rows[kWidth - 1 + i] = load_row<kVec>(x);
-    x += x_row;
+    if (i < count) next[i] = load_row<kVec>(x + i * x_row);
   }
+  x += kBatch * x_row;
+#pragma unroll 1
+  for (; count >= kBatch; count -= kBatch) {
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i) {
-    if (kFull || i < count) {
-      Row<kVec> y;
+    for (int i = 0; i < kBatch; ++i) rows[kWidth - 1 + i] = next[i];
+    if (count >= 2 * kBatch) {
 #pragma unroll
-      for (int c = 0; c < kWords; ++c) {
-        float2 acc = bias[c];
+      for (int i = 0; i < kBatch; ++i) next[i] = load_row<kVec>(x + i * x_row);
+    } else {
 #pragma unroll
-        for (int j = 0; j < kWidth; ++j) {
-          acc = fma2(make_float2(bf16_low(rows[i + j].w[c]), bf16_high(rows[i + j].w[c])), wt[j][c], acc);
-        }
-        const float2 z = silu_fast(acc);
-        y.w[c] = pack_bf16(z.x, z.y);
-      }
-      store_row<kVec>(out, y);
-      out += out_row;
-      if (!kFull) {
-#pragma unroll
-        for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[i + 1 + j];
+      for (int i = 0; i < kBatch; ++i) {
+        if (kBatch + i < count) next[i] = load_row<kVec>(x + i * x_row);
       }
     }
-  }
-  if (kFull) {
+    x += kBatch * x_row;
 #pragma unroll
-    for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[kBatch + j];
+    for (int i = 0; i < kBatch; ++i) {
+      store_row<kVec>(out, convolve<kVec, kWidth>(rows + i, wt, bias));
+      out += out_row;
+    }
+#pragma unroll
+    for (int j = 0; j < kWidth - 1; ++j) rows[j] = rows[kBatch + j];
   }
+#pragma unroll
+  for (int i = 0; i < kBatch - 1; ++i) {
+    if (i < count) {
+      rows[kWidth - 1] = next[i];
+      store_row<kVec>(out, convolve<kVec, kWidth>(rows, wt, bias));
+      out += out_row;
+#pragma unroll
+      for (int j = 0; j < kWidth - 1; ++j) rows[j] = rows[j + 1];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kWidth - 1; ++j) window[j] = rows[j];
 }
 
 template <int kVec, int kWidth>
@@ -287,9 +312,9 @@ __global__ void __launch_bounds__(kThreads, 6) conv_prefill_kernel(const ConvPre
         }
       }
     }
-    // Up to kBatch tokens that end with their block, request or tile.
+    // The tokens to the end of their block, request or tile.
     const int64_t stop = min(limit, at.ok ? at.next_end : at.end);
-    const int count = static_cast<int>(min(stop - t, static_cast<int64_t>(kBatch)));
+    const int count = static_cast<int>(stop - t);
     const __nv_bfloat16* x = p.x + t * p.x_row + channel;
     __nv_bfloat16* out = p.out + t * p.dim + channel;
     if (!at.ok) {
@@ -297,11 +322,7 @@ __global__ void __launch_bounds__(kThreads, 6) conv_prefill_kernel(const ConvPre
       t += count;
       continue;
     }
-    if (count == kBatch) {
-      convolve<kVec, kWidth, true>(x, p.x_row, out, p.dim, count, wt, bias, window);
-    } else {
-      convolve<kVec, kWidth, false>(x, p.x_row, out, p.dim, count, wt, bias, window);
-    }
+    convolve_run<kVec, kWidth>(x, p.x_row, out, p.dim, count, wt, bias, window);
     t += count;
     if (t == at.next_end) {
       const int64_t block = (at.context + static_cast<uint32_t>(t - 1 - at.begin)) / p.block_size;
@@ -326,7 +347,7 @@ cudaError_t launch_width(ConvPrefillArgs& args, bool vec, cudaStream_t stream) {
   const int channels = (vec ? kVector : 1) * kThreads;
   const int64_t groups = (args.dim + channels - 1) / channels;
   // A tile's thread reads 3 rows that the tile before reads too, and finds its request and its weights: 24 prompts of
-  // 16,000 tokens in all (8,192 channels) take 108.7 us at 64 tokens per thread, 110.5 at 32.  Smaller batches are
+  // 16,000 tokens in all (8,192 channels) took 108.7 us at 64 tokens per thread, 110.5 at 32.  Smaller batches are
   // spread over the SMs (six CTAs each) before their tiles grow.
   const int64_t work = args.n_tokens * groups;
   args.tile = work >= 64 * 6 * 148 ? 64 : work >= 32 * 4 * 148 ? 32 : 8;
