@@ -22,21 +22,27 @@
 // Two kernels.  What does not depend on the state is computed first, for all chunks side by side:
 // gdn_prefill_pairs_kernel, one CTA per (chunk, key head), scales q and k, forms their products once for
 // all value heads of the key head, and leaves q, k, T, P and the rows' factors in a workspace, as the
-// images that the second kernel copies to shared memory.  gdn_prefill_chain_kernel, one CTA per
-// (request, value head), then carries the state from chunk to chunk on the tensor cores' tcgen05
-// instructions, value rows as the M = 128 of every product:
+// images that the second kernel copies to shared memory.  gdn_prefill_chain_kernel then carries the state
+// of a (request, value head) from chunk to chunk on the tensor cores' tcgen05 instructions, value rows as
+// the M = 128 of every product:
 //   Y = S k~, O = S q~   A = S hi, lo in TMEM      B = k~, q~ (K-major)
 //   U = T R              A = R hi, lo in TMEM      B = T hi, lo
 //   P u                  A = u hi in TMEM          B = P
 //   dS = u k~            A = k_out u hi, lo        B = the same k~ tile, read MN-major
-// Eight chain warps keep the fp32 state in registers, 16 value rows each, in the layout that 16-lane TMEM
-// loads and stores use; between products they scale, split and store the next A operand.  Four warps copy
-// the next chunk in, four normalise and store the chunk before's outputs.
+// It is one persistent CTA per SM that takes (request, value head) items from a queue, longest first.
+// Eight warps keep the fp32 state in registers, 16 value rows each, in the layout that 16-lane TMEM
+// loads and stores use; between products they scale, split and store the next A operand, and one of them
+// issues.  The other eight copy the next chunk in and normalise and store the chunk before's outputs.
 //
-// History of the split, 24 prompts of 16,000 tokens in all, 16 key and 32 value heads (and one prompt of
-// 16,384): one kernel that prepared each chunk inside the chain's CTA, 1,242 us (4,878); pairs apart and the
-// chain on mma.sync with the state as its fragments, 555 us (1,646): 11,200 cycles a chunk, of which the
-// 3,200 mma.sync of a chunk are 6,400.
+// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 365-376 us, 140 in
+// the pairs kernel (43% of issue slots, 12,700 warp instructions a CTA: latency, at the four CTAs per SM
+// that 128 registers allow) and 230 in the chain (7,200 cycles a chunk: products 1,260 and their latency,
+// the rest the four steps between them; 45% of issue slots, 20% of the tensor pipe).  History of the
+// split (and of one prompt of 16,384): one kernel that prepared each chunk inside the chain's CTA, 1,242
+// us (4,878); pairs apart and the chain on mma.sync with the state as its fragments, 555 (1,646); the
+// chain on tcgen05, 430 (1,181); outputs gathered off the chain's path 418, the queue 412, one warp that
+// waits for products 400, issue with constant operands 390 (1,137); the pairs of two heads at a time,
+// blocks dealt out evenly, 374 (1,104); long prompts in pieces (732).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
