@@ -366,7 +366,8 @@ int ld_decode_packed_noalloc(const void* qkv, int64_t qkv_row_stride, const void
  * those of ld_decode called once per token, up to rounding (the recurrence's outputs stay fp32
  * until the gated norm, and sums run over chunks of LD_PREFILL_CHUNK tokens).
  *
- * Activations, a_log, dt_bias, gate, weight, out: as in ld_decode.  state: fp32 or bf16
+ * Activations, a_log, dt_bias, gate, weight, out: as in ld_decode; out must not overlap qkv or gate
+ * (their extents, from first to last row, are compared).  state: fp32 or bf16
  * (state_dtype) [n_slots, HV, 128, 128] pool, slot stride in elements (a multiple of 4 or 8); the
  * recurrence runs in fp32 and each stored state is rounded to the pool's type.
  * block_size is a positive multiple of LD_PREFILL_CHUNK.

@@ -1992,6 +1992,17 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
       !aligned(out, 2)) {
     return set_error(LD_ERR_INVALID, "prefill: the pool must be 16-byte aligned and bf16 tensors 2-byte aligned");
   }
+  // Heads of a token are written while others are still read, so outputs need memory of their own.
+  const auto begin_of = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr); };
+  const uintptr_t out_end = begin_of(out) + static_cast<uintptr_t>(2 * n_tokens * num_v_heads * kDim);
+  const auto overlaps = [&](const void* rows, int64_t stride, int64_t width) {
+    return begin_of(rows) < out_end &&
+           begin_of(out) < begin_of(rows) + static_cast<uintptr_t>(2 * ((n_tokens - 1) * stride + width));
+  };
+  if (overlaps(qkv, qkv_row_stride, (2 * num_k_heads + num_v_heads) * kDim) ||
+      overlaps(gate, gate_row_stride, num_v_heads * kDim)) {
+    return set_error(LD_ERR_INVALID, "prefill: out must not overlap qkv or gate");
+  }
   PrefillArgs args;
   args.qkv = static_cast<const __nv_bfloat16*>(qkv);
   args.qkv_row = qkv_row_stride;

@@ -10,12 +10,13 @@ import oracle
 import prompt_oracle
 
 FAKE = 1 << 20  # aligned, not NULL, never read
+FAR = 1 << 40
 
 
 def prefill_args(**changes):
     args = dict(qkv=FAKE, qkv_row=512, a=FAKE, a_row=2, b=FAKE, b_row=2, a_log=FAKE, dt_bias=FAKE, dt_dtype=0, table=FAKE,
                 table_row=4, table_width=4, block=64, context=FAKE, cu=FAKE, requests=3, state=FAKE, state_dtype=0, slots=5,
-                slot_stride=2 * 128 * 128, gate=FAKE, gate_row=256, weight=FAKE, w_dtype=1, out=FAKE, tokens=100, h=1,
+                slot_stride=2 * 128 * 128, gate=FAKE, gate_row=256, weight=FAKE, w_dtype=1, out=FAR, tokens=100, h=1,
                 hv=2, eps=1e-6, workspace=FAKE, size=1 << 40, stream=None)
     assert set(changes) <= set(args)
     return list({**args, **changes}.values())
@@ -46,6 +47,9 @@ def prefill_args(**changes):
     (dict(qkv=None), "NULL"),
     (dict(cu=None), "NULL"),
     (dict(out=None), "NULL"),
+    (dict(out=FAKE), "overlap"),
+    (dict(out=FAKE + 2 * (99 * 512 + 511)), "overlap"),
+    (dict(out=FAR, gate=FAR + 2 * 100 * 256 - 2), "overlap"),
     (dict(workspace=None), "workspace"),
     (dict(workspace=FAKE + 64), "128-byte aligned workspace"),
     (dict(size=1000), "workspace of"),
@@ -219,3 +223,13 @@ def test_oracle_of_tables_by_hand():
     assert positions.tolist() == [6, 7, 8, 0, 1, 2, 3, 4, 8, -1, -1]
     assert slot_map.tolist() == [34, 35, 200, 204, 205, 206, 207, 208, 212, -1, -1]
     assert pairs.tolist() == [[50, 8], [0, 9], [52, 0], [53, 2]]
+
+
+def test_backend_prefill_needs_indexed_state():
+    from lightdelta_b200.backend import GDNBackend
+    from lightdelta_b200.config import BackendConfig
+
+    backend = GDNBackend(BackendConfig(compute="cuda_fused", state_io="packed"))
+    with pytest.raises(ValueError, match="indexed"):
+        backend.prefill(*[None] * 13)
+    assert backend.calls["prefill"] == 0

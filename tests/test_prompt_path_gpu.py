@@ -414,7 +414,7 @@ def test_prefill_refuses_other_tensors():
     case = Prompt([10], [0])
     for change in (dict(table=case.table.long()), dict(table=case.table[0]), dict(context=ints([0, 0])), dict(cu=ints([0])),
                    dict(state=case.state.half()), dict(out=case.out[:5]), dict(gate=case.gate.float()),
-                   dict(qkv=case.qkv[:, :-1]), dict(a=case.a.cpu()), dict(block=63)):
+                   dict(qkv=case.qkv[:, :-1]), dict(a=case.a.cpu()), dict(block=63), dict(gate=case.out)):
         args = dict(qkv=case.qkv, a=case.a, b=case.b, a_log=case.a_log, dt_bias=case.dt_bias, table=case.table,
                     context=case.context, cu=case.cu, state=case.state, gate=case.gate, weight=case.weight, out=case.out,
                     block=64, eps=1e-6)
