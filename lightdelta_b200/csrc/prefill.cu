@@ -16,8 +16,10 @@
 // per row (which the fp32 factors fk, fq undo).  Operands on the way to the state (S itself, R, U and
 // T, L) go in as two fp16 terms, hi + lo, 22 bits together, after scaling each state row by a power of
 // two, so the state follows the fp32 recurrence to under 1e-6.  The two products that only reach the
-// bf16 output (S q and P u) take the hi term alone: 11 bits against the output's 8.  G is summed in
-// fp64 and kept as two floats, so differences of large sums stay exact to fp32.
+// bf16 output (S q and P u) take the hi term alone: 11 bits against the output's 8 (where a chunk's keys
+// are all but equal, the terms of P u cancel and that reaches a few 1e-3 of the output; two terms there
+// took 415 us for the 24 prompts below instead of 390).  G is summed in fp64 and kept as two floats, so
+// differences of large sums stay exact to fp32.
 //
 // Two kernels.  What does not depend on the state is computed first, for all chunks side by side:
 // gdn_prefill_pairs_kernel, one CTA per (chunk, key head), scales q and k, forms their products once for
@@ -75,8 +77,8 @@ constexpr int kKeyHalf = 2 * kHalf;   // from a half of k (or q) to its other ha
 
 __device__ unsigned int g_prefill_faults;
 
-// Workspace images.  Tiles of 128 columns are swizzled (swz) as the chain's products read them; triangular
-// matrices are packed 16 x 16 blocks (tri), which the chain's copies spread to swizzled tiles.
+// Workspace images, byte for byte what the chain's products read: tiles of 128 columns are swizzled (swz), triangular
+// matrices are packed 16 x 16 blocks (tri_block, core).
 struct __align__(128) KeyImage {  // per (chunk, key head)
   __half kq[2 * kChunk * kDim];   // columns 0-63 of k x 2^-e, then of q x 2^-e, then columns 64-127 likewise
 };
@@ -389,7 +391,6 @@ __host__ __device__ constexpr int tri_block(int ib, int jb) { return 256 * (4 * 
 __device__ __forceinline__ int core(int row, int col) {  // within a 16 x 16 block
   return (row >> 3) * 128 + (col >> 3) * 64 + (row & 7) * 8 + (col & 7);
 }
-__device__ __forceinline__ int tri(int row, int col) { return tri_block(row >> 4, col >> 4) + core(row & 15, col & 15); }
 
 // This lane's ldmatrix.x4 address in the 16 x 16 block at `m`, matrices in the order of lane_addr with
 // kRowsFirst false.
@@ -480,7 +481,6 @@ struct Blocks {
 
 // L's blocks below the diagonal ones, row by row.
 __host__ __device__ constexpr int low_block(int ib, int jb) { return 256 * (ib * (ib - 1) / 2 + jb); }
-__device__ __forceinline__ int low(int row, int col) { return low_block(row >> 4, col >> 4) + core(row & 15, col & 15); }
 
 // Rows [row_lo, row_hi) of 128 bf16 to shared memory, the others as zeros, 16 bytes a thread at a time; `at` gives
 // the element that (row, column) goes to.
@@ -1902,7 +1902,6 @@ cudaError_t launch_prefill(PrefillArgs& args, int sms, cudaStream_t stream) {
     return launch(chain, dim3(static_cast<unsigned int>(std::min<int64_t>(items, sms))), dim3(kChainThreads),
                   sizeof(ChainSmem), stream, 1, args);
   };
-  args.pass = 0;
   err = run_chain(heads * args.pieces.first_parts());
   if (err != cudaSuccess || args.pieces.count == 1) return err;
   err = launch(gdn_prefill_join_kernel, dim3(static_cast<unsigned int>(heads * (kDim / kJoinRows))), dim3(kJoinThreads),
@@ -2032,6 +2031,7 @@ extern "C" int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a
   args.next = reinterpret_cast<uint32_t*>(order);
   args.order = reinterpret_cast<int32_t*>(order) + kCounters;
   args.pieces = pieces_of(n_tokens, n_requests, num_v_heads);
+  args.pass = 0;
   args.states = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
                                          states_offset(n_tokens, n_requests, num_k_heads, num_v_heads));
   args.places = chunk_places(n_tokens, n_requests);
