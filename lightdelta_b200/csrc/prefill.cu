@@ -36,7 +36,7 @@
 // loads and stores use; between products they scale, split and store the next A operand, and one of them
 // issues.  The other eight copy the next chunk in and normalise and store the chunk before's outputs.
 //
-// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 365-376 us, 140 in
+// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 365-382 us, 140 in
 // the pairs kernel (43% of issue slots, 12,700 warp instructions a CTA: latency, at the four CTAs per SM
 // that 128 registers allow) and 230 in the chain (7,200 cycles a chunk: products 1,260 and their latency,
 // the rest the four steps between them; 45% of issue slots, 20% of the tensor pipe).  History of the

@@ -273,6 +273,26 @@ def test_prefill_long_prompt_repeats_and_stops():
     assert torch.equal(case.state, before) and torch.equal(case.out, out)
 
 
+def test_prefill_requests_that_share_a_held_block():
+    """One full block as the source of several requests, as prompts with a common beginning have it."""
+    Prompt([70, 3, 64], [64, 64, 64], rows=[[1, 2, 3], [1, 4, 0], [1, 5, 0]], seed=44).check()
+
+
+def test_prefill_long_prompt_in_a_graph():
+    """The passes and joins of a split prompt captured, replayed with new inputs, bit for bit what a call gives."""
+    case, new = Prompt([3000], [30], h=1, hv=2, seed=45), Prompt([3000], [30], h=1, hv=2, seed=46)
+    case.run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        case.run()
+    for name in ("qkv", "a", "b", "a_log", "dt_bias", "table", "gate", "weight", "state"):
+        getattr(case, name).copy_(getattr(new, name))
+    graph.replay()
+    new.run()
+    torch.cuda.synchronize()
+    assert np.array_equal(bits(case.out), bits(new.out)) and torch.equal(case.state, new.state)
+
+
 def test_prefill_many_requests():
     """Single tokens and empty requests by the hundred, in an order that the queue of items changes."""
     lens = [(7 * i) % 3 for i in range(300)]
