@@ -1705,14 +1705,16 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     x.dead = false;
     for (int64_t n = 0;; ++n) {
       const int stage = static_cast<int>(n & 1);
-      const Stage& st = s.stage[stage];
       bar_sync(kBarFull + stage);
-      if (st.work.kind == kWorkEnd) break;
-      const int32_t source = st.work.source, slot = st.work.slot;
-      [[maybe_unused]] int32_t save = st.work.save;
+      // A copy, for this chunk's store too: from the arrival at kBarChunkDone on, the moving threads may refill the
+      // stage and write its next work, so nothing of the stage is read behind that.
+      const Work work = s.stage[stage].work;
+      if (work.kind == kWorkEnd) break;
+      const int32_t source = work.source, slot = work.slot;
+      [[maybe_unused]] int32_t save = work.save;
       const int64_t element = (v0 + g) * kDim + 2 * t;
       const auto pool_at = [&](int32_t i) {
-        return static_cast<StateT*>(p.state) + i * p.slot_stride + static_cast<int64_t>(st.work.head) * kDim * kDim + element;
+        return static_cast<StateT*>(p.state) + i * p.slot_stride + static_cast<int64_t>(work.head) * kDim * kDim + element;
       };
       const auto matrix_at = [&](int32_t i) { return p.states + static_cast<int64_t>(i) * kDim * kDim + element; };
       const auto load = [&](const auto* at) {
@@ -1733,12 +1735,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       constexpr bool kShared = kSplit && std::is_same<StateT, float>::value;
       if (source > 0 || (kShared && source == kSourceMatrix)) {
         if constexpr (kShared) {
-          load(source > 0 ? pool_at(source) : matrix_at(st.work.matrix));
+          load(source > 0 ? pool_at(source) : matrix_at(work.matrix));
         } else {
           load(pool_at(source));
         }
       } else if (kSplit && !kShared && source == kSourceMatrix) {
-        load(matrix_at(st.work.matrix));
+        load(matrix_at(work.matrix));
       } else if (source != kSourceOn) {  // zeros, or the identity
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
