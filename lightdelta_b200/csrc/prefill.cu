@@ -1029,6 +1029,7 @@ struct ChainSmem {
   Cursor at;
   Work upcoming;      // what the next free stage takes
   volatile int stop;  // a wait ran out: nothing is stored any more
+  int keep;           // the issuing warp's answer for the chunk in work: no wait ran out, its state may be stored
 };
 
 // TMEM columns (32 bits x 128 lanes, lane = value row); all 512 are allocated, so they start at 0.  dS takes
@@ -1300,10 +1301,15 @@ struct Products {
 // The products that the state waits for are done.  One warp asks the barrier, the others wait for it at a named
 // barrier: asking, eight warps took so many issue slots from the one that issues that a product of 32 cycles
 // (N = 64) was issued every 48.
+//
+// With kLast, the chunk's last ones, the issuing warp also says whether the chunk's state may be stored.  `stop` may be set
+// at any moment, by the moving threads too: were every warp to read it, a slot could take some warps' rows alone.
+template <bool kLast = false>
 __device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool issuer, uint64_t limit_ns) {
   if (issuer) {
     wait_done(smem_u32(&s.done[0]), x.phase, s, x.dead, limit_ns);
     x.phase ^= 1;
+    if constexpr (kLast) s.keep = s.stop == 0;
   }
   bar_state();
   tmem_after();
@@ -1436,7 +1442,7 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   const float2 decay = make_float2(st.pair.decay, st.pair.decay);
   const float k0 = w0 * st.pair.k_scale, k1 = w1 * st.pair.k_scale;
   const float2 w02 = make_float2(k0, k0), w12 = make_float2(k1, k1);
-  wait_products(x, s, issuer, limit_ns);
+  wait_products<true>(x, s, issuer, limit_ns);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     tmem_load(tmem + kTmemDs + 64 * half, Y);
@@ -1758,7 +1764,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         }
       });
       bar_arrive(kBarChunkDone);
-      const bool to_pool = slot > 0 && s.stop == 0;
+      const bool to_pool = slot > 0 && s.keep != 0;  // read before the next chunk's answer: bar_state lies between
       if constexpr (kShared) {
         float* at = to_pool ? pool_at(slot) : nullptr;
 #pragma unroll 1

@@ -42,3 +42,16 @@ def test_the_state_warps_leave_a_stage_before_they_hand_it_back():
     for body in re.findall(r"\[&\]\([^)]*\)\s*\{(.*?)\n?\s*\};", before, re.S):
         assert not re.search(stage_names, body), f"a lambda reads the stage when it is called: {body.strip()}"
     assert len(re.findall(r"s\.stage\[stage\]\.work", before)) == 1 and "const Work work = s.stage[stage].work;" in before
+
+
+def test_the_state_warps_store_a_state_together_or_not_at_all():
+    """A wait may run out while they store, in a warp that they do not wait for.  One warp decides for all, in front of a
+    barrier that all pass, so that no slot takes some warps' rows and not the others'."""
+    loop = state_loop()
+    assert "s.stop" not in loop and "s.keep" in loop.split("bar_arrive(kBarChunkDone)")[1]
+    text = without_comments((CSRC / "prefill.cu").read_text())
+    wait = text[text.index("void wait_products("):]
+    wait = wait[:wait.index("\n}")]
+    decided, joined = wait.index("s.keep = s.stop == 0;"), wait.index("bar_state();")
+    assert wait.index("if (issuer)") < decided < joined
+    assert len(re.findall(r"s\.keep\b", text)) == 2, "one place writes it, one reads it"
