@@ -1568,7 +1568,7 @@ __device__ __noinline__ void zero_item(const PrefillArgs& p, const Work& d, int 
 template <bool kSplit>
 __device__ __forceinline__ void skip_items(const PrefillArgs& p, ChainSmem& s, int tid) {
   while (s.upcoming.kind == kWorkZero) {
-    zero_item(p, s.upcoming, tid);
+    if (s.stop == 0) zero_item(p, s.upcoming, tid);
     bar_move();
     if (tid == 0) next_item<kSplit>(p, s.at, s.upcoming);
     bar_move();
