@@ -1025,6 +1025,7 @@ struct ChainSmem {
   float s_down[kDim], u_down[kDim];  // what S q and P u of the chunk in work are scaled by, per value row
   uint64_t full[2];  // a stage's copies have landed
   uint64_t done[2];  // products finished: [0] what the state waits for, [1] what only the outputs do
+  uint64_t drained;  // after a wait that ran out: every product
   uint32_t tmem;
   Cursor at;
   Work upcoming;      // what the next free stage takes
@@ -1606,10 +1607,17 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     // copies.
     uint32_t landed = 0;
     bool late = false;
+    uint32_t owed = 0, owed_parity = 0;  // the barrier of copies that a wait ran out for
     const auto hand_over = [&](int stage, bool chunk) {
       cp_async_wait_groups<1>();  // but not for the gates, which were asked for last
       if (warp == 0 && chunk) {
-        wait_done(full(stage), (landed >> stage) & 1, s, late, p.wait_ns);
+        const uint32_t parity = (landed >> stage) & 1;
+        const bool before = late;
+        wait_done(full(stage), parity, s, late, p.wait_ns);
+        if (late && !before) {
+          owed = full(stage);
+          owed_parity = parity;
+        }
         landed ^= 1u << stage;
       }
       bar_arrive(kBarFull + stage);
@@ -1683,6 +1691,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
         hand_over(stage, more);
       }
     }
+    // Copies that are still under way must not land in shared memory that is another CTA's by then.  There is one set at
+    // most: each is waited for before the next is asked for, and after a wait that ran out there is no next.
+    if (owed != 0) {
+      bool over = false;
+      wait_done(owed, owed_parity, s, over, p.wait_ns);
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     const int g = lane >> 2, t = lane & 3;
@@ -1696,6 +1710,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
       if (lane == 0) {
         for (int i = 0; i < 2; ++i) barrier_init(smem_u32(&s.done[i]));
+        barrier_init(smem_u32(&s.drained));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       }
       __syncwarp();
@@ -1788,6 +1803,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
   if (threadIdx.x == 0 && s.stop != 0) p.next[2] = 1;
   if (warp == kStateWarp) {
     tmem_after();
+    if (s.stop != 0) {  // products that nobody waited for may still read the stages and write TMEM
+      umma_commit(elect_lane(), smem_u32(&s.drained));
+      bool over = false;
+      wait_done(smem_u32(&s.drained), 0, s, over, p.wait_ns);
+    }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(kTmemColumns));
   }
 }

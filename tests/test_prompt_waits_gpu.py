@@ -36,3 +36,15 @@ def test_a_wait_that_runs_out_leaves_the_zeros_of_invalid_requests_too():
     run_out(case, 20_000_000)
     assert capi.fault_flags() == capi.LD_FAULT_WAIT_TIMEOUT
     assert torch.equal(case.state, before) and torch.equal(case.out, out)
+
+
+def test_a_wait_that_runs_out_is_followed_by_one_for_what_is_in_flight():
+    """Before it returns, a CTA waits once more, as long at most, for the copies that it has under way: they must not land
+    in shared memory that is another CTA's by then."""
+    case = Prompt([130], [64], h=1, hv=2, seed=91)
+    before, out = case.state.clone(), case.out.clone()
+    took = run_out(case, 20_000_000)
+    assert capi.fault_flags() == capi.LD_FAULT_WAIT_TIMEOUT
+    assert torch.equal(case.state, before) and torch.equal(case.out, out)
+    assert 39.0 < took < 200.0
+    case.check()
