@@ -303,14 +303,18 @@ def prefill_workspace(tokens: int, requests: int, num_k_heads: int, num_v_heads:
 def prefill(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, out, block_size, eps=1e-6,
             workspace=None, stream=None):
     """ld_prefill on torch tensors laid out as torch.ops.lightdelta.prefill expects; `workspace` is a CUDA
-    byte tensor of prefill_workspace(...) bytes at least."""
+    byte tensor of prefill_workspace(...) bytes at least, which no other work may use until the call has run.  Without one
+    it comes from torch's allocator on the stream of the call and goes back to it there."""
     import torch
 
     hv = state.shape[1]
     h = (qkv.shape[1] // HEAD_DIM - hv) // 2
     if workspace is None:
-        workspace = torch.empty(prefill_workspace(qkv.shape[0], context.numel(), h, hv), dtype=torch.uint8,
-                                device=qkv.device)
+        # The allocator orders a block's users on the stream that asked for it, so the one that uses it has to ask.
+        own = torch.cuda.ExternalStream(_stream(qkv, stream), device=qkv.device)
+        with torch.cuda.stream(own):
+            workspace = torch.empty(prefill_workspace(qkv.shape[0], context.numel(), h, hv), dtype=torch.uint8,
+                                    device=qkv.device)
     check(lib().ld_prefill(
         qkv.data_ptr(), qkv.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_log.data_ptr(),
         dt_bias.data_ptr(), _dtype_code(dt_bias), table.data_ptr(), table.stride(0), table.shape[1], int(block_size),
