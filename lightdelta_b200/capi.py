@@ -8,6 +8,7 @@ There is no CPU fallback: if the library is missing, loading raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -170,6 +171,19 @@ def _stream(tensor, stream) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _allocating_on(tensor, stream):
+    """Context in which torch's allocator serves the stream that _stream names."""
+    import torch
+
+    if stream is None:
+        return contextlib.nullcontext()
+    if not hasattr(stream, "cuda_stream"):
+        pointer = int(stream)  # ExternalStream takes 0, the default stream's, for no pointer at all
+        stream = (torch.cuda.ExternalStream(pointer, device=tensor.device) if pointer
+                  else torch.cuda.default_stream(tensor.device))
+    return torch.cuda.stream(stream)
+
+
 def _dtype_code(tensor) -> int:
     import torch
 
@@ -311,8 +325,7 @@ def prefill(qkv, a, b, a_log, dt_bias, table, context, cu, state, gate, weight, 
     h = (qkv.shape[1] // HEAD_DIM - hv) // 2
     if workspace is None:
         # The allocator orders a block's users on the stream that asked for it, so the one that uses it has to ask.
-        own = torch.cuda.ExternalStream(_stream(qkv, stream), device=qkv.device)
-        with torch.cuda.stream(own):
+        with _allocating_on(qkv, stream):
             workspace = torch.empty(prefill_workspace(qkv.shape[0], context.numel(), h, hv), dtype=torch.uint8,
                                     device=qkv.device)
     check(lib().ld_prefill(

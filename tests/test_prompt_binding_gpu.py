@@ -9,13 +9,13 @@ from test_prompt_path_gpu import Prompt, check_outputs, check_states
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("how", ["stream", "pointer", "default"])
+@pytest.mark.parametrize("how", ["stream", "pointer", "current", "zero"])
 def test_prefill_on_a_stream_of_its_own(how, monkeypatch):
     """A call on a stream that is not the current one, while the current one goes on allocating and writing."""
     case = Prompt([700, 64], [0, 64], seed=95)
     want, size, pool = case.expect()
     side = torch.cuda.Stream()
-    given = {"stream": side, "pointer": side.cuda_stream, "default": None}[how]
+    given = {"stream": side, "pointer": side.cuda_stream, "current": None, "zero": 0}[how]
     made, real = [], torch.empty
 
     def empty(*args, **kwargs):
@@ -31,7 +31,7 @@ def test_prefill_on_a_stream_of_its_own(how, monkeypatch):
     torch.cuda.synchronize()
     (address,) = made
     owners = [s["stream"] for s in torch.cuda.memory_snapshot() if s["address"] <= address < s["address"] + s["total_size"]]
-    assert owners == [torch.cuda.current_stream().cuda_stream if how == "default" else side.cuda_stream]
+    assert owners == [side.cuda_stream if how in ("stream", "pointer") else torch.cuda.default_stream().cuda_stream]
     check_outputs(case.out, want, size)
     check_states(case.state, pool)
     assert len(junk) == 8 and capi.fault_flags() == 0
