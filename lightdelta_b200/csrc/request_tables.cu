@@ -183,17 +183,35 @@ __global__ void __launch_bounds__(kThreads) request_tables_kernel(const TablesAr
     p.state_slots[2 * r] = l.query > 0 ? block_of(p, r, l.want - 1, l, first) : 0;
     p.state_slots[2 * r + 1] = l.context > 0 ? block_of(p, r, l.have - 1, l, first) : 0;
   }
-  for (int64_t i = start; i < all_blocks; i += step) {
-    const int f = find_stretch(s.blocks, i);
-    int r = f * p.stretch;
-    int64_t first = s.blocks[f];
-    Lengths l = lengths_of(p, r);
-    while (first + (l.want - l.have) <= i) {
-      first += l.want - l.have;
-      l = lengths_of(p, ++r);
+  // New blocks past the end of their row are left out.  Lengths that ask for more blocks than the table has entries, up to
+  // 2^31 a request, must not keep the GPU busy counting them: there the entries are gone through instead.
+  const int64_t width = min(p.table_width, static_cast<int64_t>(1) << 32);  // a request has fewer blocks than 2^32
+  const int64_t entries = p.n_requests * width;
+  if (all_blocks <= entries) {
+    for (int64_t i = start; i < all_blocks; i += step) {
+      const int f = find_stretch(s.blocks, i);
+      int r = f * p.stretch;
+      int64_t first = s.blocks[f];
+      Lengths l = lengths_of(p, r);
+      while (first + (l.want - l.have) <= i) {
+        first += l.want - l.have;
+        l = lengths_of(p, ++r);
+      }
+      const int64_t b = l.have + (i - first);
+      if (b < p.table_width) p.table[r * p.table_row + b] = i < p.n_free ? p.free_blocks[i] : 0;
     }
-    const int64_t b = l.have + (i - first);
-    if (b < p.table_width) p.table[r * p.table_row + b] = i < p.n_free ? p.free_blocks[i] : 0;
+  } else {
+    for (int64_t i = start; i < entries; i += step) {
+      const int r = static_cast<int>(i / width), f = r / p.stretch;
+      const uint32_t b = static_cast<uint32_t>(i - r * width);
+      int64_t first = s.blocks[f];
+      for (int k = f * p.stretch; k < r; ++k) {
+        const Lengths l = lengths_of(p, k);
+        first += l.want - l.have;
+      }
+      const Lengths l = lengths_of(p, r);
+      if (b >= l.have && b < l.want) p.table[r * p.table_row + b] = block_of(p, r, b, l, first);
+    }
   }
   for (int64_t i = start; i < p.n_tokens; i += step) {
     int64_t position = -1, slot = -1;
