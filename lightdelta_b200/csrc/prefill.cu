@@ -13,13 +13,13 @@
 //
 // Precision.  The state and every sum stay in fp32.  Matrix instructions take fp16 operands with
 // fp32 accumulation.  q and k rows are bf16 and become fp16 exactly after scaling by a power of two
-// per row (which the fp32 factors fk, fq undo).  Operands on the way to the state (S itself, R, U and
-// T, L) go in as two fp16 terms, hi + lo, 22 bits together, after scaling each state row by a power of
-// two, so the state follows the fp32 recurrence to under 1e-6.  The two products that only reach the
-// bf16 output (S q and P u) take the hi term alone: 11 bits against the output's 8 (where a chunk's keys
-// are all but equal, the terms of P u cancel and that reaches a few 1e-3 of the output; two terms there
-// took 415 us for the 24 prompts below instead of 390).  G is summed in fp64 and kept as two floats, so
-// differences of large sums stay exact to fp32.
+// per row (which the fp32 factors fk, fq undo).  All other operands (S, R, u, T, L, P) go in as two fp16
+// terms, hi + lo, 22 bits together (P 19), after scaling each state row by a power of two, so the state
+// follows the fp32 recurrence to under 1e-6, and so do the outputs until they are rounded to bf16.  (With
+// one term for S q and P u, 11 bits, one output in ten was rounded elsewhere, and where a query is nearly
+// orthogonal to what the state holds, or a chunk's keys are all but equal, the gated norm made that a few
+// 1e-3 to 1e-2 of the output; that took 365-382 us for the 24 prompts below.)  G is summed in fp64 and kept
+// as two floats, so differences of large sums stay exact to fp32.
 //
 // Two kernels.  What does not depend on the state is computed first, for all chunks side by side:
 // gdn_prefill_pairs_kernel, one CTA per (chunk, key head), scales q and k, forms their products once for
@@ -29,7 +29,7 @@
 // the M = 128 of every product:
 //   Y = S k~, O = S q~   A = S hi, lo in TMEM      B = k~, q~ (K-major)
 //   U = T R              A = R hi, lo in TMEM      B = T hi, lo
-//   P u                  A = u hi in TMEM          B = P
+//   P u                  A = u hi, lo in TMEM      B = P hi, lo
 //   dS = u k~            A = k_out u hi, lo        B = the same k~ tile, read MN-major
 // It is one persistent CTA per SM that takes (request, value head) items from a queue, longest first.
 // Eight warps keep the fp32 state in registers, 16 value rows each, in the layout that 16-lane TMEM
@@ -84,19 +84,37 @@ struct __align__(128) KeyImage {  // per (chunk, key head)
 };
 
 constexpr int kTriBlocks = 10;  // 16 x 16 blocks on and below the diagonal of a 64 x 64 matrix
-struct __align__(128) PairImage {  // per (chunk, value head)
+constexpr int kLowBlocks = 6;   // of them, below it
+// Per (chunk, value head).  The stage that a chunk is worked from has T and P as two fp16 terms each; here the terms share
+// what room there is (unpack_chunk takes them apart again):
+//   T is a unit triangle, so the lo terms of its diagonal blocks lie transposed above the diagonal of t_hi's;
+//   P's lo terms are bytes, in 256ths of the hi term's last bit: 19 bits together.  Of a diagonal block's four core
+//   matrices the one above the diagonal is left out, and three numbers lie in bytes of others that are above it, too.
+struct PairMain {
   __half t_hi[kTriBlocks * 256];
-  __half t_lo[kTriBlocks * 256];
-  __half p[kTriBlocks * 256];
+  __half p_hi[kTriBlocks * 256];
   float beta[kChunk];
   float k_in[kChunk];   // e^{G_i} fk_i: scales S k~
   float q_in[kChunk];   // e^{G_i} fq_i 128^-1/2: scales S q~
   float k_out[kChunk];  // e^{G_C - G_j} fk_j / k_scale: scales u_j on its way into the state
-  float decay;          // e^{G_C}
-  float k_scale;        // the power of two that brings the largest of k_out to [1, 2)
-  float p_scale;        // the powers of two that P was divided by, for the chunk's largest fk and fq
+  uint8_t p_lo[kLowBlocks * 256 + 4 * 192];  // blocks below the diagonal, then three core matrices per diagonal block
+
+  // Columns 4-7 of rows 0, 1 and 2 of the first diagonal block.
+  __device__ __forceinline__ float* numbers() { return reinterpret_cast<float*>(p_lo + kLowBlocks * 256); }
+  __device__ __forceinline__ const float* numbers() const { return reinterpret_cast<const float*>(p_lo + kLowBlocks * 256); }
+  __device__ __forceinline__ float& decay() { return numbers()[1]; }    // e^{G_C}
+  __device__ __forceinline__ float& k_scale() { return numbers()[3]; }  // the power of two that brings the largest of k_out to [1, 2)
+  __device__ __forceinline__ float& p_scale() { return numbers()[5]; }  // the powers of two that P was divided by
+  __device__ __forceinline__ float decay() const { return numbers()[1]; }
+  __device__ __forceinline__ float k_scale() const { return numbers()[3]; }
+  __device__ __forceinline__ float p_scale() const { return numbers()[5]; }
 };
-static_assert(sizeof(KeyImage) % 16 == 0 && sizeof(PairImage) % 16 == 0, "images are copied 16 bytes at a time");
+struct __align__(128) PairImage {
+  PairMain main;
+  __half t_lo[kLowBlocks * 256];  // blocks below the diagonal
+};
+static_assert(sizeof(KeyImage) % 16 == 0 && sizeof(PairMain) % 16 == 0, "images are copied 16 bytes at a time");
+static_assert(sizeof(PairImage) == sizeof(PairMain) + sizeof(PairImage::t_lo), "without gaps");
 
 // Splitting a long prompt.  The chain takes a value head's chunks one after the other, so few requests with few heads
 // leave most SMs idle.  A chunk's step is linear in the state, S <- S M + B, and so is a run of chunks: M is what it
@@ -343,8 +361,8 @@ __device__ __forceinline__ void cp_async_wait_groups() {
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-__device__ __forceinline__ void barrier_init(uint32_t bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t arrivals = 1) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(arrivals) : "memory");
 }
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -388,6 +406,13 @@ __device__ __forceinline__ uint32_t block(uint32_t addr, int rb, int cb) {
 // conflicts.
 __host__ __device__ constexpr int tri_block(int ib, int jb) { return 256 * (4 * jb - jb * (jb - 1) / 2 + (ib - jb)); }
 
+// The blocks below the diagonal in the order of their places, and block i's number among all ten.
+__host__ __device__ constexpr int below_block(int ib, int jb) { return jb == 0 ? ib - 1 : jb == 1 ? ib + 1 : 5; }
+__host__ __device__ constexpr int below_place(int i) { return i + 1 + (i >= 3) + (i >= 5); }
+static_assert(256 * below_place(below_block(3, 0)) == tri_block(3, 0) && 256 * below_place(below_block(2, 1)) == tri_block(2, 1) &&
+                  256 * below_place(below_block(3, 1)) == tri_block(3, 1) && 256 * below_place(below_block(3, 2)) == tri_block(3, 2),
+              "column by column");
+
 __device__ __forceinline__ int core(int row, int col) {  // within a 16 x 16 block
   return (row >> 3) * 128 + (col >> 3) * 64 + (row & 7) * 8 + (col & 7);
 }
@@ -411,6 +436,41 @@ __device__ __forceinline__ void split(float2 x, uint32_t& hi, uint32_t& lo) {
   const __half2 l = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// The same with hi cut off instead of rounded, 22 bits together instead of 23, which spares the way back from fp16: the
+// chain's splits are on the state's path (one prompt of 16,384 tokens: 777 -> 750 us).
+__device__ __forceinline__ void split_masked(float2 x, uint32_t& hi, uint32_t& lo) {
+  const float2 f = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
+                               __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+  hi = pack_half(f.x, f.y);
+  const float2 r = fma2(f, make_float2(-1.0f, -1.0f), x);
+  lo = pack_half(r.x, r.y);
+}
+
+// x as a fp16 term and a byte: what that leaves, in 256ths of its last bit, plus 128.  A last bit is 2^(e - 25), e the
+// biased exponent; terms below fp16's normal range keep no byte.
+__device__ __forceinline__ void split_byte(float2 x, uint32_t& hi, uint32_t& bytes) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
+  const float2 f = __half22float2(h);
+  const float2 r = fma2(f, make_float2(-1.0f, -1.0f), x);  // exact
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  const float s0 = __uint_as_float((160u << 23) - ((hi & 0x7c00u) << 13));  // 2^(33 - e)
+  const float s1 = __uint_as_float((160u << 23) - ((hi & 0x7c000000u) >> 3));
+  // The sum's last mantissa bits are the rounded byte; half a last bit would be 256.
+  constexpr float kShift = 8388608.0f + 128.0f;
+  const uint32_t b0 = __float_as_uint(fminf(fmaf(r.x, s0, kShift), kShift + 127.0f));
+  const uint32_t b1 = __float_as_uint(fminf(fmaf(r.y, s1, kShift), kShift + 127.0f));
+  bytes = __byte_perm(b0, b1, 0x0040) & 0xffffu;
+}
+
+// The lo terms of two elements from their hi terms and bytes (the low ones of 16-bit halves).
+__device__ __forceinline__ uint32_t lo_terms(uint32_t hi, uint32_t bytes) {
+  const uint32_t last = hi & 0x7c007c00u, shifted = bytes | 0x64006400u;  // 2^(e - 15) each; 1024 + byte
+  const __half2 bit = __hmul2(*reinterpret_cast<const __half2*>(&last), __float2half2_rn(0x1p-10f));
+  const __half2 part = __hfma2(*reinterpret_cast<const __half2*>(&shifted), __float2half2_rn(0x1p-8f), __float2half2_rn(-4.5f));
+  const __half2 lo = __hmul2(bit, part);
+  return *reinterpret_cast<const uint32_t*>(&lo);
 }
 
 // 2^s with s such that the largest magnitude m lands in [2^13, 2^14), and 2^-s: fp16's two terms then
@@ -648,7 +708,7 @@ __device__ __forceinline__ void row_products(PairSmem& s, const Blocks& mine, in
 }
 
 // The factors of the chunk's rows for one value head, row i = 0..63 by two warps, straight to its image.
-__device__ __forceinline__ void row_factors(const PrefillArgs& p, PairSmem& s, int place, int i, PairImage& image) {
+__device__ __forceinline__ void row_factors(const PrefillArgs& p, PairSmem& s, int place, int i, PairMain& image) {
   const float in = exp2_fast(s.g_hi[place][i] + s.g_lo[place][i]);
   image.beta[i] = s.beta[place][i];
   image.k_in[i] = in * s.fk[i];
@@ -660,16 +720,16 @@ __device__ __forceinline__ void row_factors(const PrefillArgs& p, PairSmem& s, i
   const float k_out = out(i), power = largest_power(k_out, out(i ^ 32));
   image.k_out[i] = k_out * inverse_power(power);
   if (i == kChunk - 1) {
-    image.decay = in;
-    image.k_scale = power;
-    image.p_scale = s.fk_power * s.fq_power;
+    image.decay() = in;
+    image.k_scale() = power;
+    image.p_scale() = s.fk_power * s.fq_power;
   }
 }
 
-// L and P of this warp's blocks for one value head; P goes straight to the image, 128 bytes a store.
+// L and P of this warp's blocks for one value head, two terms each; P goes straight to the image, 128 and 64 bytes a store.
 __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s, PairHead& head, int place,
                                               const Blocks& mine, int lane, const float (&kk)[3][2][4],
-                                              const float (&qk)[3][2][4], __half* p_image) {
+                                              const float (&qk)[3][2][4], PairMain& image) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int b = 0; b < 3; ++b) {
@@ -684,7 +744,8 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
       row_k[half] = s.beta[place][i] * s.fk[i] * s.fk_power;
       row_q[half] = p.q_scale * s.fq_unit[i];
     }
-    __half* to_p = p_image + tri_block(mine.ib(b), mine.jb(b)) + core(g, 2 * t);
+    const int to_p = tri_block(mine.ib(b), mine.jb(b)) + core(g, 2 * t);
+    const int to_byte = (b > 0 ? 256 * below_block(mine.row, mine.jb(b)) : 256 * kLowBlocks + 192 * mine.w) + core(g, 2 * t);
     const int to_l = low_block(mine.row, mine.jb(b)) + core(g, 2 * t);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -711,7 +772,12 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
           *reinterpret_cast<uint32_t*>(&head.l_hi[to_l + core(8 * half, 8 * m)]) = hi;
           *reinterpret_cast<uint32_t*>(&head.l_lo[to_l + core(8 * half, 8 * m)]) = lo;
         }
-        *reinterpret_cast<uint32_t*>(&to_p[core(8 * half, 8 * m)]) = pack_half(p0, p1);
+        uint32_t hi, bytes;
+        split_byte(make_float2(p0, p1), hi, bytes);
+        *reinterpret_cast<uint32_t*>(&image.p_hi[to_p + core(8 * half, 8 * m)]) = hi;
+        // Of a diagonal block, pairs with an element on or below the diagonal.
+        const bool kept = b > 0 || half > m || (half == m && 2 * t <= g);
+        if (kept) *reinterpret_cast<uint16_t*>(&image.p_lo[to_byte + (b > 0 ? core(8 * half, 8 * m) : 64 * (half + m))]) = bytes;
       }
     }
   }
@@ -956,9 +1022,9 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
         __syncthreads();
       }
     }
-    if ((w >> 1) < heads) row_factors(p, s, at + (w >> 1), tid & (kChunk - 1), images[w >> 1]);
+    if ((w >> 1) < heads) row_factors(p, s, at + (w >> 1), tid & (kChunk - 1), images[w >> 1].main);
 #pragma unroll 1
-    for (int i = 0; i < heads; ++i) decayed_pairs(p, s, s.head(i), at + i, mine, lane, kk, qk, images[i].p);
+    for (int i = 0; i < heads; ++i) decayed_pairs(p, s, s.head(i), at + i, mine, lane, kk, qk, images[i].main);
     __syncwarp();
     if ((lane >> 4) < heads) invert_diagonal(s.head(lane >> 4), w, lane & 15);
     __syncthreads();
@@ -969,11 +1035,26 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
     __syncthreads();
 #pragma unroll 1
     for (int i = 0; i < heads; ++i) {
-      uint4* to = reinterpret_cast<uint4*>(images + i);  // t_hi and t_lo come first
-      const uint4* from = reinterpret_cast<const uint4*>(&s.head(i));
-      constexpr int kPieces = 2 * sizeof(PairHead::t_hi) / 16;
+      PairHead& head = s.head(i);
 #pragma unroll
-      for (int k = 0; k < kPieces / kPairThreads; ++k) to[k * kPairThreads + tid] = from[k * kPairThreads + tid];
+      for (int k = 0; k < 2 * kLowBlocks * 32 / kPairThreads; ++k) {  // 16 bytes of the blocks below the diagonal
+        const int at = k * kPairThreads + tid, low = at % (kLowBlocks * 32);
+        const int from = 256 * below_place(low >> 5) + 8 * (low & 31);
+        if (at < kLowBlocks * 32) {
+          *reinterpret_cast<uint4*>(&images[i].main.t_hi[from]) = *reinterpret_cast<const uint4*>(&head.t_hi[from]);
+        } else {
+          *reinterpret_cast<uint4*>(&images[i].t_lo[8 * low]) = *reinterpret_cast<const uint4*>(&head.t_lo[from]);
+        }
+      }
+      // This warp's diagonal block, its lo terms transposed above the diagonal, where hi has zeros and lo has none below.
+      uint32_t hi[4], lo[4];
+      ldsm4(core_addr(head.t_hi, lane) + 2 * tri_block(w, w), hi);
+      ldsm4_t(core_addr(head.t_lo, lane) + 2 * tri_block(w, w), lo);
+      uint32_t* to = reinterpret_cast<uint32_t*>(&images[i].main.t_hi[tri_block(w, w) + core(lane >> 2, 2 * (lane & 3))]);
+      to[0] = hi[0] | lo[0];
+      to[32] = lo[2];  // the upper right core matrix: the lower left one's
+      to[64] = hi[2];
+      to[96] = hi[3] | lo[3];
     }
   }
 }
@@ -981,6 +1062,10 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
 // ------------------------------------------------------------------------------------------
 // chain: the state through the chunks
 // ------------------------------------------------------------------------------------------
+constexpr int kIssuers = 3;   // warps that issue products
+// Moving warps with a task of their own beside the common ones: warp 0 issues P u, these ask for a stage's bulk copies and
+// wait for them, and find out the upcoming work.  All by warp 0, the moving threads took longer than the chain.
+constexpr int kCopyWarp = 3, kTakeWarp = 5;
 constexpr int kVRow = kDim + 8;  // bf16 per row of a stage's v and gate: the 16 bytes spread their rows over the banks
 
 // What a stage holds: one chunk of one item.
@@ -1013,7 +1098,9 @@ struct Cursor {
 
 struct __align__(1024) Stage {
   __half kq[2 * kChunk * kDim];
-  PairImage pair;
+  PairMain pair;  // t_hi without lo terms above the diagonal once it is unpacked
+  __align__(16) __half t_lo[kTriBlocks * 256];
+  __half p_lo[kTriBlocks * 256];
   __align__(16) __nv_bfloat16 v[kChunk * kVRow];
   __align__(16) __nv_bfloat16 gate[kChunk * kVRow];
   Work work;
@@ -1024,8 +1111,8 @@ struct ChainSmem {
   __align__(16) float o[kChunk * kORow];
   float s_down[kDim], u_down[kDim];  // what S q and P u of the chunk in work are scaled by, per value row
   uint64_t full[2];  // a stage's copies have landed
-  uint64_t done[2];  // products finished: [0] what the state waits for, [1] what only the outputs do
-  uint64_t drained;  // after a wait that ran out: every product
+  uint64_t done[3];  // products finished: [0] what the state waits for, [1] P u, [2] S q
+  uint64_t drained;  // after a wait that ran out: every product, a commit of each warp that issues some
   uint32_t tmem;
   Cursor at;
   Work upcoming;      // what the next free stage takes
@@ -1033,26 +1120,72 @@ struct ChainSmem {
   int keep;           // the issuing warp's answer for the chunk in work: no wait ran out, its state may be stored
 };
 
+static_assert(sizeof(ChainSmem) <= 227 * 1024, "shared memory of a CTA");
+
 // TMEM columns (32 bits x 128 lanes, lane = value row); all 512 are allocated, so they start at 0.  dS takes
 // the place of Y and T R, which are in registers by then, and P u that of R.
 constexpr uint32_t kTmemS = 0, kTmemR = 128, kTmemPu = 128, kTmemU = 192, kTmemW = 224, kTmemY = 288, kTmemTr = 352,
-                   kTmemDs = 288, kTmemO = 416, kTmemColumns = 512;
+                   kTmemDs = 288, kTmemO = 416, kTmemUlo = 480, kTmemColumns = 512;
 
-// The chunk's images to a stage by two bulk copies, its v rows by the moving threads.
+// The chunk's images to a stage by bulk copies, its v rows by the moving threads.
 template <bool kVec>
 __device__ __forceinline__ void copy_chunk(const PrefillArgs& p, Stage& st, const Work& d, uint32_t full, int tid, bool late) {
   // What was read and written in this stage so far comes before the bulk copies, which go through the async
   // proxy (a barrier lies between that and this thread).
-  if (tid == 0 && !late) {  // after a wait that ran out there are no more of them, and the ones before have landed
+  if (tid == 32 * kCopyWarp && !late) {  // after a wait that ran out there are no more of them, and the ones before have landed
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     barrier_expect(full, sizeof(KeyImage) + sizeof(PairImage) + p.extra_tx);
     bulk_copy(smem_u32(st.kq), p.keys + d.place * p.num_k_heads + d.head / p.heads_ratio, sizeof(KeyImage), full);
-    bulk_copy(smem_u32(&st.pair), p.pairs + d.place * p.num_v_heads + d.head, sizeof(PairImage), full);
+    const PairImage* pair = p.pairs + d.place * p.num_v_heads + d.head;
+    bulk_copy(smem_u32(&st.pair), &pair->main, sizeof(PairMain), full);
+#pragma unroll
+    for (int col = 0; col < 3; ++col) {  // a column's blocks below its diagonal one
+      bulk_copy(smem_u32(&st.t_lo[tri_block(col + 1, col)]), &pair->t_lo[256 * below_block(col + 1, col)], (3 - col) * 512, full);
+    }
   }
   // Rows of no token are zeros: their beta is 0, but 0 times what lies there need not be 0.
   load_rows<kVec, kMoveThreads>(p.qkv + d.token0 * p.qkv_row + (2 * p.num_k_heads + d.head) * kDim, p.qkv_row, d.row_lo,
                                 d.row_hi, reinterpret_cast<uint16_t*>(st.v), tid,
                                 [](int row, int col) { return row * kVRow + col; });
+}
+
+// The lo terms of a stage's T and P from what their image has of them, and zeros where T's were, by the moving threads.  The
+// upper right core matrices of diagonal blocks of t_lo and p_lo are zeros from the start and stay so.
+__device__ __forceinline__ void unpack_chunk(Stage& st, int tid) {
+  const int warp = tid >> 5, lane = tid & 31;
+  constexpr int kUnits = 8 * (4 * kLowBlocks + 3 * 4);  // rows of 8 elements
+#pragma unroll 1
+  for (int unit = tid; unit < kUnits; unit += kMoveThreads) {
+    int at = 256 * below_place(unit >> 5) + 8 * (unit & 31);
+    if (unit >= 32 * kLowBlocks) {
+      const int diagonal = unit - 32 * kLowBlocks, block = diagonal / 24, row = diagonal - 24 * block;
+      at = tri_block(block, block) + 8 * row + (row >= 8 ? 64 : 0);
+    }
+    const uint2 b = *reinterpret_cast<const uint2*>(&st.pair.p_lo[8 * unit]);
+    const uint4 h = *reinterpret_cast<const uint4*>(&st.pair.p_hi[at]);
+    *reinterpret_cast<uint4*>(&st.p_lo[at]) =
+        make_uint4(lo_terms(h.x, __byte_perm(b.x, 0, 0x4140)), lo_terms(h.y, __byte_perm(b.x, 0, 0x4342)),
+                   lo_terms(h.z, __byte_perm(b.y, 0, 0x4140)), lo_terms(h.w, __byte_perm(b.y, 0, 0x4342)));
+  }
+  if (warp >= kMoveThreads / 32 - 4) {
+    const int w = warp & 3, g = lane >> 2, t = lane & 3;
+    const uint32_t from = core_addr(st.pair.t_hi, lane) + 2 * tri_block(w, w);
+    uint32_t m[4], turned[4];
+    ldsm4(from, m);
+    ldsm4_t(from, turned);
+    __syncwarp();
+    const uint32_t below = 2 * t + 1 < g ? 0xffffffffu : 2 * t < g ? 0xffffu : 0u;
+    const uint32_t upto = 2 * t + 1 <= g ? 0xffffffffu : 2 * t <= g ? 0xffffu : 0u;
+    const int at = tri_block(w, w) + core(g, 2 * t);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(&st.pair.t_hi[at]);
+    uint32_t* lo = reinterpret_cast<uint32_t*>(&st.t_lo[at]);
+    lo[0] = turned[0] & below;
+    lo[64] = turned[1];  // lower left
+    lo[96] = turned[3] & below;
+    hi[0] = m[0] & upto;
+    hi[32] = 0;
+    hi[96] = m[3] & upto;
+  }
 }
 
 // The chunk's gate rows, which only the moving threads read, when the ones before have been used.
@@ -1093,16 +1226,16 @@ __device__ __forceinline__ void gather_outputs(ChainSmem& s, const Stage& st, in
   }
 }
 
-// Gated RMSNorm of the output tile.  A warp takes two rows at a time, 16 lanes and twice four values per lane each.
-// The loop stays rolled: the chain's warps run through so much straight code that the instruction cache is what
-// they compete for.
+// Gated RMSNorm of the output tile.  A warp takes two rows at a time, 16 lanes and twice four values per lane each, and
+// two such turns are unrolled, no more: the chain's warps run through so much straight code that the instruction cache is
+// what they compete for.
 template <bool kVec>
 __device__ __forceinline__ void store_outputs(const PrefillArgs& p, const ChainSmem& s, const Stage& st, const Work& d,
                                               const float2 (&wt)[4], int tid) {
   const int part = tid & 15;
   const bool stop = s.stop != 0 || d.quiet;
   __nv_bfloat16* out = p.out + (d.token0 * p.num_v_heads + d.head) * kDim + 4 * part;
-#pragma unroll 1
+#pragma unroll 2
   for (int i = tid >> 4; i < kChunk; i += kMoveThreads / 16) {
     float2 o[2][2], sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -1215,8 +1348,8 @@ __device__ __forceinline__ void store_split(const float (&x)[kTiles][4], int fir
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const float(&f)[4] = x[first + 2 * ks + m];
-      split(mul2(make_float2(f[0], f[1]), make_float2(up0, up0)), hi[ks][2 * m], lo[ks][2 * m]);
-      split(mul2(make_float2(f[2], f[3]), make_float2(up1, up1)), hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
+      split_masked(mul2(make_float2(f[0], f[1]), make_float2(up0, up0)), hi[ks][2 * m], lo[ks][2 * m]);
+      split_masked(mul2(make_float2(f[2], f[3]), make_float2(up1, up1)), hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
     }
   }
   tmem_store(hi_at, hi);
@@ -1238,64 +1371,64 @@ struct StateWarp {
   float S[16][4];  // rows v0 + g, v0 + g + 8; columns 8n + 2t, + 1
   uint32_t phase;
   bool dead;
+  bool issuer;  // issues what the state waits for
+  bool reader;  // issues S q
 };
 
-// The products of one chunk, issued by one warp.  Everything here is a constant (the stage is a template argument
-// and shared memory starts at a known address), so operands are immediates: with descriptors from registers a
-// product of 32 cycles (N = 64) was issued every 46, in a rolled loop every 90.
 extern __shared__ __align__(1024) unsigned char chain_raw[];
 
-template <int kStage>
+// The products of one chunk.  Three warps issue them, since a warp issues one every 30 to 45 cycles whatever its size: one
+// state warp those that the state waits for, another one S q beside T R, and a moving warp P u when the chunk is done.  All by
+// the first, the 28 products that only the outputs need took 750 cycles a chunk.
 struct Products {
-  static __device__ __forceinline__ const Stage& stage() { return reinterpret_cast<ChainSmem*>(chain_raw)->stage[kStage]; }
+  const Stage& st;
+  uint32_t elected;
+
+  __device__ __forceinline__ explicit Products(const Stage& stage) : st(stage), elected(elect_lane()) { tmem_after(); }
   static __device__ __forceinline__ uint32_t done(int i) { return smem_u32(&reinterpret_cast<ChainSmem*>(chain_raw)->done[i]); }
 
-  // Y = S k~, two terms.
-  static __device__ __forceinline__ void state_keys(uint32_t elected) {
-    const uint64_t k = tile_desc(smem_u32(stage().kq));
+  // D = S x~, two terms, for k~ or q~.
+  __device__ __forceinline__ void of_state(uint32_t d, const __half* tile, uint32_t bar) const {
+    const uint64_t b = tile_desc(smem_u32(tile));
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i) {  // k-steps of lo, then of hi
       const uint32_t ks = i & 7;
-      umma(elected, kTmemY, kTmemS + 64 - 8 * (i & 8) + 8 * ks, k + ((ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2),
+      umma(elected, d, kTmemS + 64 - 8 * (i & 8) + 8 * ks, b + ((ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2),
            mma_shape(64, false), i > 0);
     }
-    umma_commit(elected, done(0));
+    umma_commit(elected, bar);
   }
 
-  // U = T R (the product of the two lo terms is below fp32's last bit), then O = S q~ (hi term), which nobody waits
-  // for yet.  T's column block ks starts at row block ks.
-  static __device__ __forceinline__ void corrections(uint32_t elected) {
-    const uint64_t t_hi = tri_desc(smem_u32(stage().pair.t_hi)), t_lo = tri_desc(smem_u32(stage().pair.t_lo));
+  // D = X M for a triangle M, two terms each (the product of the two lo terms is below fp32's last bit).  M's column block
+  // ks starts at row block ks.
+  __device__ __forceinline__ void of_triangle(uint32_t d, uint32_t x_hi, uint32_t x_lo, const __half* m_hi, const __half* m_lo,
+                                              uint32_t bar) const {
+    const uint64_t b_hi = tri_desc(smem_u32(m_hi)), b_lo = tri_desc(smem_u32(m_lo));
 #pragma unroll
     for (uint32_t ks = 0; ks < 4; ++ks) {  // small terms first in each column block
       const uint32_t at = 2 * tri_block(ks, ks) >> 4, shape = mma_shape(64 - 16 * ks, false);
-      umma(elected, kTmemTr + 16 * ks, kTmemR + 8 * ks, t_lo + at, shape, ks > 0);
-      umma(elected, kTmemTr + 16 * ks, kTmemR + 32 + 8 * ks, t_hi + at, shape, true);
-      umma(elected, kTmemTr + 16 * ks, kTmemR + 8 * ks, t_hi + at, shape, true);
+      umma(elected, d + 16 * ks, x_hi + 8 * ks, b_lo + at, shape, ks > 0);
+      umma(elected, d + 16 * ks, x_lo + 8 * ks, b_hi + at, shape, true);
+      umma(elected, d + 16 * ks, x_hi + 8 * ks, b_hi + at, shape, true);
     }
-    umma_commit(elected, done(0));
-    const uint64_t q = tile_desc(smem_u32(stage().kq + kHalf));
-#pragma unroll
-    for (uint32_t ks = 0; ks < 8; ++ks) {
-      umma(elected, kTmemO, kTmemS + 8 * ks, q + ((ks >> 2) * (2 * kKeyHalf >> 4) + (ks & 3) * 2), mma_shape(64, false),
-           ks > 0);
-    }
+    umma_commit(elected, bar);
   }
 
-  // dS = (k_out u) k~, two terms, then P u, which completes the outputs.
-  static __device__ __forceinline__ void update(uint32_t elected) {
-    const uint64_t k = tile_desc(smem_u32(stage().kq)), p = tri_desc(smem_u32(stage().pair.p));
+  __device__ __forceinline__ void state_keys() const { of_state(kTmemY, st.kq, done(0)); }
+  __device__ __forceinline__ void state_queries() const { of_state(kTmemO, st.kq + kHalf, done(2)); }
+  __device__ __forceinline__ void corrections() const {
+    of_triangle(kTmemTr, kTmemR, kTmemR + 32, st.pair.t_hi, st.t_lo, done(0));
+  }
+  __device__ __forceinline__ void within() const { of_triangle(kTmemPu, kTmemU, kTmemUlo, st.pair.p_hi, st.p_lo, done(1)); }
+
+  // dS = (k_out u) k~, two terms.
+  __device__ __forceinline__ void update() const {
+    const uint64_t k = tile_desc(smem_u32(st.kq));
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {  // k-steps of lo, then of hi
       umma(elected, kTmemDs, kTmemW + 32 - 8 * (i & 4) + 8 * (i & 3), k + (i & 3) * (2048 >> 4), mma_shape(128, true), i > 0);
     }
     umma_commit(elected, done(0));
-#pragma unroll
-    for (uint32_t ks = 0; ks < 4; ++ks) {
-      umma(elected, kTmemPu + 16 * ks, kTmemU + 8 * ks, p + (2 * tri_block(ks, ks) >> 4), mma_shape(64 - 16 * ks, false),
-           ks > 0);
-    }
-    umma_commit(elected, done(1));
   }
 };
 
@@ -1305,26 +1438,30 @@ struct Products {
 //
 // With kLast, the chunk's last ones, the issuing warp also says whether the chunk's state may be stored.  `stop` may be set
 // at any moment, by the moving threads too: were every warp to read it, a slot could take some warps' rows alone.
+//
+// S q, which reads S where the next chunk's goes, is over with the chunk, too: its issuer waits for it here.
 template <bool kLast = false>
-__device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, bool issuer, uint64_t limit_ns) {
-  if (issuer) {
+__device__ __forceinline__ void wait_products(StateWarp& x, ChainSmem& s, uint64_t limit_ns) {
+  if (x.issuer) {
     wait_done(smem_u32(&s.done[0]), x.phase, s, x.dead, limit_ns);
     x.phase ^= 1;
     if constexpr (kLast) s.keep = s.stop == 0;
+  }
+  if (kLast && x.reader) {
+    wait_done(smem_u32(&s.done[2]), x.phase, s, x.dead, limit_ns);
+    x.phase ^= 1;
   }
   bar_state();
   tmem_after();
 }
 
-// One chunk.  `tmem` carries this warp's lanes; one warp (`issuer`) issues the products.  `taken` returns when
-// the outputs of the chunk before have left TMEM.
+// One chunk.  `tmem` carries this warp's lanes.  `taken` returns when the outputs of the chunk before have left TMEM.
 //
-// Parity waits are sound because the warp that waits on a barrier has seen a phase before the next one can begin:
-// done[0] has one warp that both commits and waits, and done[1]'s next commit comes after `taken`, which the
-// waiting threads release.
+// Parity waits are sound because the warp that waits on a barrier has seen a phase before the next one can begin: each
+// has one warp that both commits and waits.
 template <typename Taken>
 __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stage, uint32_t tmem, int v0, int lane,
-                                            bool issuer, uint64_t limit_ns, Taken taken) {
+                                            uint64_t limit_ns, Taken taken) {
   const int g = lane >> 2, t = lane & 3;
   const Stage& st = s.stage[stage];
 
@@ -1336,18 +1473,10 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   tmem_stored();
   tmem_before();
   bar_state();
-  if (issuer && !x.dead) {
-    tmem_after();
-    const uint32_t elected = elect_lane();
-    if (stage == 0) {
-      Products<0>::state_keys(elected);
-    } else {
-      Products<1>::state_keys(elected);
-    }
-  }
+  if (x.issuer && !x.dead) Products(st).state_keys();
 
   // R = beta (v - k_in Y).
-  wait_products(x, s, issuer, limit_ns);
+  wait_products(x, s, limit_ns);
   float Y[8][4];
   tmem_load(tmem + kTmemY, Y);
   const uint32_t v_base =
@@ -1383,30 +1512,22 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
   tmem_stored();
   tmem_before();
   bar_state();
-  // U = T R (the product of the two lo terms is below fp32's last bit).  T's column block ks starts at row
-  // block ks.
-  if (issuer && !x.dead) {
-    tmem_after();
-    const uint32_t elected = elect_lane();
-    if (stage == 0) {
-      Products<0>::corrections(elected);
-    } else {
-      Products<1>::corrections(elected);
-    }
-  }
+  // U = T R, and S q beside it.
+  if (x.issuer && !x.dead) Products(st).corrections();
+  if (x.reader && !x.dead) Products(st).state_queries();
 
-  // u, and k_out u in two terms.  The largest k_out is in [1, 2), so u's row scale serves both.
-  wait_products(x, s, issuer, limit_ns);
+  // k_out u, in two terms.  The largest k_out is in [1, 2), so u's row scale serves both.
+  wait_products(x, s, limit_ns);
   tmem_load(tmem + kTmemTr, Y);
   const float r_down0 = down0, r_down1 = down1;
   scale_rows(Y, up0, down0, up1, down1);
   const float w0 = r_down0 * down0, w1 = r_down1 * down1;
   if (t == 0) {
-    s.u_down[v0 + g] = w0 * st.pair.p_scale;
-    s.u_down[v0 + g + 8] = w1 * st.pair.p_scale;
+    s.u_down[v0 + g] = w0 * st.pair.p_scale();
+    s.u_down[v0 + g + 8] = w1 * st.pair.p_scale();
   }
   {
-    uint32_t hi[4][4];
+    uint32_t hi[4][4], lo[4][4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
@@ -1414,36 +1535,31 @@ __device__ __forceinline__ void chain_chunk(StateWarp& x, ChainSmem& s, int stag
         float(&f)[4] = Y[2 * ks + m];
         const float2 u0 = mul2(make_float2(f[0], f[1]), make_float2(up0, up0));
         const float2 u1 = mul2(make_float2(f[2], f[3]), make_float2(up1, up1));
-        hi[ks][2 * m] = pack_half(u0.x, u0.y);
-        hi[ks][2 * m + 1] = pack_half(u1.x, u1.y);
+        f[0] = u0.x;
+        f[1] = u0.y;
+        f[2] = u1.x;
+        f[3] = u1.y;
         const float2 kout = *reinterpret_cast<const float2*>(&st.pair.k_out[16 * ks + 8 * m + 2 * t]);
-        const float2 k0 = mul2(u0, kout), k1 = mul2(u1, kout);
-        f[0] = k0.x;
-        f[1] = k0.y;
-        f[2] = k1.x;
-        f[3] = k1.y;
+        split_masked(mul2(u0, kout), hi[ks][2 * m], lo[ks][2 * m]);
+        split_masked(mul2(u1, kout), hi[ks][2 * m + 1], lo[ks][2 * m + 1]);
       }
     }
-    tmem_store(tmem + kTmemU, hi);
+    tmem_store(tmem + kTmemW, hi);
+    tmem_store(tmem + kTmemW + 32, lo);
   }
-  store_split(Y, 0, 1.0f, 1.0f, tmem + kTmemW, tmem + kTmemW + 32);
   tmem_stored();
   tmem_before();
   bar_state();
-  if (issuer && !x.dead) {
-    tmem_after();
-    const uint32_t elected = elect_lane();
-    if (stage == 0) {
-      Products<0>::update(elected);
-    } else {
-      Products<1>::update(elected);
-    }
-  }
+  if (x.issuer && !x.dead) Products(st).update();
+  // u, in two terms, for P u, while dS is at work.
+  store_split(Y, 0, 1.0f, 1.0f, tmem + kTmemU, tmem + kTmemUlo);
+  tmem_stored();
+  tmem_before();
   // S <- decay S + dS, one fp32 fused multiply-add per element.
-  const float2 decay = make_float2(st.pair.decay, st.pair.decay);
-  const float k0 = w0 * st.pair.k_scale, k1 = w1 * st.pair.k_scale;
+  const float2 decay = make_float2(st.pair.decay(), st.pair.decay());
+  const float k0 = w0 * st.pair.k_scale(), k1 = w1 * st.pair.k_scale();
   const float2 w02 = make_float2(k0, k0), w12 = make_float2(k1, k1);
-  wait_products<true>(x, s, issuer, limit_ns);
+  wait_products<true>(x, s, limit_ns);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     tmem_load(tmem + kTmemDs + 64 * half, Y);
@@ -1603,25 +1719,37 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int tid = threadIdx.x;
     const auto full = [&](int stage) { return smem_u32(&s.full[stage]); };
-    // A stage is handed over when its copies have landed: every thread waits for its own, warp 0 for the bulk
-    // copies.
+    // A stage is handed over when its copies have landed (every thread waits for its own, one warp for the bulk
+    // copies) and its second terms are unpacked.
     uint32_t landed = 0;
     bool late = false;
     uint32_t owed = 0, owed_parity = 0;  // the barrier of copies that a wait ran out for
     const auto hand_over = [&](int stage, bool chunk) {
       cp_async_wait_groups<1>();  // but not for the gates, which were asked for last
-      if (warp == 0 && chunk) {
-        const uint32_t parity = (landed >> stage) & 1;
-        const bool before = late;
-        wait_done(full(stage), parity, s, late, p.wait_ns);
-        if (late && !before) {
-          owed = full(stage);
-          owed_parity = parity;
+      if (chunk) {
+        if (warp == kCopyWarp) {
+          const uint32_t parity = (landed >> stage) & 1;
+          const bool before = late;
+          wait_done(full(stage), parity, s, late, p.wait_ns);
+          if (late && !before) {
+            owed = full(stage);
+            owed_parity = parity;
+          }
+          landed ^= 1u << stage;
         }
-        landed ^= 1u << stage;
+        bar_move();  // they have landed for everybody
+        unpack_chunk(s.stage[stage], tid);
+        // Products read what was written here, and later copies write over it, both through the async proxy.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       bar_arrive(kBarFull + stage);
     };
+    {  // the core matrices that unpack_chunk leaves alone: 32 words in each of two stages' eight diagonal blocks
+      Stage& st = s.stage[tid >> 7];
+      const int block = (tid >> 5) & 3, at = tri_block(block, block) + 64 + 2 * lane;
+      *reinterpret_cast<uint32_t*>(&st.t_lo[at]) = 0;
+      *reinterpret_cast<uint32_t*>(&st.p_lo[at]) = 0;
+    }
     if (tid == 0) {
       for (int i = 0; i < 2; ++i) barrier_init(full(i));
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1659,14 +1787,18 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     uint32_t phase = 0;
     bool dead = false;
     for (int stage = 0;; stage ^= 1) {
+      // Without this the compiler turns the loop around its first test and keeps code twice, and the chain's warps compete
+      // for the instruction cache: 884 us instead of 777 (one prompt of 16,384 tokens).
+      asm volatile("" ::: "memory");
       Stage& st = s.stage[stage];
       const Work d = st.work;
       if (d.kind == kWorkEnd) break;
       const bool refill = more;
-      if (refill && tid == 0) next_work<kSplit>(p, s.at, s.upcoming);  // while the chain is at work
-      __syncwarp();
       bar_sync(kBarChunkDone);
-      if (warp == 0) {
+      if (refill && tid == 32 * kTakeWarp) next_work<kSplit>(p, s.at, s.upcoming);  // while P u is at work
+      __syncwarp();
+      if (warp == 0) {  // P u, and with it the outputs are whole
+        if (!dead) Products(st).within();
         wait_done(smem_u32(&s.done[1]), phase, s, dead, p.wait_ns);
         phase ^= 1;
       }
@@ -1702,28 +1834,29 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
     const int g = lane >> 2, t = lane & 3;
     // A warp reaches the TMEM lanes of its number mod 4; two warps share them, 16 lanes each.
     const int v0 = 32 * (warp & 3) + 16 * ((warp - kStateWarp) >> 2);
-    const bool issuer = warp == kStateWarp;
-    if (issuer) {
+    StateWarp x;
+    x.phase = 0;
+    x.dead = false;
+    x.issuer = warp == kStateWarp;
+    x.reader = warp == kStateWarp + 1;
+    if (x.issuer) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)),
                    "n"(kTmemColumns)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
       if (lane == 0) {
-        for (int i = 0; i < 2; ++i) barrier_init(smem_u32(&s.done[i]));
-        barrier_init(smem_u32(&s.drained));
+        for (int i = 0; i < 3; ++i) barrier_init(smem_u32(&s.done[i]));
+        barrier_init(smem_u32(&s.drained), kIssuers);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       }
       __syncwarp();
       tmem_before();
     }
     grid_dependency_wait();
-    if (issuer && lane == 0) s.stop = p.pass == 0 ? 0 : static_cast<int>(p.next[2]);  // ran out in the first pass
+    if (x.issuer && lane == 0) s.stop = p.pass == 0 ? 0 : static_cast<int>(p.next[2]);  // ran out in the first pass
     __syncthreads();  // the barriers are there
     tmem_after();
     const uint32_t tmem = static_cast<uint32_t>(v0) << 16;
-    StateWarp x;
-    x.phase = 0;
-    x.dead = false;
     for (int64_t n = 0;; ++n) {
       const int stage = static_cast<int>(n & 1);
       bar_sync(kBarFull + stage);
@@ -1772,7 +1905,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
           }
         }
       }
-      chain_chunk(x, s, stage, tmem, v0, lane, issuer, p.wait_ns, [&] {
+      chain_chunk(x, s, stage, tmem, v0, lane, p.wait_ns, [&] {
         if (n >= 1) {
           bar_sync(kBarTaken);
           tmem_after();
@@ -1801,10 +1934,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) gdn_prefill_chain_kernel(con
   tmem_before();
   __syncthreads();
   if (threadIdx.x == 0 && s.stop != 0) p.next[2] = 1;
+  // Products that nobody waited for may still read the stages and write TMEM.
+  const bool drain = s.stop != 0;
+  if (drain && (warp == 0 || warp == kStateWarp || warp == kStateWarp + 1)) umma_commit(elect_lane(), smem_u32(&s.drained));
   if (warp == kStateWarp) {
     tmem_after();
-    if (s.stop != 0) {  // products that nobody waited for may still read the stages and write TMEM
-      umma_commit(elect_lane(), smem_u32(&s.drained));
+    if (drain) {
       bool over = false;
       wait_done(smem_u32(&s.drained), 0, s, over, p.wait_ns);
     }

@@ -53,5 +53,5 @@ def test_the_state_warps_store_a_state_together_or_not_at_all():
     wait = text[text.index("void wait_products("):]
     wait = wait[:wait.index("\n}")]
     decided, joined = wait.index("s.keep = s.stop == 0;"), wait.index("bar_state();")
-    assert wait.index("if (issuer)") < decided < joined
+    assert wait.index("if (x.issuer)") < decided < joined
     assert len(re.findall(r"s\.keep\b", text)) == 2, "one place writes it, one reads it"
