@@ -21,6 +21,13 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
+// Within a few ulp, 0 of 0.
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // z sigmoid(z) in two special-function operations, within a few fp32 ulps (far below bf16's rounding).
 __device__ __forceinline__ float silu_fast(float z) { return z * rcp_fast(1.0f + exp2_fast(-1.44269504f * z)); }
 

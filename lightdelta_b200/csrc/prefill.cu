@@ -12,8 +12,8 @@
 // matrix, and only the state passes from chunk to chunk.
 //
 // Precision.  The state and every sum stay in fp32.  Matrix instructions take fp16 operands with
-// fp32 accumulation.  q and k rows are bf16 and become fp16 exactly after scaling by a power of two
-// per row (which the fp32 factors fk, fq undo).  All other operands (S, R, u, T, L, P) go in as two fp16
+// fp32 accumulation.  q and k rows are bf16 and become fp16 after scaling by a power of two per row (which
+// the fp32 factors fk, fq undo), exactly but for elements below 2^-30 of their row's largest.  All other operands (S, R, u, T, L, P) go in as two fp16
 // terms, hi + lo, 22 bits together (P 19), after scaling each state row by a power of two, so the state
 // follows the fp32 recurrence to under 1e-6, and so do the outputs until they are rounded to bf16.  (With
 // one term for S q and P u, 11 bits, one output in ten was rounded elsewhere, and where a query is nearly
@@ -518,7 +518,7 @@ struct PairSmem {
   };
   float g_hi[kGroup][kChunk], g_lo[kGroup][kChunk], beta[kGroup][kChunk];
   float fk[kChunk], fq[kChunk];
-  float fk_unit[kChunk], fq_unit[kChunk];  // divided by their largest's power of two
+  float fk_unit[kChunk], fq_unit[kChunk];  // divided by the power of two of the longest normalised row
   float fk_power, fq_power;
 
   __device__ __forceinline__ __half* kq() { return reinterpret_cast<__half*>(tiles); }
@@ -538,6 +538,10 @@ struct Blocks {
   __device__ __forceinline__ int ib(int b) const { return b == 0 ? w : row; }
   __device__ __forceinline__ int jb(int b) const { return b == 0 ? w : col + b - 1; }
 };
+
+// Rows' products divided by the longest lengths' powers of two are below 4, and with q's 128^-1/2 below 0.36: times this
+// they fill fp16's range, and P's terms reach down to 2^-37 of the longest rows' product.
+constexpr float kPUp = 16384.0f;
 
 // L's blocks below the diagonal ones, row by row.
 __host__ __device__ constexpr int low_block(int ib, int jb) { return 256 * (ib * (ib - 1) / 2 + jb); }
@@ -563,8 +567,9 @@ __device__ __forceinline__ void load_rows(const __nv_bfloat16* base, int64_t row
   }
 }
 
-// Scales one row from bf16 to fp16 in place, by one thread: exact, since a power of two brings the row's
-// largest magnitude to [1, 2).  Returns that power's inverse.
+// Scales one row from bf16 to fp16 in place, by one thread: a power of two brings the row's largest magnitude to
+// [2^13, 2^14), so that elements down to 2^-30 of it keep bf16's eight bits above fp16's smallest step, 2^-24, and sums
+// of 128 products of two rows stay below 2^35.  Returns that power's inverse.
 __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
   uint16_t* row = tile + i * 64;
   __nv_bfloat162 top = __floats2bfloat162_rn(0.0f, 0.0f);  // the largest magnitudes so far of even and odd columns
@@ -576,8 +581,8 @@ __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
     for (int n = 0; n < 4; ++n) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[n])));
   }
   const uint32_t top2 = *reinterpret_cast<const uint32_t*>(&top);  // bf16 magnitudes order as integers
-  const int e = min(max(static_cast<int>(max(top2 >> 16, top2 & 0xffffu) >> 7), 1), 253);
-  const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
+  const int e = min(max(static_cast<int>(max(top2 >> 16, top2 & 0xffffu) >> 7), 14), 253);
+  const float down = __uint_as_float(static_cast<uint32_t>(267 - e) << 23);  // 2^(140 - e)
 #pragma unroll
   for (int piece = 0; piece < kDim / 8; ++piece) {
     uint4* at = reinterpret_cast<uint4*>(row + (piece >> 3) * kKeyHalf + (((piece & 7) ^ (i & 7)) << 3));
@@ -591,7 +596,7 @@ __device__ __forceinline__ float scale_row(uint16_t* tile, int i) {
     }
     *at = make_uint4(y[0], y[1], y[2], y[3]);
   }
-  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
 }
 
 // The power of two at or below the largest of 64 positive floats, of which each lane of a warp has two.  Operands that
@@ -701,8 +706,11 @@ __device__ __forceinline__ void row_products(PairSmem& s, const Blocks& mine, in
     if (t == g / 2) {
       const int i = 16 * mine.w + g + 8 * half;
       const float up_k = s.fk[i], up_q = s.fq[i];
-      s.fk[i] = up_k * rsqrtf(k2 * up_k * up_k + 1e-6f);
-      s.fq[i] = up_q * rsqrtf(q2 * up_q * up_q + 1e-6f);
+      const float fk = up_k * rsqrtf(k2 * up_k * up_k + 1e-6f), fq = up_q * rsqrtf(q2 * up_q * up_q + 1e-6f);
+      s.fk[i] = fk;
+      s.fq[i] = fq;
+      s.fk_unit[i] = fk * sqrt_fast(k2);  // the normalised row's length, for now
+      s.fq_unit[i] = fq * sqrt_fast(q2);
     }
   }
 }
@@ -722,7 +730,7 @@ __device__ __forceinline__ void row_factors(const PrefillArgs& p, PairSmem& s, i
   if (i == kChunk - 1) {
     image.decay() = in;
     image.k_scale() = power;
-    image.p_scale() = s.fk_power * s.fq_power;
+    image.p_scale() = s.fk_power * s.fq_power * (1.0f / kPUp);
   }
 }
 
@@ -742,7 +750,7 @@ __device__ __forceinline__ void decayed_pairs(const PrefillArgs& p, PairSmem& s,
       g_hi[half] = s.g_hi[place][i];
       g_lo[half] = s.g_lo[place][i];
       row_k[half] = s.beta[place][i] * s.fk[i] * s.fk_power;
-      row_q[half] = p.q_scale * s.fq_unit[i];
+      row_q[half] = kPUp * p.q_scale * s.fq_unit[i];
     }
     const int to_p = tri_block(mine.ib(b), mine.jb(b)) + core(g, 2 * t);
     const int to_byte = (b > 0 ? 256 * below_block(mine.row, mine.jb(b)) : 256 * kLowBlocks + 192 * mine.w) + core(g, 2 * t);
@@ -1003,10 +1011,9 @@ __global__ void __launch_bounds__(kPairThreads, 4) gdn_prefill_pairs_kernel(cons
   if (w < 2) {
     const float* f = w == 0 ? s.fk : s.fq;
     float* unit = w == 0 ? s.fk_unit : s.fq_unit;
-    const float x = f[lane], y = f[lane + 32];
-    const float power = largest_power(x, y), down = inverse_power(power);
-    unit[lane] = x * down;
-    unit[lane + 32] = y * down;
+    const float power = largest_power(unit[lane], unit[lane + 32]), down = inverse_power(power);
+    unit[lane] = f[lane] * down;
+    unit[lane + 32] = f[lane + 32] * down;
     if (lane == 0) (w == 0 ? s.fk_power : s.fq_power) = power;
   }
   __syncthreads();

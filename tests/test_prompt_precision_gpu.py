@@ -102,6 +102,38 @@ def test_queries_nearly_orthogonal_to_what_the_state_holds(cosine, pool):
     check_states_closely(case.state, after)
 
 
+@pytest.mark.parametrize("power", [12, 18, 22])
+def test_small_channels_beside_a_large_one(power):
+    """One channel of the keys is 2^power times the others and the queries leave it out, so they read the columns that
+    the small ones made.  bf16's 8 bits of those are kept (q, k as one fp16 each, 2^-24 the smallest step, the row's
+    largest at 2^13 or more), P's entries, 2^-power, are good to 2^-25 of a range of 2^11, 2^(power - 36) = 2^-14 at 22,
+    and the sums of 127 terms to 2^-17: 2^-13 of sum |q| |k| |u| over the small channels, and bf16's half step."""
+    case = Prompt([5, 3], [0, 0], h=1, hv=2, decay=1e-3, seed=62)
+    case.qkv[:, DIM] = 2.0 ** power * torch.sign(case.qkv[:, DIM].float()).bfloat16()
+    case.qkv[:, 0] = 0
+    case.b[:] = case.b * 0.3 - 1  # steps of about a quarter, so that tokens do not cancel one another
+    want, _, _ = case.expect()
+    case.run()
+    torch.cuda.synchronize()
+    qkv, f64 = case.qkv.cpu().double(), lambda t: t.cpu().double()
+    q, k = qkv[:, :DIM], qkv[:, DIM:2 * DIM]
+    q, k = (x / ((x * x).sum(-1, keepdim=True) + 1e-6).sqrt() for x in (q, k))
+    q = q * DIM ** -0.5
+    gate = f64(case.gate)
+    shape = (f64(case.weight) * gate * torch.sigmoid(gate)).abs()
+    v = qkv[:, 2 * DIM:].view(-1, 2, DIM)
+    cu = case.cu.tolist()
+    for r in range(2):
+        for t in range(cu[r], cu[r + 1]):
+            # |u| is below twice the largest v so far of its row (steps below 1, keys of one direction).
+            u = 2 * v[cu[r]:t + 1].abs().amax(0)
+            size = u * (q[t].abs() * k[cu[r]:t + 1].abs()).sum()
+            o = want[t] / (shape[t] + 1e-300)  # o rstd; rstd is at most 1e3
+            through = (size + size.amax(-1, keepdim=True) * o.abs()) * 1e3 * shape[t]
+            off = (f64(case.out[t]) - want[t]).abs() / (2.0 ** -8 * want[t].abs() + 2.0 ** -13 * through)
+            assert off.max() <= 1.0, f"outputs {off.max():.2f} times their bound off"
+
+
 @pytest.mark.parametrize("lens,contexts,heads,block", [
     ([64], [0], (1, 1), 64),
     ([130, 1, 64, 63, 200, 9], [64, 63, 64, 65, 57, 5], (1, 2), 64),
