@@ -398,7 +398,10 @@ int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a
 
 /*
  * Bytes of device memory that ld_prefill needs as `workspace` (128-byte aligned) for a call of these sizes:
- * about 16 KiB per token at 16 key and 32 value heads, and up to 15 MiB for prompts in pieces.  It is written and read by the call alone, needs no
+ * 32 KiB per key head and 16.25 KiB per value head for each of min(n_tokens, n_tokens / 64 + 2 n_requests)
+ * chunks (at 16 key and 32 value heads about 16 KiB per token and, where requests have more than a few tokens,
+ * 2 MiB per request: 0.39 GB for 128 requests of 7,000 tokens in all, 4.3 GB for 4,096 of one token each), 4
+ * bytes per request, and up to 15 MiB for prompts in pieces.  It is written and read by the call alone, needs no
  * clearing, and may be used again by work behind the call on the same stream; calls that may overlap (other
  * streams, graphs that run side by side) need one each.  Negative: -LD_ERR_INVALID.
  */

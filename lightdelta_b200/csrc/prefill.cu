@@ -199,10 +199,11 @@ struct PrefillArgs {
   uint32_t extra_tx;  // test only: bytes that a chunk's copies announce beyond what they copy (normally 0)
 };
 
-// Chunk c of request r is kept at place chunk_base(cu[r], r) + c.  A request of n tokens has at most
-// n / 64 + 2 chunks (both ends may be short), so places never overlap, and nobody has to count chunks.
+// Chunk c of request r is kept at place chunk_base(cu[r], r) + c.  A request of n tokens has at most n / 64 + 2 chunks (both
+// ends may be short) and at most n, so places never overlap, and nobody has to count chunks.
 __host__ __device__ __forceinline__ int64_t chunk_base(int64_t first_token, int64_t request) {
-  return first_token / kChunk + 2 * request;
+  const int64_t whole = first_token / kChunk + 2 * request;
+  return first_token < whole ? first_token : whole;
 }
 
 // A request that runs.

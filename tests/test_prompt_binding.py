@@ -1,5 +1,6 @@
 """CPU tests of the ctypes binding of the prompt path: what it hands to the C entry points, with the library faked."""
 
+import random
 from contextlib import contextmanager
 from types import SimpleNamespace
 
@@ -65,3 +66,29 @@ def test_prefill_uses_the_workspace_that_it_is_given(monkeypatch):
     fake = Fake(monkeypatch)
     call(workspace=mine, stream=77)
     assert fake.made == [] and fake.launched == dict(workspace=mine.data_ptr(), size=2000, stream=77)
+
+
+@pytest.mark.parametrize("tokens,requests,h,hv", [(7001, 128, 16, 32), (128, 128, 16, 32), (4096, 4096, 16, 32), (300, 7, 2, 6),
+                                                  (16384, 1, 16, 48), (1, 1, 1, 1)])
+def test_the_workspace_is_what_the_header_says(native, tokens, requests, h, hv):
+    """Room for each chunk that the requests can have: two beyond their whole ones, and never more than tokens."""
+    chunks = min(tokens, tokens // 64 + 2 * requests)
+    least = chunks * (32768 * h + 16640 * hv) + 4 * requests
+    assert least <= native.prefill_workspace(tokens, requests, h, hv) <= least + 256 + 15 * 2 ** 20
+
+
+def test_places_of_chunks_do_not_overlap():
+    """The rule that gives request r of a batch its places, min(first, first // 64 + 2 r) and on, for requests of any
+    lengths that begin anywhere in a chunk; none lies behind what the workspace has room for."""
+    rng = random.Random(5)
+    for _ in range(3000):
+        lens = [rng.choice((0, 0, 1, 1, 2, 3, 63, 64, 65, 130, rng.randrange(500))) for _ in range(rng.randrange(1, 9))]
+        lens += [1] * rng.randrange(4)
+        total, first, end = sum(lens), 0, 0
+        for r, n in enumerate(lens):
+            base = min(first, first // 64 + 2 * r)
+            assert base >= end
+            if n:
+                end = base + (rng.choice((0, 1, 62, 63)) + n + 63) // 64
+            first += n
+        assert end <= min(total, total // 64 + 2 * len(lens))
