@@ -441,7 +441,11 @@ int ld_conv_prefill(const void* x, int64_t x_row_stride, int64_t n_tokens, int64
  *   state_slots[r]      (slot of the block of r's last new token, slot of the block of its last held
  *                       token), 0 where there is no such token.  With them as `indices` and
  *                       accepted = 2, ld_decode takes a one-token request from its held state to its
- *                       new block's slot, across a block's end too;
+ *                       new block's slot, across a block's end too; a request without context has a
+ *                       null source there, which ld_decode answers with zeros (ld_prefill runs it).
+ *                       They are not for ld_conv_update and ld_conv_decode, which read and write the
+ *                       window of one slot, indices' first: the new block's, which nobody has written.
+ *                       ld_conv_prefill takes single tokens from the held window to the new block's;
  *   used[0]             free blocks taken, over all requests.
  * positions and slot_map hold n_tokens entries; those behind the last token are -1.  A token whose
  * block is null (<= 0) has slot -1.
