@@ -382,11 +382,13 @@ int ld_decode_packed_noalloc(const void* qkv, int64_t qkv_row_stride, const void
  * An in-kernel wait that runs out (LD_FAULT_WAIT_TIMEOUT) leaves what its CTA has not stored yet as it
  * was, as in ld_decode.
  *
- * Products take fp16 operands with fp32 sums: two terms each (22 bits) on the way to the state, which
- * so follows the fp32 recurrence to a few 1e-7 of a state row's largest value, and one term (11 bits)
- * for what only reaches the bf16 outputs.  Results do not depend on the order of execution, but their
- * last bits may on n_requests and n_tokens: few long prompts of few heads run in pieces whose states
- * are joined.
+ * Products take fp16 operands, two terms each (22 bits together, 19 where a chunk's tokens read one another),
+ * with fp32 sums, so states follow the fp32 recurrence to a few 1e-7 of a state row's largest value, and outputs
+ * do until they are rounded to bf16, once.  q and k elements below 2^-30 of their row's largest lose bits.
+ * Results do not depend on the order of execution, but their last bits may on n_requests and n_tokens: few long
+ * prompts of few heads run in pieces whose states are joined.
+ *
+ * cu ascends: a request that shares tokens with another gives unspecified outputs and states.
  */
 int ld_prefill(const void* qkv, int64_t qkv_row_stride, const void* a, int64_t a_row_stride, const void* b,
                int64_t b_row_stride, const float* a_log, const void* dt_bias, int dt_bias_dtype, const int32_t* table,
