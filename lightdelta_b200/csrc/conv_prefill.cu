@@ -347,7 +347,7 @@ cudaError_t launch_width(ConvPrefillArgs& args, bool vec, cudaStream_t stream) {
   const int channels = (vec ? kVector : 1) * kThreads;
   const int64_t groups = (args.dim + channels - 1) / channels;
   // A tile's thread reads 3 rows that the tile before reads too, and finds its request and its weights: 24 prompts of
-  // 16,000 tokens in all (8,192 channels) took 108.7 us at 64 tokens per thread, 110.5 at 32.  Smaller batches are
+  // 16,000 tokens in all (8,192 channels) take 98.3 us at 64 tokens per thread, 104.0 at 32.  Smaller batches are
   // spread over the SMs (six CTAs each) before their tiles grow.
   const int64_t work = args.n_tokens * groups;
   args.tile = work >= 64 * 6 * 148 ? 64 : work >= 32 * 4 * 148 ? 32 : 8;

@@ -13,13 +13,13 @@
 //
 // Precision.  The state and every sum stay in fp32.  Matrix instructions take fp16 operands with
 // fp32 accumulation.  q and k rows are bf16 and become fp16 after scaling by a power of two per row (which
-// the fp32 factors fk, fq undo), exactly but for elements below 2^-30 of their row's largest.  All other operands (S, R, u, T, L, P) go in as two fp16
-// terms, hi + lo, 22 bits together (P 19), after scaling each state row by a power of two, so the state
-// follows the fp32 recurrence to under 1e-6, and so do the outputs until they are rounded to bf16.  (With
-// one term for S q and P u, 11 bits, one output in ten was rounded elsewhere, and where a query is nearly
-// orthogonal to what the state holds, or a chunk's keys are all but equal, the gated norm made that a few
-// 1e-3 to 1e-2 of the output; that took 365-382 us for the 24 prompts below.)  G is summed in fp64 and kept
-// as two floats, so differences of large sums stay exact to fp32.
+// the fp32 factors fk, fq undo), exactly but for elements below 2^-30 of their row's largest.  All other
+// operands (S, R, u, T, L, P) go in as two fp16 terms, hi + lo, 22 bits together (P 19), after scaling each
+// state row by a power of two, so the state follows the fp32 recurrence to under 1e-6, and so do the outputs
+// until they are rounded to bf16.  (With one term for S q and P u, 11 bits, one output in ten was rounded
+// elsewhere, and where a query is nearly orthogonal to what the state holds, or a chunk's keys are all but
+// equal, the gated norm made that a few 1e-3 to 1e-2 of the output; that took 377 us for the 24 prompts
+// below.)  G is summed in fp64 and kept as two floats, so differences of large sums stay exact to fp32.
 //
 // Two kernels.  What does not depend on the state is computed first, for all chunks side by side:
 // gdn_prefill_pairs_kernel, one CTA per (chunk, key head), scales q and k, forms their products once for
@@ -33,18 +33,19 @@
 //   dS = u k~            A = k_out u hi, lo        B = the same k~ tile, read MN-major
 // It is one persistent CTA per SM that takes (request, value head) items from a queue, longest first.
 // Eight warps keep the fp32 state in registers, 16 value rows each, in the layout that 16-lane TMEM
-// loads and stores use; between products they scale, split and store the next A operand, and one of them
-// issues.  The other eight copy the next chunk in and normalise and store the chunk before's outputs.
+// loads and stores use; between products they scale, split and store the next A operand, and two of them
+// issue.  The other eight copy the next chunk in, issue P u, and normalise and store the chunk before's outputs.
 //
-// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 365-382 us, 140 in
-// the pairs kernel (43% of issue slots, 12,700 warp instructions a CTA: latency, at the four CTAs per SM
-// that 128 registers allow) and 230 in the chain (7,200 cycles a chunk: products 1,260 and their latency,
-// the rest the four steps between them; 45% of issue slots, 20% of the tensor pipe).  History of the
-// split (and of one prompt of 16,384): one kernel that prepared each chunk inside the chain's CTA, 1,242
-// us (4,878); pairs apart and the chain on mma.sync with the state as its fragments, 555 (1,646); the
-// chain on tcgen05, 430 (1,181); outputs gathered off the chain's path 418, the queue 412, one warp that
-// waits for products 400, issue with constant operands 390 (1,137); the pairs of two heads at a time,
-// blocks dealt out evenly, 374 (1,104); long prompts in pieces (732).
+// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 402-414 us, 124 in
+// the pairs kernel (47% of issue slots, 14,600 warp instructions a CTA: latency, at the four CTAs per SM
+// that 128 registers allow) and 304 in the chain (7,900 cycles a chunk: the four steps between its products,
+// and the moving threads' own loop, which is nearly as long; 46% of issue slots, 24% of the tensor pipe).
+// History of the split (and of one prompt of 16,384): one kernel that prepared each chunk inside the
+// chain's CTA, 1,242 us (4,878); pairs apart and the chain on mma.sync with the state as its fragments, 555
+// (1,646); the chain on tcgen05, 430 (1,181); outputs gathered off the chain's path 418, the queue 412, one
+// warp that waits for products 400, issue with constant operands 390 (1,137); the pairs of two heads at a
+// time, blocks dealt out evenly, 374 (1,104); long prompts in pieces (742); second terms for the outputs
+// 407 (751), of which 30 are what unpacking them takes from the moving threads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -124,8 +125,8 @@ static_assert(sizeof(PairImage) == sizeof(PairMain) + sizeof(PairImage::t_lo), "
 // their states, all at once.  That is three times the work for the middle pieces, in the time of two pieces.
 // With room for `slots` CTAs per value head there are (slots - 1) / 2 middle pieces, and one more of half their length,
 // whose M and B share a CTA, where a slot is left over: 16,384 tokens of one request with 32 value heads (4 slots,
-// 4 pieces, 2 of 3.5 parts of the chain's time) take 732 us, unsplit 1,104; with 4 value heads (16 pieces) 215 instead of
-// 1,010, and 1,600 tokens with 8 value heads 91 instead of 122.
+// 4 pieces, 2 of 3.5 parts of the chain's time) take 751 us, unsplit 1,189; with 4 value heads (16 pieces) 225 instead of
+// 1,085, and 1,600 tokens with 8 value heads 81 instead of 121.
 struct Pieces {
   int count;       // 1: no request is split
   bool half_last;  // the last middle piece has half the length of the others
