@@ -46,3 +46,10 @@ def test_a_first_token_needs_prefill():
     # Two fp32 recurrences, one step: sums of 128 in either, 2 * 2^-17 of the largest value.
     assert (got - want).abs().max() <= 2.0 ** -16 * want.abs().max()
     assert capi.fault_flags() == 0 and out.shape[-1] == DIM
+
+
+@pytest.mark.parametrize("lens,contexts,pad", [([0, 0], [0, 64], 5), ([0], [0], 1), ([0, 3, 0, 0], [7, 64, 0, 64], 2)])
+def test_a_batch_padded_with_empty_requests(lens, contexts, pad):
+    """Rows of a captured batch that hold no request now: nothing is written for them, whatever their contexts say."""
+    case = Prompt(lens, contexts, h=1, hv=2, pad=pad, seed=99)
+    case.check()
