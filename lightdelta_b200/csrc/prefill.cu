@@ -36,7 +36,7 @@
 // loads and stores use; between products they scale, split and store the next A operand, and two of them
 // issue.  The other eight copy the next chunk in, issue P u, and normalise and store the chunk before's outputs.
 //
-// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 402-414 us, 124 in
+// What bounds it: 24 prompts of 16,000 tokens in all, 16 key and 32 value heads, take 400-414 us, 124 in
 // the pairs kernel (47% of issue slots, 14,600 warp instructions a CTA: latency, at the four CTAs per SM
 // that 128 registers allow) and 304 in the chain (7,900 cycles a chunk: the four steps between its products,
 // and the moving threads' own loop, which is nearly as long; 46% of issue slots, 24% of the tensor pipe).
